@@ -84,13 +84,20 @@ def _blocks(x):
     return x.reshape(*x.shape[:-1], n, BLOCK)
 
 
+def _inverse_and_scale(amax):
+    """448 / amax and amax / 448, each a division: with a Python number on one side torch would
+    multiply by a rounded reciprocal."""
+    top = torch.full_like(amax, FP8_MAX)
+    return top / amax, amax / top
+
+
 def _quantize(x):
     """Rows of x (32 bits) in e4m3 with a scale for each 128 elements of a row."""
     b = _blocks(x)
     amax = b.abs().amax(-1).clamp(min=AMAX_FLOOR)
-    q = (b * (FP8_MAX / amax).unsqueeze(-1)).to(torch.float8_e4m3fn)
-    q = q.reshape(*x.shape[:-1], -1)[..., : x.shape[-1]].contiguous()
-    return q, amax / FP8_MAX
+    inverse, scale = _inverse_and_scale(amax)
+    q = (b * inverse.unsqueeze(-1)).to(torch.float8_e4m3fn)
+    return q.reshape(*x.shape[:-1], -1)[..., : x.shape[-1]].contiguous(), scale
 
 
 def _spread(scale, like, dtype):
@@ -104,8 +111,9 @@ def _quantize_weight(w):
     p = torch.nn.functional.pad(w, (0, -k % BLOCK, 0, -n % BLOCK))
     b = p.reshape(p.shape[0] // BLOCK, BLOCK, p.shape[1] // BLOCK, BLOCK)
     amax = b.abs().amax((1, 3)).clamp(min=AMAX_FLOOR)
-    q = (b * (FP8_MAX / amax)[:, None, :, None]).to(torch.float8_e4m3fn)
-    return q.reshape(p.shape)[:n, :k].contiguous(), amax / FP8_MAX
+    inverse, scale = _inverse_and_scale(amax)
+    q = (b * inverse[:, None, :, None]).to(torch.float8_e4m3fn)
+    return q.reshape(p.shape)[:n, :k].contiguous(), scale
 
 
 def _spread_weight(scale, like, dtype):
