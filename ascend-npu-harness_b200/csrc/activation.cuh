@@ -1,0 +1,105 @@
+// GELU (tanh form) and SiLU as device functors, and their derivatives: shared by the elementwise
+// activation and by its checkpointed form.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace hc {
+
+struct ActOp {
+    static constexpr bool kBinary = false;
+    uint32_t act;  // 0 = GELU (tanh form), 1 = SiLU
+    __device__ float apply(float v, float) const {
+        if (act == 0) {
+            const float kSqrt2OverPi = 0.7978845608f;
+            const float kGeluCoeff = 0.044715f;
+            float x3 = __fmul_rn(__fmul_rn(v, v), v);
+            float inner = __fmul_rn(kSqrt2OverPi, __fadd_rn(v, __fmul_rn(kGeluCoeff, x3)));
+            float t = tanhf(inner);
+            return __fmul_rn(__fmul_rn(0.5f, v), __fadd_rn(1.0f, t));
+        }
+        if (v >= 0.0f) {
+            float e = expf(-v);
+            return __fdiv_rn(v, __fadd_rn(1.0f, e));
+        }
+        float e = expf(v);
+        return __fdiv_rn(__fmul_rn(v, e), __fadd_rn(1.0f, e));
+    }
+};
+
+// 16-bit outputs: the same functions through the logistic sigmoid, which needs one exponential
+// and one reciprocal instead of tanhf / expf / IEEE division:
+//   GELU_tanh(x) = 0.5 x (1 + tanh u) = x * sigmoid(2u),  u = sqrt(2/pi) (x + 0.044715 x^3);
+//   SiLU(x) = x * sigmoid(x);  sigmoid(z) = 1 / (1 + 2^(-z log2 e)).
+// With the constants folded into the base-2 exponent, both are x / (1 + 2^y), y = -x (a + b x^2):
+// GELU a = 2 sqrt(2/pi) log2 e, b = 0.044715 a; SiLU a = log2 e, b = 0.  Relative error ~1e-6, far
+// below the rounding of the bf16/fp16 result (2^-9 / 2^-12); the fp32 path (ActOp) keeps the
+// golden's operation order.  y is clamped to 126, so 1 + 2^y stays finite: for x -> -inf the
+// result is x * 2^-126-ish, i.e. 0 after rounding to 16 bits, as the golden gives.
+__device__ __forceinline__ float ex2_ftz(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_ftz(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+struct FastActOp {
+    static constexpr bool kBinary = false;
+    float a, b;  // y = -x (a + b x^2)
+    __host__ static FastActOp make(uint32_t act) {
+        const double log2e = 1.4426950408889634;
+        const double k = 2.0 * 0.7978845608028654 * log2e;  // 2 sqrt(2/pi) log2 e
+        return act == 0 ? FastActOp{static_cast<float>(k), static_cast<float>(0.044715 * k)}
+                        : FastActOp{static_cast<float>(log2e), 0.f};
+    }
+    __device__ float2 apply2(float2 x) const {
+        const float2 w = __ffma2_rn(make_float2(-b, -b), __fmul2_rn(x, x), make_float2(-a, -a));
+        const float2 y = __fmul2_rn(x, w);
+        float2 d = make_float2(ex2_ftz(fminf(y.x, 126.f)), ex2_ftz(fminf(y.y, 126.f)));
+        d = __fadd2_rn(d, make_float2(1.f, 1.f));
+        // MUFU rcp: measured faster here than three Newton steps on the FMA pipe
+        return __fmul2_rn(x, make_float2(rcp_ftz(d.x), rcp_ftz(d.y)));
+    }
+    __device__ float apply(float v, float) const { return apply2(make_float2(v, v)).x; }
+};
+
+// Slope of either activation at x, with act(x) = x s, s = sigmoid(z(x)):
+//   act'(x) = s + x s (1 - s) z'(x)
+//   GELU z = 2 sqrt(2/pi) (x + 0.044715 x^3), z' = 2 sqrt(2/pi) (1 + 0.134145 x^2);  SiLU z = x, z' = 1.
+// With e = exp(-z) and r = 1 / (1 + e): s = r and 1 - s = e r, so neither side of the sigmoid
+// cancels.  e is held below overflow, where r is 0 for every purpose here.
+// x is held to [-16, 16] for GELU and [-200, 200] for SiLU (NaN passes): beyond that the slope equals
+// its limit 0 or 1 in fp32, while x^3 of a huge x would overflow into 0 * inf, and a huge negative x
+// would multiply the smallest s that the held exponent gives.
+// Exact = false (16-bit gradients) takes the base-2 exponential and the hardware reciprocal as
+// FastActOp does, relative error ~1e-6, far below the rounding of the 16-bit result; true takes
+// expf and an IEEE division.
+template <bool Exact>
+struct ActSlope {
+    float a, b;    // z = x (a + b x^2); times log2 e when !Exact
+    float za, zb;  // z' = za + zb x^2
+    float limit;
+    __host__ static ActSlope make(uint32_t act) {
+        const double k = 2.0 * 0.7978845608028654, log2e = Exact ? 1.0 : 1.4426950408889634;
+        if (act == 0)
+            return ActSlope{static_cast<float>(k * log2e), static_cast<float>(0.044715 * k * log2e),
+                            static_cast<float>(k), static_cast<float>(3 * 0.044715 * k), 16.0f};
+        return ActSlope{static_cast<float>(log2e), 0.f, 1.f, 0.f, 200.0f};
+    }
+    __device__ __forceinline__ float operator()(float x) const {
+        if (fabsf(x) > limit) x = copysignf(limit, x);
+        const float x2 = x * x;
+        const float z = x * fmaf(b, x2, a);
+        const float e = Exact ? expf(fminf(-z, 88.f)) : ex2_ftz(fminf(-z, 126.f));
+        const float r = Exact ? __fdiv_rn(1.0f, 1.0f + e) : rcp_ftz(1.0f + e);
+        return fmaf(x * r * (e * r), fmaf(zb, x2, za), r);
+    }
+};
+
+}  // namespace hc

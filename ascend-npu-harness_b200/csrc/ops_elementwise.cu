@@ -12,6 +12,7 @@
 //                        (fp32; bf16/fp16 use the sigmoid form of FastActOp, see there)
 #include <cuda_runtime.h>
 
+#include "activation.cuh"
 #include "hc_device.cuh"
 #include "hc_internal.h"
 
@@ -121,67 +122,6 @@ struct AxpyOp {
     static constexpr bool kBinary = false;
     float alpha, beta;
     __device__ float apply(float x, float) const { return __fadd_rn(__fmul_rn(alpha, x), beta); }
-};
-
-struct ActOp {
-    static constexpr bool kBinary = false;
-    uint32_t act;  // 0 = GELU (tanh form), 1 = SiLU
-    __device__ float apply(float v, float) const {
-        if (act == 0) {
-            const float kSqrt2OverPi = 0.7978845608f;
-            const float kGeluCoeff = 0.044715f;
-            float x3 = __fmul_rn(__fmul_rn(v, v), v);
-            float inner = __fmul_rn(kSqrt2OverPi, __fadd_rn(v, __fmul_rn(kGeluCoeff, x3)));
-            float t = tanhf(inner);
-            return __fmul_rn(__fmul_rn(0.5f, v), __fadd_rn(1.0f, t));
-        }
-        if (v >= 0.0f) {
-            float e = expf(-v);
-            return __fdiv_rn(v, __fadd_rn(1.0f, e));
-        }
-        float e = expf(v);
-        return __fdiv_rn(__fmul_rn(v, e), __fadd_rn(1.0f, e));
-    }
-};
-
-// 16-bit outputs: the same functions through the logistic sigmoid, which needs one exponential
-// and one reciprocal instead of tanhf / expf / IEEE division:
-//   GELU_tanh(x) = 0.5 x (1 + tanh u) = x * sigmoid(2u),  u = sqrt(2/pi) (x + 0.044715 x^3);
-//   SiLU(x) = x * sigmoid(x);  sigmoid(z) = 1 / (1 + 2^(-z log2 e)).
-// With the constants folded into the base-2 exponent, both are x / (1 + 2^y), y = -x (a + b x^2):
-// GELU a = 2 sqrt(2/pi) log2 e, b = 0.044715 a; SiLU a = log2 e, b = 0.  Relative error ~1e-6, far
-// below the rounding of the bf16/fp16 result (2^-9 / 2^-12); the fp32 path (ActOp) keeps the
-// golden's operation order.  y is clamped to 126, so 1 + 2^y stays finite: for x -> -inf the
-// result is x * 2^-126-ish, i.e. 0 after rounding to 16 bits, as the golden gives.
-__device__ __forceinline__ float ex2_ftz(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float rcp_ftz(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-struct FastActOp {
-    static constexpr bool kBinary = false;
-    float a, b;  // y = -x (a + b x^2)
-    __host__ static FastActOp make(uint32_t act) {
-        const double log2e = 1.4426950408889634;
-        const double k = 2.0 * 0.7978845608028654 * log2e;  // 2 sqrt(2/pi) log2 e
-        return act == 0 ? FastActOp{static_cast<float>(k), static_cast<float>(0.044715 * k)}
-                        : FastActOp{static_cast<float>(log2e), 0.f};
-    }
-    __device__ float2 apply2(float2 x) const {
-        const float2 w = __ffma2_rn(make_float2(-b, -b), __fmul2_rn(x, x), make_float2(-a, -a));
-        const float2 y = __fmul2_rn(x, w);
-        float2 d = make_float2(ex2_ftz(fminf(y.x, 126.f)), ex2_ftz(fminf(y.y, 126.f)));
-        d = __fadd2_rn(d, make_float2(1.f, 1.f));
-        // MUFU rcp: measured faster here than three Newton steps on the FMA pipe
-        return __fmul2_rn(x, make_float2(rcp_ftz(d.x), rcp_ftz(d.y)));
-    }
-    __device__ float apply(float v, float) const { return apply2(make_float2(v, v)).x; }
 };
 
 template <typename T, typename Op>

@@ -1,0 +1,292 @@
+// Operators around the 8-bit block format (fp8_block.cuh): quantise and dequantise, and the
+// activation that keeps its input in 8 bits for the backward pass.
+//
+//   quantize_fp8_block         x -> (q, scale), blocks of 128 elements of a row, or 128 x 128 tiles
+//   dequantize_fp8_block       (q, scale) -> x
+//   activation_gelu_silu_ckpt  x -> (act(x), q, scale): the output from the unrounded x, the
+//                              checkpoint from x
+//   ..._ckpt_bwd               (dy, q, scale) -> dx = dy * act'(q * scale)
+//
+// All are HBM streams: per element the forward moves 2 e + 1 + 1/32 bytes (e = element size) and
+// the backward the same, against ~10 flops and two special-function calls.
+#include <cuda_runtime.h>
+
+#include "activation.cuh"
+#include "fp8_block.cuh"
+#include "hc_device.cuh"
+#include "hc_internal.h"
+
+namespace hc {
+namespace {
+
+constexpr int kThreads = 256;
+
+enum ActKind : int { kGelu = 0, kSilu = 1, kNoAct = 2 };
+
+// The function a forward kernel applies to the unrounded x next to the checkpoint.
+template <typename T>
+struct ActOf {
+    using Op = FastActOp;
+    static Op make(uint32_t act) { return FastActOp::make(act); }
+};
+template <>
+struct ActOf<float> {
+    using Op = ActOp;
+    static Op make(uint32_t act) { return ActOp{act}; }
+};
+
+// ---------------------------------------------------------------------------------------
+// Any row length and alignment: one warp per block of a row, lane l takes elements l + 32 i.
+// ---------------------------------------------------------------------------------------
+template <typename T, bool HasAct>
+__global__ void __launch_bounds__(kThreads) block_fwd_kernel(const T* __restrict__ x, T* __restrict__ y,
+                                                             uint8_t* __restrict__ q, float* __restrict__ scale,
+                                                             uint32_t rows, uint32_t cols, uint32_t row_blocks,
+                                                             typename ActOf<T>::Op op) {
+    const uint32_t lane = threadIdx.x & 31;
+    const uint64_t total = static_cast<uint64_t>(rows) * row_blocks;
+    const uint64_t stride = static_cast<uint64_t>(gridDim.x) * (kThreads / 32);
+    for (uint64_t b = static_cast<uint64_t>(blockIdx.x) * (kThreads / 32) + threadIdx.x / 32; b < total; b += stride) {
+        const uint64_t row = b / row_blocks;
+        const uint32_t c0 = static_cast<uint32_t>(b - row * row_blocks) * kFp8Block;
+        const uint64_t base = row * cols + c0;
+        const uint32_t n = min(kFp8Block, cols - c0);
+        float v[4];
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] = lane + 32 * i < n ? elem<T>::to_f(x[base + lane + 32 * i]) : 0.f;
+            m = max(m, abs_bits(v[i]));
+        }
+        float inv, s;
+        fp8_block_scale(warp_umax(m), inv, s);
+        if (lane == 0) scale[b] = s;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (lane + 32 * i < n) {
+                q[base + lane + 32 * i] = fp8_encode(__fmul_rn(v[i], inv));
+                if (HasAct) y[base + lane + 32 * i] = elem<T>::from_f(op.apply(v[i], 0.f));
+            }
+    }
+}
+
+// Act: the gradient dy * slope(q * scale); otherwise q * scale.
+template <typename T, bool HasAct>
+__global__ void __launch_bounds__(kThreads) block_bwd_kernel(const T* __restrict__ dy, const uint8_t* __restrict__ q,
+                                                             const float* __restrict__ scale, T* __restrict__ out,
+                                                             uint32_t rows, uint32_t cols, uint32_t row_blocks,
+                                                             ActSlope<sizeof(T) == 4> slope) {
+    const uint32_t lane = threadIdx.x & 31;
+    const uint64_t total = static_cast<uint64_t>(rows) * row_blocks;
+    const uint64_t stride = static_cast<uint64_t>(gridDim.x) * (kThreads / 32);
+    for (uint64_t b = static_cast<uint64_t>(blockIdx.x) * (kThreads / 32) + threadIdx.x / 32; b < total; b += stride) {
+        const uint64_t row = b / row_blocks;
+        const uint32_t c0 = static_cast<uint32_t>(b - row * row_blocks) * kFp8Block;
+        const uint64_t base = row * cols + c0;
+        const uint32_t n = min(kFp8Block, cols - c0);
+        const float s = scale[b];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (lane + 32 * i < n) {
+                const float v = __fmul_rn(fp8_decode(q[base + lane + 32 * i]), s);
+                out[base + lane + 32 * i] =
+                    elem<T>::from_f(HasAct ? __fmul_rn(elem<T>::to_f(dy[base + lane + 32 * i]), slope(v)) : v);
+            }
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// 128 x 128 tiles (weights: laid out once, so plain): one CTA per tile, two passes, the second
+// from cache.
+// ---------------------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(kThreads) tile_quant_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
+                                                              float* __restrict__ scale, uint32_t rows, uint32_t cols,
+                                                              uint32_t col_tiles, uint64_t tiles) {
+    __shared__ uint32_t part[kThreads / 32];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    for (uint64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+        const uint32_t r0 = static_cast<uint32_t>(t / col_tiles) * kFp8Block;
+        const uint32_t c0 = static_cast<uint32_t>(t % col_tiles) * kFp8Block;
+        const uint32_t nr = min(kFp8Block, rows - r0), nc = min(kFp8Block, cols - c0);
+        uint32_t m = 0;
+        for (uint32_t r = warp; r < nr; r += kThreads / 32)
+            for (uint32_t c = lane; c < nc; c += 32)
+                m = max(m, abs_bits(elem<T>::to_f(x[static_cast<uint64_t>(r0 + r) * cols + c0 + c])));
+        m = warp_umax(m);
+        if (lane == 0) part[warp] = m;
+        __syncthreads();
+        for (int w = 0; w < kThreads / 32; ++w) m = max(m, part[w]);
+        float inv, s;
+        fp8_block_scale(m, inv, s);
+        if (threadIdx.x == 0) scale[t] = s;
+        for (uint32_t r = warp; r < nr; r += kThreads / 32)
+            for (uint32_t c = lane; c < nc; c += 32) {
+                const uint64_t i = static_cast<uint64_t>(r0 + r) * cols + c0 + c;
+                q[i] = fp8_encode(__fmul_rn(elem<T>::to_f(x[i]), inv));
+            }
+        __syncthreads();  // part is rewritten by the next tile
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) tile_dequant_kernel(const uint8_t* __restrict__ q,
+                                                                const float* __restrict__ scale, T* __restrict__ x,
+                                                                uint32_t rows, uint32_t cols, uint32_t col_tiles,
+                                                                uint64_t tiles) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    for (uint64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+        const uint32_t r0 = static_cast<uint32_t>(t / col_tiles) * kFp8Block;
+        const uint32_t c0 = static_cast<uint32_t>(t % col_tiles) * kFp8Block;
+        const uint32_t nr = min(kFp8Block, rows - r0), nc = min(kFp8Block, cols - c0);
+        const float s = scale[t];
+        for (uint32_t r = warp; r < nr; r += kThreads / 32)
+            for (uint32_t c = lane; c < nc; c += 32) {
+                const uint64_t i = static_cast<uint64_t>(r0 + r) * cols + c0 + c;
+                x[i] = elem<T>::from_f(__fmul_rn(fp8_decode(q[i]), s));
+            }
+    }
+}
+
+// Grid of a grid-stride launch over `items`, at most what is resident at once.
+template <typename K>
+unsigned grid_of(K kernel, uint64_t items, uint64_t per_block) {
+    const uint64_t blocks = (items + per_block - 1) / per_block;
+    const uint64_t cap = static_cast<uint64_t>(resident_blocks(reinterpret_cast<const void*>(kernel), kThreads, 0));
+    return static_cast<unsigned>(blocks < cap ? blocks : (cap ? cap : 1));
+}
+
+template <typename T, bool HasAct>
+int launch_fwd(const void* x, void* y, void* q, float* scale, uint32_t rows, uint32_t cols, uint32_t act,
+               cudaStream_t s, const char* name) {
+    const uint32_t nb = (cols + kFp8Block - 1) / kFp8Block;
+    const auto op = ActOf<T>::make(act);
+    const uint64_t blocks = static_cast<uint64_t>(rows) * nb;
+    auto* k = block_fwd_kernel<T, HasAct>;
+    k<<<grid_of(k, blocks, kThreads / 32), kThreads, 0, s>>>(static_cast<const T*>(x), static_cast<T*>(y),
+                                                             static_cast<uint8_t*>(q), scale, rows, cols, nb, op);
+    return check_launch(name);
+}
+
+template <typename T, bool HasAct>
+int launch_bwd(const void* dy, const void* q, const float* scale, void* out, uint32_t rows, uint32_t cols, uint32_t act,
+               cudaStream_t s, const char* name) {
+    const uint32_t nb = (cols + kFp8Block - 1) / kFp8Block;
+    const auto slope = ActSlope<sizeof(T) == 4>::make(act);
+    const uint64_t blocks = static_cast<uint64_t>(rows) * nb;
+    auto* k = block_bwd_kernel<T, HasAct>;
+    k<<<grid_of(k, blocks, kThreads / 32), kThreads, 0, s>>>(static_cast<const T*>(dy), static_cast<const uint8_t*>(q),
+                                                             scale, static_cast<T*>(out), rows, cols, nb, slope);
+    return check_launch(name);
+}
+
+template <typename T>
+int launch_quant(const void* x, void* q, float* scale, const fp8_block_tiling_data* t, cudaStream_t s) {
+    if (t->blockRows == 1)
+        return launch_fwd<T, false>(x, nullptr, q, scale, t->rows, t->cols, 0, s, "quantize_fp8_block");
+    const uint32_t ct = (t->cols + kFp8Block - 1) / kFp8Block;
+    const uint64_t tiles = static_cast<uint64_t>((t->rows + kFp8Block - 1) / kFp8Block) * ct;
+    auto* k = tile_quant_kernel<T>;
+    k<<<grid_of(k, tiles, 1), kThreads, 0, s>>>(static_cast<const T*>(x), static_cast<uint8_t*>(q), scale, t->rows,
+                                                t->cols, ct, tiles);
+    return check_launch("quantize_fp8_block");
+}
+
+template <typename T>
+int launch_dequant(const void* q, const float* scale, void* x, const fp8_block_tiling_data* t, cudaStream_t s) {
+    if (t->blockRows == 1)
+        return launch_bwd<T, false>(nullptr, q, scale, x, t->rows, t->cols, 0, s, "dequantize_fp8_block");
+    const uint32_t ct = (t->cols + kFp8Block - 1) / kFp8Block;
+    const uint64_t tiles = static_cast<uint64_t>((t->rows + kFp8Block - 1) / kFp8Block) * ct;
+    auto* k = tile_dequant_kernel<T>;
+    k<<<grid_of(k, tiles, 1), kThreads, 0, s>>>(static_cast<const uint8_t*>(q), scale, static_cast<T*>(x), t->rows,
+                                                t->cols, ct, tiles);
+    return check_launch("dequantize_fp8_block");
+}
+
+// Largest row count and row length: block counts and 32-bit column indices stay clear of overflow.
+constexpr uint32_t kMaxDim = 0x7FFFFFFFu;
+
+int check_block_args(const char* name, const fp8_block_tiling_data* t, int dtype, const void* a, const void* b,
+                     const void* c) {
+    if (!t) return fail(HC_ERR_INVALID, "%s: null tiling", name);
+    if (t->blockRows != 1 && t->blockRows != kFp8Block)
+        return fail(HC_ERR_INVALID, "%s: blockRows %u (1 or 128)", name, t->blockRows);
+    if (dtype != HC_DTYPE_F32 && dtype != HC_DTYPE_F16 && dtype != HC_DTYPE_BF16)
+        return fail(HC_ERR_UNSUPPORTED, "%s: dtype %d not supported (F32, F16, BF16)", name, dtype);
+    if (t->rows > kMaxDim || t->cols > kMaxDim) return fail(HC_ERR_UNSUPPORTED, "%s: sizes over 2^31 - 1", name);
+    if (t->rows && t->cols && (!a || !b || !c)) return fail(HC_ERR_INVALID, "%s: null pointer", name);
+    return HC_OK;
+}
+
+int check_ckpt_args(const char* name, const activation_gelu_silu_ckpt_tiling_data* t, int dtype, const void* a,
+                    const void* b, const void* c, const void* d) {
+    if (!t) return fail(HC_ERR_INVALID, "%s: null tiling", name);
+    if (t->actType > 1) return fail(HC_ERR_INVALID, "%s: actType %u (0 = GELU, 1 = SiLU)", name, t->actType);
+    if (dtype != HC_DTYPE_F32 && dtype != HC_DTYPE_F16 && dtype != HC_DTYPE_BF16)
+        return fail(HC_ERR_UNSUPPORTED, "%s: dtype %d not supported (F32, F16, BF16)", name, dtype);
+    if (t->rows > kMaxDim || t->cols > kMaxDim) return fail(HC_ERR_UNSUPPORTED, "%s: sizes over 2^31 - 1", name);
+    if (t->rows && t->cols && (!a || !b || !c || !d)) return fail(HC_ERR_INVALID, "%s: null pointer", name);
+    return HC_OK;
+}
+
+}  // namespace
+}  // namespace hc
+
+using namespace hc;
+
+extern "C" int hc_quantize_fp8_block_launch(const void* x, void* q, float* scale, const fp8_block_tiling_data* t,
+                                            int dtype, void* stream) {
+    if (int rc = check_block_args("quantize_fp8_block", t, dtype, x, q, scale)) return rc;
+    if (t->rows == 0 || t->cols == 0) return ok();
+    if (fault_hit("launch")) return fail(HC_ERR_INJECTED, "quantize_fp8_block: injected launch failure");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    switch (dtype) {
+        case HC_DTYPE_F32: return launch_quant<float>(x, q, scale, t, s);
+        case HC_DTYPE_F16: return launch_quant<f16_t>(x, q, scale, t, s);
+        default: return launch_quant<bf16_t>(x, q, scale, t, s);
+    }
+}
+
+extern "C" int hc_dequantize_fp8_block_launch(const void* q, const float* scale, void* x,
+                                              const fp8_block_tiling_data* t, int dtype, void* stream) {
+    if (int rc = check_block_args("dequantize_fp8_block", t, dtype, q, scale, x)) return rc;
+    if (t->rows == 0 || t->cols == 0) return ok();
+    if (fault_hit("launch")) return fail(HC_ERR_INJECTED, "dequantize_fp8_block: injected launch failure");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    switch (dtype) {
+        case HC_DTYPE_F32: return launch_dequant<float>(q, scale, x, t, s);
+        case HC_DTYPE_F16: return launch_dequant<f16_t>(q, scale, x, t, s);
+        default: return launch_dequant<bf16_t>(q, scale, x, t, s);
+    }
+}
+
+extern "C" int hc_activation_gelu_silu_ckpt_launch(const void* x, void* y, void* q, float* scale,
+                                                   const activation_gelu_silu_ckpt_tiling_data* t, int dtype,
+                                                   void* stream) {
+    static const char* name = "activation_gelu_silu_ckpt";
+    if (int rc = check_ckpt_args(name, t, dtype, x, y, q, scale)) return rc;
+    if (t->rows == 0 || t->cols == 0) return ok();
+    if (fault_hit("launch")) return fail(HC_ERR_INJECTED, "%s: injected launch failure", name);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    switch (dtype) {
+        case HC_DTYPE_F32: return launch_fwd<float, true>(x, y, q, scale, t->rows, t->cols, t->actType, s, name);
+        case HC_DTYPE_F16: return launch_fwd<f16_t, true>(x, y, q, scale, t->rows, t->cols, t->actType, s, name);
+        default: return launch_fwd<bf16_t, true>(x, y, q, scale, t->rows, t->cols, t->actType, s, name);
+    }
+}
+
+extern "C" int hc_activation_gelu_silu_ckpt_bwd_launch(const void* dy, const void* q, const float* scale, void* dx,
+                                                       const activation_gelu_silu_ckpt_tiling_data* t, int dtype,
+                                                       void* stream) {
+    static const char* name = "activation_gelu_silu_ckpt_bwd";
+    if (int rc = check_ckpt_args(name, t, dtype, dy, q, scale, dx)) return rc;
+    if (t->rows == 0 || t->cols == 0) return ok();
+    if (fault_hit("launch")) return fail(HC_ERR_INJECTED, "%s: injected launch failure", name);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    switch (dtype) {
+        case HC_DTYPE_F32: return launch_bwd<float, true>(dy, q, scale, dx, t->rows, t->cols, t->actType, s, name);
+        case HC_DTYPE_F16: return launch_bwd<f16_t, true>(dy, q, scale, dx, t->rows, t->cols, t->actType, s, name);
+        default: return launch_bwd<bf16_t, true>(dy, q, scale, dx, t->rows, t->cols, t->actType, s, name);
+    }
+}

@@ -21,11 +21,23 @@
 //   hc::flash_attention_fwd_fused(q, k, v, scale, mask_type) -> (o, lse)   (k, v may have fewer heads: GQA)
 //   hc::flash_attention_bwd(q, k, v, o, lse, dout, scale, mask_type) -> (dq, dk, dv, delta)
 //                                          (no reference counterpart; K/V with the query head count)
-// hc.load_torch_ops() also registers the backward as the autograd formula of the forward op.
+//   hc::layer_norm_fwd_train(x, gamma, beta, eps) -> (y, mean, rstd)
+//   hc::layer_norm_bwd(dy, x, gamma, mean, rstd) -> (dx, dgamma, dbeta)
+//   hc::layer_norm_ckpt(x, gamma, beta, eps) -> (y, q, scale, rstd)        normalised rows kept in 8 bits
+//   hc::layer_norm_ckpt_bwd(dy, q, scale, gamma, rstd) -> (dx, dgamma, dbeta)
+//   hc::activation_gelu_silu_ckpt(x, act) -> (y, q, scale)                 x kept in 8 bits
+//   hc::activation_gelu_silu_ckpt_bwd(dy, q, scale, act) -> dx
+//   hc::quantize_fp8_block(x, block_rows) -> (q, scale), hc::dequantize_fp8_block(q, scale, dtype, block_rows) -> x
+//   hc::matmul_fp8_block(a, a_scale, b, b_scale, bias?, dtype) -> c
+//                                          (no reference counterparts)
+// hc.load_torch_ops() also registers the attention backward as the autograd formula of the forward
+// op; the two layer norms and the checkpointed activation have theirs here (class names ending in
+// Function), since a Python formula would cost more host time than the kernels take on small rows.
 // Load with torch.ops.load_library("ascend-npu-harness_b200/lib/libhc_torch.so").
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include <cmath>
@@ -281,6 +293,303 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> flash_attention_bwd_c
 }
 
 // ---------------------------------------------------------------------------------------------
+// 8-bit blocks and layer norm for training
+// ---------------------------------------------------------------------------------------------
+constexpr int64_t kFp8BlockSize = 128;
+
+// A tensor argument of the given type and shape on `like`'s device.
+void check_arg(const at::Tensor& t, const char* what, at::ScalarType type, at::IntArrayRef shape, const at::Tensor& like) {
+    check_input(t, what);
+    TORCH_CHECK(t.scalar_type() == type, "hc: ", what, " must be ", type, ", got ", t.scalar_type());
+    TORCH_CHECK(t.sizes() == shape, "hc: ", what, " must have shape ", shape, ", got ", t.sizes());
+    TORCH_CHECK(t.device() == like.device(), "hc: ", what, " is on another device");
+}
+
+std::vector<int64_t> fp8_scale_shape(at::IntArrayRef x, int64_t block_rows) {
+    TORCH_CHECK(!x.empty(), "hc: 8-bit blocks need at least one dimension");
+    TORCH_CHECK(block_rows == 1 || (block_rows == kFp8BlockSize && x.size() == 2),
+                "hc: block_rows is 1, or 128 for a 2-D weight");
+    std::vector<int64_t> s(x.begin(), x.end());
+    s.back() = (s.back() + kFp8BlockSize - 1) / kFp8BlockSize;
+    if (block_rows != 1) s[0] = (s[0] + kFp8BlockSize - 1) / kFp8BlockSize;
+    return s;
+}
+
+std::pair<at::Tensor, at::Tensor> fp8_outputs(const at::Tensor& x, int64_t block_rows) {
+    return {at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn)),
+            at::empty(fp8_scale_shape(x.sizes(), block_rows), x.options().dtype(at::kFloat))};
+}
+
+uint32_t rows_of(const at::Tensor& x) { return u32(x.size(-1) ? x.numel() / x.size(-1) : 0, "rows"); }
+uint32_t cols_of(const at::Tensor& x) { return u32(x.size(-1), "cols"); }
+
+std::tuple<at::Tensor, at::Tensor> quantize_fp8_block_cuda(const at::Tensor& x, int64_t block_rows) {
+    check_input(x, "x");
+    c10::cuda::CUDAGuard guard(x.device());
+    auto [q, scale] = fp8_outputs(x, block_rows);
+    fp8_block_tiling_data t{rows_of(x), cols_of(x), u32(block_rows, "block_rows")};
+    ok_or_throw(hc_quantize_fp8_block_launch(x.data_ptr(), q.data_ptr(), scale.data_ptr<float>(), &t, dtype_code(x),
+                                             stream_of(x)),
+                "quantize_fp8_block");
+    return {q, scale};
+}
+
+at::Tensor dequantize_fp8_block_cuda(const at::Tensor& q, const at::Tensor& scale, at::ScalarType dtype,
+                                     int64_t block_rows) {
+    check_arg(q, "q", at::kFloat8_e4m3fn, q.sizes(), q);
+    check_arg(scale, "scale", at::kFloat, fp8_scale_shape(q.sizes(), block_rows), q);
+    c10::cuda::CUDAGuard guard(q.device());
+    at::Tensor x = at::empty(q.sizes(), q.options().dtype(dtype));
+    fp8_block_tiling_data t{rows_of(q), cols_of(q), u32(block_rows, "block_rows")};
+    ok_or_throw(hc_dequantize_fp8_block_launch(q.data_ptr(), scale.data_ptr<float>(), x.data_ptr(), &t, dtype_code(x),
+                                               stream_of(q)),
+                "dequantize_fp8_block");
+    return x;
+}
+
+at::Tensor matmul_fp8_block_cuda(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b,
+                                 const at::Tensor& b_scale, const std::optional<at::Tensor>& bias, at::ScalarType dtype) {
+    TORCH_CHECK(a.dim() == 2 && b.dim() == 2 && a.size(1) == b.size(1), "hc: matmul_fp8_block needs a [M, K] and b [N, K]");
+    check_arg(a, "a", at::kFloat8_e4m3fn, a.sizes(), a);
+    check_arg(b, "b", at::kFloat8_e4m3fn, b.sizes(), a);
+    check_arg(a_scale, "a_scale", at::kFloat, fp8_scale_shape(a.sizes(), 1), a);
+    check_arg(b_scale, "b_scale", at::kFloat, fp8_scale_shape(b.sizes(), kFp8BlockSize), a);
+    if (bias) check_arg(*bias, "bias", dtype, {b.size(0)}, a);
+    c10::cuda::CUDAGuard guard(a.device());
+    at::Tensor c = at::empty({a.size(0), b.size(0)}, a.options().dtype(dtype));
+    matmul_fp8_block_tiling_data t{u32(a.size(0), "M"), u32(a.size(1), "K"), u32(b.size(0), "N")};
+    ok_or_throw(hc_matmul_fp8_block_launch(a.data_ptr(), a_scale.data_ptr<float>(), b.data_ptr(), b_scale.data_ptr<float>(),
+                                           bias ? bias->data_ptr() : nullptr, c.data_ptr(), &t, dtype_code(c), stream_of(a)),
+                "matmul_fp8_block");
+    return c;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> activation_gelu_silu_ckpt_cuda(const at::Tensor& x, int64_t act) {
+    check_input(x, "x");
+    c10::cuda::CUDAGuard guard(x.device());
+    auto [q, scale] = fp8_outputs(x, 1);
+    at::Tensor y = at::empty_like(x);
+    activation_gelu_silu_ckpt_tiling_data t{rows_of(x), cols_of(x), u32(act, "act")};
+    ok_or_throw(hc_activation_gelu_silu_ckpt_launch(x.data_ptr(), y.data_ptr(), q.data_ptr(), scale.data_ptr<float>(), &t,
+                                                    dtype_code(x), stream_of(x)),
+                "activation_gelu_silu_ckpt");
+    return {y, q, scale};
+}
+
+at::Tensor activation_gelu_silu_ckpt_bwd_cuda(const at::Tensor& dy, const at::Tensor& q, const at::Tensor& scale,
+                                              int64_t act) {
+    check_input(dy, "dy");
+    check_arg(q, "q", at::kFloat8_e4m3fn, dy.sizes(), dy);
+    check_arg(scale, "scale", at::kFloat, fp8_scale_shape(dy.sizes(), 1), dy);
+    c10::cuda::CUDAGuard guard(dy.device());
+    at::Tensor dx = at::empty_like(dy);
+    activation_gelu_silu_ckpt_tiling_data t{rows_of(dy), cols_of(dy), u32(act, "act")};
+    ok_or_throw(hc_activation_gelu_silu_ckpt_bwd_launch(dy.data_ptr(), q.data_ptr(), scale.data_ptr<float>(), dx.data_ptr(),
+                                                        &t, dtype_code(dy), stream_of(dy)),
+                "activation_gelu_silu_ckpt_bwd");
+    return dx;
+}
+
+layer_norm_tiling_data ln_tiling(const at::Tensor& x, double eps) {
+    return {rows_of(x), cols_of(x), 0, static_cast<float>(eps)};
+}
+
+void check_ln(const at::Tensor& x, const at::Tensor& gamma, const char* what) {
+    TORCH_CHECK(x.dim() >= 1, "hc: layer norm needs at least one dimension");
+    check_arg(gamma, what, at::kFloat, {x.size(-1)}, x);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_fwd_train_cuda(const at::Tensor& x, const at::Tensor& gamma,
+                                                                         const at::Tensor& beta, double eps) {
+    check_input(x, "x");
+    check_ln(x, gamma, "gamma");
+    check_ln(x, beta, "beta");
+    c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor y = at::empty_like(x);
+    at::Tensor mean = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+    at::Tensor rstd = at::empty_like(mean);
+    const layer_norm_tiling_data t = ln_tiling(x, eps);
+    ok_or_throw(hc_layer_norm_fwd_train_launch(x.data_ptr(), gamma.data_ptr<float>(), beta.data_ptr<float>(), y.data_ptr(),
+                                               mean.data_ptr<float>(), rstd.data_ptr<float>(), nullptr, nullptr, &t,
+                                               dtype_code(x), stream_of(x)),
+                "layer_norm_fwd_train");
+    return {y, mean, rstd};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> layer_norm_ckpt_cuda(const at::Tensor& x, const at::Tensor& gamma,
+                                                                                const at::Tensor& beta, double eps) {
+    check_input(x, "x");
+    check_ln(x, gamma, "gamma");
+    check_ln(x, beta, "beta");
+    c10::cuda::CUDAGuard guard(x.device());
+    auto [q, scale] = fp8_outputs(x, 1);
+    at::Tensor y = at::empty_like(x);
+    at::Tensor rstd = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+    const layer_norm_tiling_data t = ln_tiling(x, eps);
+    ok_or_throw(hc_layer_norm_fwd_train_launch(x.data_ptr(), gamma.data_ptr<float>(), beta.data_ptr<float>(), y.data_ptr(),
+                                               nullptr, rstd.data_ptr<float>(), q.data_ptr(), scale.data_ptr<float>(), &t,
+                                               dtype_code(x), stream_of(x)),
+                "layer_norm_ckpt");
+    return {y, q, scale, rstd};
+}
+
+// Outputs and workspace of a layer norm backward, allocated on the current stream.
+struct LnGrads {
+    at::Tensor dx, dgamma, dbeta, work;
+    layer_norm_tiling_data t;
+    LnGrads(const at::Tensor& dy, const at::Tensor& gamma) : t(ln_tiling(dy, 0.0)) {
+        size_t bytes = 0;
+        ok_or_throw(hc_layer_norm_bwd_workspace_size(&t, dtype_code(dy), &bytes), "layer_norm_bwd");
+        dx = at::empty_like(dy);
+        dgamma = at::empty_like(gamma);
+        dbeta = at::empty_like(gamma);
+        work = at::empty({static_cast<int64_t>(bytes)}, dy.options().dtype(at::kByte));
+    }
+};
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_bwd_cuda(const at::Tensor& dy, const at::Tensor& x,
+                                                                   const at::Tensor& gamma, const at::Tensor& mean,
+                                                                   const at::Tensor& rstd) {
+    check_input(dy, "dy");
+    check_ln(dy, gamma, "gamma");
+    check_arg(x, "x", dy.scalar_type(), dy.sizes(), dy);
+    check_arg(mean, "mean", at::kFloat, dy.sizes().slice(0, dy.dim() - 1), dy);
+    check_arg(rstd, "rstd", at::kFloat, dy.sizes().slice(0, dy.dim() - 1), dy);
+    c10::cuda::CUDAGuard guard(dy.device());
+    LnGrads g(dy, gamma);
+    ok_or_throw(hc_layer_norm_bwd_launch(dy.data_ptr(), x.data_ptr(), gamma.data_ptr<float>(), mean.data_ptr<float>(),
+                                         rstd.data_ptr<float>(), g.dx.data_ptr(), g.dgamma.data_ptr<float>(),
+                                         g.dbeta.data_ptr<float>(), g.work.data_ptr(), g.work.numel(), &g.t,
+                                         dtype_code(dy), stream_of(dy)),
+                "layer_norm_bwd");
+    return {g.dx, g.dgamma, g.dbeta};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_ckpt_bwd_cuda(const at::Tensor& dy, const at::Tensor& q,
+                                                                        const at::Tensor& scale, const at::Tensor& gamma,
+                                                                        const at::Tensor& rstd) {
+    check_input(dy, "dy");
+    check_ln(dy, gamma, "gamma");
+    check_arg(q, "q", at::kFloat8_e4m3fn, dy.sizes(), dy);
+    check_arg(scale, "scale", at::kFloat, fp8_scale_shape(dy.sizes(), 1), dy);
+    check_arg(rstd, "rstd", at::kFloat, dy.sizes().slice(0, dy.dim() - 1), dy);
+    c10::cuda::CUDAGuard guard(dy.device());
+    LnGrads g(dy, gamma);
+    ok_or_throw(hc_layer_norm_ckpt_bwd_launch(dy.data_ptr(), q.data_ptr(), scale.data_ptr<float>(), gamma.data_ptr<float>(),
+                                              rstd.data_ptr<float>(), g.dx.data_ptr(), g.dgamma.data_ptr<float>(),
+                                              g.dbeta.data_ptr<float>(), g.work.data_ptr(), g.work.numel(), &g.t,
+                                              dtype_code(dy), stream_of(dy)),
+                "layer_norm_ckpt_bwd");
+    return {g.dx, g.dgamma, g.dbeta};
+}
+
+// ---------------------------------------------------------------------------------------------
+// Autograd formulas
+// ---------------------------------------------------------------------------------------------
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+using Tensors3 = std::tuple<at::Tensor, at::Tensor, at::Tensor>;
+using Tensors4 = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+using TensorRef = const at::Tensor&;
+
+template <typename F>
+c10::TypedOperatorHandle<F> op_handle(const char* name) {
+    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").template typed<F>();
+}
+
+// The ops below their autograd layer.
+Tensors3 ln_fwd_train_below(TensorRef x, TensorRef gamma, TensorRef beta, double eps) {
+    static const auto op = op_handle<Tensors3(TensorRef, TensorRef, TensorRef, double)>("hc::layer_norm_fwd_train");
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return op.call(x, gamma, beta, eps);
+}
+Tensors4 ln_ckpt_below(TensorRef x, TensorRef gamma, TensorRef beta, double eps) {
+    static const auto op = op_handle<Tensors4(TensorRef, TensorRef, TensorRef, double)>("hc::layer_norm_ckpt");
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return op.call(x, gamma, beta, eps);
+}
+Tensors3 act_ckpt_below(TensorRef x, int64_t act) {
+    static const auto op = op_handle<Tensors3(TensorRef, int64_t)>("hc::activation_gelu_silu_ckpt");
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return op.call(x, act);
+}
+
+void no_double_backward(const char* op) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "hc::", op, " has no second derivative (create_graph=True)");
+}
+
+struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
+    static variable_list forward(AutogradContext* ctx, TensorRef x, TensorRef gamma, TensorRef beta, double eps) {
+        auto [y, mean, rstd] = ln_fwd_train_below(x, gamma, beta, eps);
+        ctx->save_for_backward({x, gamma, mean, rstd});
+        ctx->mark_non_differentiable({mean, rstd});
+        return {y, mean, rstd};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        no_double_backward("layer_norm_fwd_train");
+        if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+        const auto s = ctx->get_saved_variables();
+        auto [dx, dgamma, dbeta] = layer_norm_bwd_cuda(grads[0].contiguous(), s[0], s[1], s[2], s[3]);
+        return {dx, dgamma, dbeta, at::Tensor()};
+    }
+};
+
+struct LayerNormCkptFunction : torch::autograd::Function<LayerNormCkptFunction> {
+    static variable_list forward(AutogradContext* ctx, TensorRef x, TensorRef gamma, TensorRef beta, double eps) {
+        auto [y, q, scale, rstd] = ln_ckpt_below(x, gamma, beta, eps);
+        ctx->save_for_backward({q, scale, gamma, rstd});
+        ctx->mark_non_differentiable({q, scale, rstd});
+        return {y, q, scale, rstd};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        no_double_backward("layer_norm_ckpt");
+        if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+        const auto s = ctx->get_saved_variables();
+        auto [dx, dgamma, dbeta] = layer_norm_ckpt_bwd_cuda(grads[0].contiguous(), s[0], s[1], s[2], s[3]);
+        return {dx, dgamma, dbeta, at::Tensor()};
+    }
+};
+
+struct ActivationCkptFunction : torch::autograd::Function<ActivationCkptFunction> {
+    static variable_list forward(AutogradContext* ctx, TensorRef x, int64_t act) {
+        auto [y, q, scale] = act_ckpt_below(x, act);
+        ctx->save_for_backward({q, scale});
+        ctx->mark_non_differentiable({q, scale});
+        ctx->saved_data["act"] = act;
+        return {y, q, scale};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        no_double_backward("activation_gelu_silu_ckpt");
+        if (!grads[0].defined()) return {at::Tensor(), at::Tensor()};
+        const auto s = ctx->get_saved_variables();
+        return {activation_gelu_silu_ckpt_bwd_cuda(grads[0].contiguous(), s[0], s[1], ctx->saved_data["act"].toInt()),
+                at::Tensor()};
+    }
+};
+
+template <typename... T>
+bool wants_grad(const T&... t) {
+    return at::GradMode::is_enabled() && (t.requires_grad() || ...);
+}
+
+Tensors3 layer_norm_fwd_train_autograd(TensorRef x, TensorRef gamma, TensorRef beta, double eps) {
+    if (!wants_grad(x, gamma, beta)) return ln_fwd_train_below(x, gamma, beta, eps);
+    const variable_list o = LayerNormFunction::apply(x, gamma, beta, eps);
+    return {o[0], o[1], o[2]};
+}
+Tensors4 layer_norm_ckpt_autograd(TensorRef x, TensorRef gamma, TensorRef beta, double eps) {
+    if (!wants_grad(x, gamma, beta)) return ln_ckpt_below(x, gamma, beta, eps);
+    const variable_list o = LayerNormCkptFunction::apply(x, gamma, beta, eps);
+    return {o[0], o[1], o[2], o[3]};
+}
+Tensors3 activation_gelu_silu_ckpt_autograd(TensorRef x, int64_t act) {
+    if (!wants_grad(x)) return act_ckpt_below(x, act);
+    const variable_list o = ActivationCkptFunction::apply(x, act);
+    return {o[0], o[1], o[2]};
+}
+
+// ---------------------------------------------------------------------------------------------
 // Meta kernels (shapes only)
 // ---------------------------------------------------------------------------------------------
 at::Tensor same_meta(const at::Tensor& x) { return at::empty_like(x); }
@@ -320,6 +629,45 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> flash_attention_bwd_m
             at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat))};
 }
 
+std::tuple<at::Tensor, at::Tensor> quantize_fp8_block_meta(const at::Tensor& x, int64_t block_rows) {
+    auto [q, scale] = fp8_outputs(x, block_rows);
+    return {q, scale};
+}
+at::Tensor dequantize_fp8_block_meta(const at::Tensor& q, const at::Tensor&, at::ScalarType dtype, int64_t) {
+    return at::empty(q.sizes(), q.options().dtype(dtype));
+}
+at::Tensor matmul_fp8_block_meta(const at::Tensor& a, const at::Tensor&, const at::Tensor& b, const at::Tensor&,
+                                 const std::optional<at::Tensor>&, at::ScalarType dtype) {
+    TORCH_CHECK(a.dim() == 2 && b.dim() == 2 && a.size(1) == b.size(1), "hc: matmul_fp8_block needs a [M, K] and b [N, K]");
+    return at::empty({a.size(0), b.size(0)}, a.options().dtype(dtype));
+}
+Tensors3 activation_gelu_silu_ckpt_meta(const at::Tensor& x, int64_t) {
+    auto [q, scale] = fp8_outputs(x, 1);
+    return {at::empty_like(x), q, scale};
+}
+at::Tensor activation_gelu_silu_ckpt_bwd_meta(const at::Tensor& dy, const at::Tensor&, const at::Tensor&, int64_t) {
+    return at::empty_like(dy);
+}
+at::Tensor row_stat_meta(const at::Tensor& x) {
+    TORCH_CHECK(x.dim() >= 1, "hc: layer norm needs at least one dimension");
+    return at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+}
+Tensors3 layer_norm_fwd_train_meta(const at::Tensor& x, const at::Tensor&, const at::Tensor&, double) {
+    return {at::empty_like(x), row_stat_meta(x), row_stat_meta(x)};
+}
+Tensors4 layer_norm_ckpt_meta(const at::Tensor& x, const at::Tensor&, const at::Tensor&, double) {
+    auto [q, scale] = fp8_outputs(x, 1);
+    return {at::empty_like(x), q, scale, row_stat_meta(x)};
+}
+Tensors3 layer_norm_bwd_meta(const at::Tensor& dy, const at::Tensor&, const at::Tensor& gamma, const at::Tensor&,
+                             const at::Tensor&) {
+    return {at::empty_like(dy), at::empty_like(gamma), at::empty_like(gamma)};
+}
+Tensors3 layer_norm_ckpt_bwd_meta(const at::Tensor& dy, const at::Tensor&, const at::Tensor&, const at::Tensor& gamma,
+                                  const at::Tensor&) {
+    return {at::empty_like(dy), at::empty_like(gamma), at::empty_like(gamma)};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(hc, m) {
@@ -336,6 +684,15 @@ TORCH_LIBRARY(hc, m) {
     m.def("flash_attention_fwd_fused(Tensor q, Tensor k, Tensor v, float scale, int mask_type) -> (Tensor, Tensor)");
     m.def("flash_attention_bwd(Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor dout, float scale, "
           "int mask_type) -> (Tensor, Tensor, Tensor, Tensor)");
+    m.def("quantize_fp8_block(Tensor x, int block_rows=1) -> (Tensor, Tensor)");
+    m.def("dequantize_fp8_block(Tensor q, Tensor scale, ScalarType dtype, int block_rows=1) -> Tensor");
+    m.def("matmul_fp8_block(Tensor a, Tensor a_scale, Tensor b, Tensor b_scale, Tensor? bias, ScalarType dtype) -> Tensor");
+    m.def("activation_gelu_silu_ckpt(Tensor x, int act) -> (Tensor, Tensor, Tensor)");
+    m.def("activation_gelu_silu_ckpt_bwd(Tensor dy, Tensor q, Tensor scale, int act) -> Tensor");
+    m.def("layer_norm_fwd_train(Tensor x, Tensor gamma, Tensor beta, float eps) -> (Tensor, Tensor, Tensor)");
+    m.def("layer_norm_bwd(Tensor dy, Tensor x, Tensor gamma, Tensor mean, Tensor rstd) -> (Tensor, Tensor, Tensor)");
+    m.def("layer_norm_ckpt(Tensor x, Tensor gamma, Tensor beta, float eps) -> (Tensor, Tensor, Tensor, Tensor)");
+    m.def("layer_norm_ckpt_bwd(Tensor dy, Tensor q, Tensor scale, Tensor gamma, Tensor rstd) -> (Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(hc, CUDA, m) {
@@ -350,6 +707,15 @@ TORCH_LIBRARY_IMPL(hc, CUDA, m) {
     m.impl("matmul_bias", &matmul_bias_cuda);
     m.impl("flash_attention_fwd_fused", &flash_attention_fwd_fused_cuda);
     m.impl("flash_attention_bwd", &flash_attention_bwd_cuda);
+    m.impl("quantize_fp8_block", &quantize_fp8_block_cuda);
+    m.impl("dequantize_fp8_block", &dequantize_fp8_block_cuda);
+    m.impl("matmul_fp8_block", &matmul_fp8_block_cuda);
+    m.impl("activation_gelu_silu_ckpt", &activation_gelu_silu_ckpt_cuda);
+    m.impl("activation_gelu_silu_ckpt_bwd", &activation_gelu_silu_ckpt_bwd_cuda);
+    m.impl("layer_norm_fwd_train", &layer_norm_fwd_train_cuda);
+    m.impl("layer_norm_bwd", &layer_norm_bwd_cuda);
+    m.impl("layer_norm_ckpt", &layer_norm_ckpt_cuda);
+    m.impl("layer_norm_ckpt_bwd", &layer_norm_ckpt_bwd_cuda);
 }
 
 TORCH_LIBRARY_IMPL(hc, Meta, m) {
@@ -364,4 +730,19 @@ TORCH_LIBRARY_IMPL(hc, Meta, m) {
     m.impl("matmul_bias", &matmul_bias_meta);
     m.impl("flash_attention_fwd_fused", &flash_attention_fwd_fused_meta);
     m.impl("flash_attention_bwd", &flash_attention_bwd_meta);
+    m.impl("quantize_fp8_block", &quantize_fp8_block_meta);
+    m.impl("dequantize_fp8_block", &dequantize_fp8_block_meta);
+    m.impl("matmul_fp8_block", &matmul_fp8_block_meta);
+    m.impl("activation_gelu_silu_ckpt", &activation_gelu_silu_ckpt_meta);
+    m.impl("activation_gelu_silu_ckpt_bwd", &activation_gelu_silu_ckpt_bwd_meta);
+    m.impl("layer_norm_fwd_train", &layer_norm_fwd_train_meta);
+    m.impl("layer_norm_bwd", &layer_norm_bwd_meta);
+    m.impl("layer_norm_ckpt", &layer_norm_ckpt_meta);
+    m.impl("layer_norm_ckpt_bwd", &layer_norm_ckpt_bwd_meta);
+}
+
+TORCH_LIBRARY_IMPL(hc, Autograd, m) {
+    m.impl("activation_gelu_silu_ckpt", &activation_gelu_silu_ckpt_autograd);
+    m.impl("layer_norm_fwd_train", &layer_norm_fwd_train_autograd);
+    m.impl("layer_norm_ckpt", &layer_norm_ckpt_autograd);
 }

@@ -79,6 +79,18 @@ class FlashAttentionFwdFusedTiling(C.Structure):
                 ("D", C.c_uint32), ("D_v", C.c_uint32), ("scale", C.c_float), ("maskType", C.c_uint32)]
 
 
+class Fp8BlockTiling(C.Structure):
+    _fields_ = [("rows", C.c_uint32), ("cols", C.c_uint32), ("blockRows", C.c_uint32)]
+
+
+class MatmulFp8BlockTiling(C.Structure):
+    _fields_ = [("M", C.c_uint32), ("K", C.c_uint32), ("N", C.c_uint32)]
+
+
+class ActivationGeluSiluCkptTiling(C.Structure):
+    _fields_ = [("rows", C.c_uint32), ("cols", C.c_uint32), ("actType", C.c_uint32)]
+
+
 _vp = C.c_void_p
 _i = C.c_int
 _u32 = C.c_uint32
@@ -142,6 +154,17 @@ SIGNATURES = {
     "hc_flash_attention_bwd_last_path": (_i, []),
     "hc_flash_attention_last_path": (_i, []),
     "hc_matmul_bias_last_path": (_i, []),
+    "hc_quantize_fp8_block_launch": (_i, [_vp, _vp, _vp, _P(Fp8BlockTiling), _i, _vp]),
+    "hc_dequantize_fp8_block_launch": (_i, [_vp, _vp, _vp, _P(Fp8BlockTiling), _i, _vp]),
+    "hc_matmul_fp8_block_launch": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _P(MatmulFp8BlockTiling), _i, _vp]),
+    "hc_matmul_fp8_block_last_path": (_i, []),
+    "hc_activation_gelu_silu_ckpt_launch": (_i, [_vp, _vp, _vp, _vp, _P(ActivationGeluSiluCkptTiling), _i, _vp]),
+    "hc_activation_gelu_silu_ckpt_bwd_launch": (_i, [_vp, _vp, _vp, _vp, _P(ActivationGeluSiluCkptTiling), _i, _vp]),
+    "hc_layer_norm_fwd_train_launch": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _P(LayerNormTiling), _i, _vp]),
+    "hc_layer_norm_bwd_workspace_size": (_i, [_P(LayerNormTiling), _i, _P(_sz)]),
+    "hc_layer_norm_bwd_launch": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _P(LayerNormTiling), _i, _vp]),
+    "hc_layer_norm_ckpt_bwd_launch": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _P(LayerNormTiling), _i,
+                                           _vp]),
 }
 
 _lib = None
@@ -362,6 +385,190 @@ def flash_attention_bwd(q, k, v, o, lse, dout, causal: bool, scale: float | None
     return dq, dk, dv, delta
 
 
+FP8_BLOCK = 128  # elements of a row (and rows of a weight tile) that share a scale
+
+
+def _expect(t, what: str, shape, dtype, like):
+    """Checks a tensor argument of the 8-bit block operators and returns its pointer."""
+    torch = _torch()
+    names = {torch.float8_e4m3fn: "float8_e4m3fn", torch.float32: "float32"}
+    if t.dtype != dtype:
+        raise HcError(HC_ERR_INVALID, f"{what} must be {names.get(dtype, dtype)}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise HcError(HC_ERR_INVALID, f"{what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.device != like.device:
+        raise HcError(HC_ERR_INVALID, f"{what} is on {t.device}, expected {like.device}")
+    return _ptr(t)
+
+
+def _rows_cols(x):
+    if x.dim() < 1:
+        raise HcError(HC_ERR_INVALID, "expected at least one dimension")
+    cols = x.shape[-1]
+    return (x.numel() // cols if cols else 0), cols
+
+
+def _fp8_scale_shape(shape, block_rows: int):
+    n = -(-shape[-1] // FP8_BLOCK)
+    if block_rows == 1:
+        return (*shape[:-1], n)
+    if block_rows != FP8_BLOCK or len(shape) != 2:
+        raise HcError(HC_ERR_INVALID, "block_rows is 1, or 128 for a 2-D weight")
+    return (-(-shape[0] // FP8_BLOCK), n)
+
+
+def _fp8_outputs(x, block_rows: int):
+    torch = _torch()
+    return (torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device),
+            torch.empty(_fp8_scale_shape(x.shape, block_rows), dtype=torch.float32, device=x.device))
+
+
+def _on(x):
+    """Makes x's device current for the launch."""
+    return _torch().cuda.device(x.device)
+
+
+def quantize_fp8_block(x, block_rows: int = 1, stream=None):
+    """x (f32/f16/bf16) in 8-bit blocks: (q e4m3 of x's shape, fp32 scale).  block_rows 1: a scale for each 128
+    elements of a row; 128: for each 128 x 128 tile of a 2-D weight."""
+    if not x.is_cuda:
+        raise HcError(HC_ERR_INVALID, "expected a CUDA tensor")
+    q, scale = _fp8_outputs(x, block_rows)
+    t = Fp8BlockTiling(*_rows_cols(x), block_rows)
+    with _on(x):
+        check(load().hc_quantize_fp8_block_launch(_ptr(x), _ptr(q), _ptr(scale), C.byref(t), dtype_code(x),
+                                                  _stream(stream)))
+    return q, scale
+
+
+def dequantize_fp8_block(q, scale, dtype, block_rows: int = 1, stream=None):
+    """The values that 8-bit blocks stand for, in `dtype`."""
+    torch = _torch()
+    x = torch.empty(q.shape, dtype=dtype, device=q.device)
+    qp = _expect(q, "q", q.shape, torch.float8_e4m3fn, q)
+    sp = _expect(scale, "scale", _fp8_scale_shape(q.shape, block_rows), torch.float32, q)
+    t = Fp8BlockTiling(*_rows_cols(q), block_rows)
+    with _on(q):
+        check(load().hc_dequantize_fp8_block_launch(qp, sp, _ptr(x), C.byref(t), dtype_code(x), _stream(stream)))
+    return x
+
+
+def matmul_fp8_block(a, a_scale, b, b_scale, bias=None, dtype=None, stream=None):
+    """C [M, N] = a . b^T (+ bias) with a [M, K] and b [N, K] in 8-bit blocks (block_rows 1 and 128); C and bias
+    of `dtype` (bf16 when not given)."""
+    torch = _torch()
+    dtype = dtype or torch.bfloat16
+    f8 = torch.float8_e4m3fn
+    if a.dim() != 2 or b.dim() != 2 or a.shape[1] != b.shape[1]:
+        raise HcError(HC_ERR_INVALID, "matmul_fp8_block needs a [M, K] and b [N, K]")
+    (M, K), N = a.shape, b.shape[0]
+    ap, bp = _expect(a, "a", (M, K), f8, a), _expect(b, "b", (N, K), f8, a)
+    asp = _expect(a_scale, "a_scale", _fp8_scale_shape((M, K), 1), torch.float32, a)
+    bsp = _expect(b_scale, "b_scale", _fp8_scale_shape((N, K), FP8_BLOCK), torch.float32, a)
+    biasp = None if bias is None else _expect(bias, "bias", (N,), dtype, a)
+    c = torch.empty((M, N), dtype=dtype, device=a.device)
+    t = MatmulFp8BlockTiling(M, K, N)
+    with _on(a):
+        check(load().hc_matmul_fp8_block_launch(ap, asp, bp, bsp, biasp, _ptr(c), C.byref(t), dtype_code(c),
+                                                _stream(stream)))
+    return c
+
+
+def activation_gelu_silu_ckpt(x, act: str, stream=None):
+    """(y, q, scale): act(x) and x in 8-bit blocks for activation_gelu_silu_ckpt_bwd."""
+    if act not in ("gelu", "silu"):
+        raise HcError(HC_ERR_INVALID, f"unknown activation {act!r}")
+    if not x.is_cuda:
+        raise HcError(HC_ERR_INVALID, "expected a CUDA tensor")
+    y = _torch().empty_like(x)
+    q, scale = _fp8_outputs(x, 1)
+    t = ActivationGeluSiluCkptTiling(*_rows_cols(x), 0 if act == "gelu" else 1)
+    with _on(x):
+        check(load().hc_activation_gelu_silu_ckpt_launch(_ptr(x), _ptr(y), _ptr(q), _ptr(scale), C.byref(t),
+                                                         dtype_code(x), _stream(stream)))
+    return y, q, scale
+
+
+def activation_gelu_silu_ckpt_bwd(dy, q, scale, act: str, stream=None):
+    """dx = dy * act'(q * scale)."""
+    torch = _torch()
+    if act not in ("gelu", "silu"):
+        raise HcError(HC_ERR_INVALID, f"unknown activation {act!r}")
+    dx = torch.empty_like(dy)
+    qp = _expect(q, "q", dy.shape, torch.float8_e4m3fn, dy)
+    sp = _expect(scale, "scale", _fp8_scale_shape(dy.shape, 1), torch.float32, dy)
+    t = ActivationGeluSiluCkptTiling(*_rows_cols(dy), 0 if act == "gelu" else 1)
+    with _on(dy):
+        check(load().hc_activation_gelu_silu_ckpt_bwd_launch(_ptr(dy), qp, sp, _ptr(dx), C.byref(t), dtype_code(dy),
+                                                             _stream(stream)))
+    return dx
+
+
+def _ln_fwd(x, gamma, beta, eps, ckpt, stream):
+    torch = _torch()
+    rows, last = _rows_cols(x)
+    gp, bp = (_expect(v, n, (last,), torch.float32, x) for v, n in ((gamma, "gamma"), (beta, "beta")))
+    y = torch.empty_like(x)
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    mean = None if ckpt else torch.empty_like(rstd)
+    q, scale = _fp8_outputs(x, 1) if ckpt else (None, None)
+    t = LayerNormTiling(rows, last, 0, eps)
+    with _on(x):
+        check(load().hc_layer_norm_fwd_train_launch(_ptr(x), gp, bp, _ptr(y), _ptr(mean), _ptr(rstd), _ptr(q),
+                                                    _ptr(scale), C.byref(t), dtype_code(x), _stream(stream)))
+    return y, mean, rstd, q, scale
+
+
+def layer_norm_fwd_train(x, gamma, beta, eps: float, stream=None):
+    """(y, mean, rstd): the layer norm with the statistics that layer_norm_bwd needs."""
+    return _ln_fwd(x, gamma, beta, eps, False, stream)[:3]
+
+
+def layer_norm_ckpt(x, gamma, beta, eps: float, stream=None):
+    """(y, q, scale, rstd): the layer norm, keeping its normalised rows in 8-bit blocks for layer_norm_ckpt_bwd."""
+    y, _, rstd, q, scale = _ln_fwd(x, gamma, beta, eps, True, stream)
+    return y, q, scale, rstd
+
+
+def _ln_bwd_outputs(dy, gamma):
+    torch = _torch()
+    rows, last = _rows_cols(dy)
+    t = LayerNormTiling(rows, last, 0, 0.0)
+    size = _sz()
+    check(load().hc_layer_norm_bwd_workspace_size(C.byref(t), dtype_code(dy), C.byref(size)))
+    work = torch.empty(max(size.value, 1), dtype=torch.uint8, device=dy.device)
+    grads = (torch.empty_like(dy), torch.empty_like(gamma), torch.empty_like(gamma))
+    return t, work, size, grads
+
+
+def layer_norm_bwd(dy, x, gamma, mean, rstd, stream=None):
+    """(dx, dgamma, dbeta) of the layer norm of x, from layer_norm_fwd_train's statistics."""
+    torch = _torch()
+    xp = _expect(x, "x", dy.shape, dy.dtype, dy)
+    gp = _expect(gamma, "gamma", dy.shape[-1:], torch.float32, dy)
+    mp, rp = (_expect(v, n, dy.shape[:-1], torch.float32, dy) for v, n in ((mean, "mean"), (rstd, "rstd")))
+    t, work, size, (dx, dg, db) = _ln_bwd_outputs(dy, gamma)
+    with _on(dy):
+        check(load().hc_layer_norm_bwd_launch(_ptr(dy), xp, gp, mp, rp, _ptr(dx), _ptr(dg), _ptr(db), _ptr(work),
+                                              size.value, C.byref(t), dtype_code(dy), _stream(stream)))
+    return dx, dg, db
+
+
+def layer_norm_ckpt_bwd(dy, q, scale, gamma, rstd, stream=None):
+    """(dx, dgamma, dbeta) from the 8-bit rows that layer_norm_ckpt kept."""
+    torch = _torch()
+    qp = _expect(q, "q", dy.shape, torch.float8_e4m3fn, dy)
+    sp = _expect(scale, "scale", _fp8_scale_shape(dy.shape, 1), torch.float32, dy)
+    gp = _expect(gamma, "gamma", dy.shape[-1:], torch.float32, dy)
+    rp = _expect(rstd, "rstd", dy.shape[:-1], torch.float32, dy)
+    t, work, size, (dx, dg, db) = _ln_bwd_outputs(dy, gamma)
+    with _on(dy):
+        check(load().hc_layer_norm_ckpt_bwd_launch(_ptr(dy), qp, sp, gp, rp, _ptr(dx), _ptr(dg), _ptr(db),
+                                                   _ptr(work), size.value, C.byref(t), dtype_code(dy),
+                                                   _stream(stream)))
+    return dx, dg, db
+
+
 _torch_ops_loaded = False
 
 
@@ -369,7 +576,9 @@ def load_torch_ops():
     """Registers the `hc` torch custom ops (lib/libhc_torch.so, csrc/torch_ops.cpp) and returns torch.ops.hc.
     The ops call the same C ABI as this module, on the current CUDA stream; they raise on CPU tensors.
     hc::flash_attention_fwd_fused gets an autograd formula: hc::flash_attention_bwd (q, k, v get
-    gradients; the lse output is not differentiable)."""
+    gradients; the lse output is not differentiable).  hc::layer_norm_fwd_train, hc::layer_norm_ckpt and
+    hc::activation_gelu_silu_ckpt are differentiable in their first output through their _bwd ops, the latter two
+    from the 8-bit blocks they return, without keeping their input."""
     global _torch_ops_loaded
     torch = _torch()
     if not _torch_ops_loaded:

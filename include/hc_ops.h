@@ -1,5 +1,7 @@
 /*
- * hc_ops.h -- C-ABI kernel launches for the ten ladder operators on B200 (sm_100a).
+ * hc_ops.h -- C-ABI kernel launches for the ten ladder operators on B200 (sm_100a), and for the
+ * operators next to them that the reference does not have (attention backward, layer norm for
+ * training, 8-bit blocks; at the end).
  *
  * Each entry point replaces one AscendC kernel entry
  *   extern "C" __global__ __aicore__ <op>_kernel(GM_ADDR in..., GM_ADDR out..., GM_ADDR workspace,
@@ -11,7 +13,7 @@
  *   - the reference's AscendC "tileNum" field is accepted and ignored: the grid is sized
  *     from the SM count;
  *   - launches are asynchronous on `stream` (cudaStream_t as void*, NULL = default stream);
- *   - there is no workspace argument: no kernel here needs global scratch memory.
+ *   - there is no workspace argument: no ladder kernel needs global scratch memory.
  *
  * Every launch validates its arguments on the host and returns HC_ERR_INVALID /
  * HC_ERR_UNSUPPORTED instead of running; there is no CPU fallback anywhere.
@@ -277,6 +279,96 @@ int hc_flash_attention_bwd_last_path(void);
  * M >= 256: two SMs per 256x256 tile), 0 = none yet. */
 int hc_flash_attention_last_path(void);
 int hc_matmul_bias_last_path(void);
+
+/* ------------------------------------------------------------------------------------------
+ * 8-bit blocks (no counterpart in the reference).
+ *
+ * Format: e4m3 codes, one byte each, with an fp32 scale for each block of 128 elements of a row
+ * (blockRows 1: activations and checkpoints; scale [rows, ceil(cols / 128)]) or for each 128 x 128
+ * tile (blockRows 128: weights; scale [ceil(rows / 128), ceil(cols / 128)]).  Blocks at the end of
+ * a row or column may be short.  With amax = max(max |x| of the block, 2^-100):
+ *     q = e4m3(x * (448 / amax)) to nearest even,  scale = amax / 448,  x ~ q * scale,
+ * every step in fp32, so the codes are the same bits from any implementation.  A block that holds
+ * an infinity or a NaN reads back as NaN.  Relative error of an element within 2^6 * 448 of the
+ * block's largest: at most 2^-4.
+ *
+ * All buffers are dense; outputs must not overlap inputs or each other.  Sizes up to 2^31 - 1
+ * each, element offsets are 64-bit.  Launches with no elements return HC_OK.
+ * ---------------------------------------------------------------------------------------- */
+struct fp8_block_tiling_data {
+    uint32_t rows;
+    uint32_t cols;
+    uint32_t blockRows;  /* 1 or 128 */
+};
+
+/* x [rows, cols] (F32, F16 or BF16) -> q, scale. */
+int hc_quantize_fp8_block_launch(const void* x, void* q, float* scale, const struct fp8_block_tiling_data* t,
+                                 int dtype, void* stream);
+/* q, scale -> x [rows, cols] (F32, F16 or BF16): fp32(q) * scale, rounded once. */
+int hc_dequantize_fp8_block_launch(const void* q, const float* scale, void* x,
+                                   const struct fp8_block_tiling_data* t, int dtype, void* stream);
+
+struct matmul_fp8_block_tiling_data {
+    uint32_t M;
+    uint32_t K;
+    uint32_t N;
+};
+
+/* C[M,N] = A . B^T + bias for a linear layer with 8-bit blocks: a [M,K] with a_scale
+ * [M, ceil(K/128)] (blockRows 1), b [N,K] with b_scale [ceil(N/128), ceil(K/128)] (blockRows 128),
+ * bias [N] of C's type or NULL, C of type `dtype` (F32, F16 or BF16), fp32 sums, one rounding.
+ * K >= 1.  The gradient to A is the same call with the transposed weight and its transposed
+ * scales. */
+int hc_matmul_fp8_block_launch(const void* a, const float* a_scale, const void* b, const float* b_scale,
+                               const void* bias, void* c, const struct matmul_fp8_block_tiling_data* t, int dtype,
+                               void* stream);
+/* Kernel selection of the last successful launch on this thread: 1 tcgen05 with the weight as the
+ * row operand (few tokens), 2 SIMT, 3 tcgen05 CTA pairs, 0 none yet. */
+int hc_matmul_fp8_block_last_path(void);
+
+struct activation_gelu_silu_ckpt_tiling_data {
+    uint32_t rows;
+    uint32_t cols;
+    uint32_t actType;  /* 0 = GELU (tanh form), 1 = SiLU */
+};
+
+/* y = act(x) as hc_activation_gelu_silu_launch gives it, and x in 8-bit blocks (blockRows 1) for
+ * the backward pass. */
+int hc_activation_gelu_silu_ckpt_launch(const void* x, void* y, void* q, float* scale,
+                                        const struct activation_gelu_silu_ckpt_tiling_data* t, int dtype,
+                                        void* stream);
+/* dx = dy * act'(q * scale). */
+int hc_activation_gelu_silu_ckpt_bwd_launch(const void* dy, const void* q, const float* scale, void* dx,
+                                            const struct activation_gelu_silu_ckpt_tiling_data* t, int dtype,
+                                            void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Layer norm for training (no counterpart in the reference, whose ladder is forward only).
+ * ---------------------------------------------------------------------------------------- */
+
+/* The layer norm of x [rows, lastDim] with the statistics its backward needs: y, mean [rows] (may
+ * be NULL) and rstd [rows] = 1 / sqrt(var + eps), fp32.  With q and q_scale (both or neither) the
+ * normalised rows (x - mean) * rstd are also kept in 8-bit blocks (blockRows 1). */
+int hc_layer_norm_fwd_train_launch(const void* x, const float* gamma, const float* beta, void* y, float* mean,
+                                   float* rstd, void* q, float* q_scale, const struct layer_norm_tiling_data* t,
+                                   int dtype, void* stream);
+
+/* Gradients of the layer norm: dx [rows, lastDim] (of x's type), dgamma and dbeta [lastDim] fp32.
+ * With xh = (x - mean) * rstd and g = dy * gamma:
+ *     dx = rstd * (g - mean(g) - xh * mean(g * xh)), dgamma = sum_rows dy * xh, dbeta = sum_rows dy.
+ * No rows: dgamma and dbeta are zero.  `workspace` (16-byte aligned, at least
+ * hc_layer_norm_bwd_workspace_size() bytes, contents irrelevant) holds partial sums between the
+ * launches of one call: calls that may overlap in time need one each.  The sums are added in a
+ * fixed order, so results do not change from call to call. */
+int hc_layer_norm_bwd_workspace_size(const struct layer_norm_tiling_data* t, int dtype, size_t* bytes);
+int hc_layer_norm_bwd_launch(const void* dy, const void* x, const float* gamma, const float* mean, const float* rstd,
+                             void* dx, float* dgamma, float* dbeta, void* workspace, size_t workspace_bytes,
+                             const struct layer_norm_tiling_data* t, int dtype, void* stream);
+/* The same from the 8-bit rows that hc_layer_norm_fwd_train_launch kept: xh = q * q_scale. */
+int hc_layer_norm_ckpt_bwd_launch(const void* dy, const void* q, const float* q_scale, const float* gamma,
+                                  const float* rstd, void* dx, float* dgamma, float* dbeta, void* workspace,
+                                  size_t workspace_bytes, const struct layer_norm_tiling_data* t, int dtype,
+                                  void* stream);
 
 #ifdef __cplusplus
 }
