@@ -6,16 +6,42 @@
 //
 // The sums are fp32 and C is rounded once, to bf16, fp16 or fp32.
 //
-// SIMT path: 64x64 output tiles, 16x16 threads, 4x4 outputs per thread; codes are scaled to fp32 as
-// they are staged (one more fp32 rounding per operand).
+// A block's products go through tcgen05.mma (kind::f8f6f4) into a TMEM accumulator that holds this
+// block alone; an epilogue reads it, multiplies by the block's two scales and adds it to the
+// running sum in registers, while the tensor core works on the next block in another accumulator.
+//
+// Two tensor-core kernels (K a multiple of 16, 16-byte aligned operands):
+//   * CTA pairs, 256x256 tiles, for products that fill the GPU with them;
+//   * otherwise the weight as the 128-row operand and up to 128 tokens as the columns, K split over
+//     a thread-block cluster whose CTAs join their sums through distributed shared memory.
+// SIMT path for the rest: 64x64 output tiles, 16x16 threads, 4x4 outputs per thread; codes are scaled
+// to fp32 as they are staged (one more fp32 rounding per operand).
+// Waits are bounded as in the other tensor-core kernels.
+#include <cuda.h>
 #include <cuda_runtime.h>
+
+#include <mutex>
 
 #include "fp8_block.cuh"
 #include "hc_device.cuh"
 #include "hc_internal.h"
+#include "sm100.cuh"
+#include "tmap.h"
 
 namespace hc {
 namespace mm8 {
+
+using namespace sm100;
+
+enum : uint32_t {
+    kErrProducer = 1u << 0,
+    kErrMmaFull = 1u << 1,
+    kErrMmaAcc = 1u << 2,
+    kErrEpi = 1u << 3,
+    kErrDrain = 1u << 4,
+};
+
+__device__ uint32_t g_mm8_error_word;
 
 struct Params {
     const uint8_t* a;
@@ -25,7 +51,519 @@ struct Params {
     const void* bias;
     void* c;
     uint32_t M, N, K, kb;  // kb = ceil(K / 128)
+    uint32_t nb;           // ceil(N / 128)
+    uint32_t tiles_m, tiles_n, num_tiles;
+    uint32_t vec_store;    // rows of C start on 16-byte boundaries
 };
+
+// K blocks are 128 e4m3 bytes deep: one swizzle row, one scale.
+constexpr uint32_t kBK = 128;
+constexpr uint32_t kPanel = 128 * kBK;  // 16 KB: 128 rows of either operand
+
+// ======================================================================================
+// CTA pairs: 256x256 tiles of C, cta_group::2.  CTA rank r of the pair holds rows
+// [128 r, 128 r + 128) of A and of the result and stages columns [128 r, 128 r + 128) of B.
+//   warp 0      TMA producer: A and B panel of a K block, 32 KB per stage, 6 stages
+//   warp 1      issues the four K=32 MMAs of a block (even CTA, for the pair) into one of two TMEM
+//               accumulators of 256 columns
+//   warps 2-9   promotion: warp w reads TMEM lanes 32 (w % 4) .. + 31 (thread = row) and 128 of the 256
+//               columns, so both scales are one number per thread and block: 128 running sums per
+//               thread, one multiply-add each (as f32x2 pairs)
+// A block costs the tensor core 512 cycles (256 x 256 x 128 at 2 x 8192 products per cycle); reading
+// 128 x 256 accumulators takes 256 (512 B/cycle/SM) and the multiply-adds 256, side by side.
+// ======================================================================================
+constexpr uint32_t kPairStages = 6;
+constexpr uint32_t kPairThreads = 320;
+constexpr uint32_t kPairEpiWarps = 8;
+constexpr uint32_t kPairStageBytes = 2 * kPanel;
+constexpr uint32_t kPairOffTile = kPairStages * kPairStageBytes;                // transposing tiles of the epilogue warps
+constexpr uint32_t kPairOffBar = kPairOffTile + kPairEpiWarps * 32 * 33 * 4;
+constexpr uint32_t kPairSmem = kPairOffBar + 256 + 1024;
+constexpr uint32_t kPairGroupM = 8;  // pair-tile rows per rasterisation group (A and B panels shared in L2)
+
+struct PairBars {
+    uint64_t full[kPairStages], empty[kPairStages];
+    uint64_t acc_full[2], acc_empty[2];
+    uint64_t mma_done;
+};
+
+__device__ __forceinline__ void pair_tile(const Params& p, uint32_t t, uint32_t& tm, uint32_t& tn) {
+    const uint32_t per_group = kPairGroupM * p.tiles_n;
+    const uint32_t g = t / per_group;
+    const uint32_t first_m = g * kPairGroupM;
+    const uint32_t gsize = min(kPairGroupM, p.tiles_m - first_m);
+    const uint32_t r = t - g * per_group;
+    tm = first_m + r % gsize;
+    tn = r / gsize;
+}
+
+// acc[0..15] += d[0..15] * s, two at a time.
+__device__ __forceinline__ void scale_add16(float2* acc, const uint32_t* d, float s) {
+    const float2 s2 = make_float2(s, s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        acc[i] = __ffma2_rn(make_float2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), s2, acc[i]);
+}
+
+// One row's 128 sums to C (vec_store): packs of 16 bytes, the last columns one by one.
+template <typename T>
+__device__ __forceinline__ void store_row(const Params& p, const float2* acc, uint64_t row, uint32_t n0) {
+    constexpr uint32_t P = elem<T>::kPack;
+    const T* bias = static_cast<const T*>(p.bias);
+    T* crow = static_cast<T*>(p.c) + row * p.N;
+#pragma unroll
+    for (uint32_t j = 0; j < 128; j += P) {
+        float v[P];
+#pragma unroll
+        for (uint32_t e = 0; e < P; ++e) {
+            const float2 pr = acc[(j + e) / 2];
+            v[e] = (e & 1) ? pr.y : pr.x;
+            if (bias && n0 + j + e < p.N) v[e] += elem<T>::to_f(bias[n0 + j + e]);
+        }
+        if (n0 + j + P <= p.N) {
+            *reinterpret_cast<pack<T>*>(crow + n0 + j) = pack_from_f<T>(v);
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < P; ++e)
+                if (n0 + j + e < p.N) crow[n0 + j + e] = elem<T>::from_f(v[e]);
+        }
+    }
+}
+
+// A warp's 32 rows x 128 sums to C for any row alignment: 32 x 32 tiles are turned in shared memory
+// so that a store instruction writes 32 neighbouring columns of one row.
+template <typename T>
+__device__ __forceinline__ void store_turned(const Params& p, const float2* acc, float* tile, uint32_t row0, uint32_t n0,
+                                             uint32_t lane) {
+    const T* bias = static_cast<const T*>(p.bias);
+#pragma unroll
+    for (uint32_t c = 0; c < 4; ++c) {
+#pragma unroll
+        for (uint32_t j = 0; j < 32; ++j) tile[lane * 33 + j] = (j & 1) ? acc[c * 16 + j / 2].y : acc[c * 16 + j / 2].x;
+        __syncwarp();
+        const uint32_t n = n0 + c * 32 + lane;
+        const float b = bias && n < p.N ? elem<T>::to_f(bias[n]) : 0.f;
+#pragma unroll 4
+        for (uint32_t r = 0; r < 32; ++r)
+            if (row0 + r < p.M && n < p.N)
+                static_cast<T*>(p.c)[static_cast<uint64_t>(row0 + r) * p.N + n] =
+                    elem<T>::from_f(bias ? tile[r * 33 + lane] + b : tile[r * 33 + lane]);
+        __syncwarp();
+    }
+}
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    mm8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const Params p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    PairBars* bars = reinterpret_cast<PairBars*>(smem + kPairOffBar);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kPairOffBar + sizeof(PairBars));
+    volatile uint32_t* abort_flag = tmem_slot + 1;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();  // 0: issues the MMAs of the pair
+    const uint32_t cluster = blockIdx.x / 2, clusters = gridDim.x / 2;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < kPairStages; ++s) {
+            mbar_init(&bars->full[s], 1);
+            mbar_init(&bars->empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&bars->acc_full[b], 1);
+            mbar_init(&bars->acc_empty[b], 2 * kPairEpiWarps);
+        }
+        mbar_init(&bars->mma_done, 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(tmem_slot, 512);
+        tmem_relinquish_pair();
+    }
+    if (warp == 0 && lane == 0) {
+        prefetch_tmap(&tm_a);
+        prefetch_tmap(&tm_b);
+    }
+    tc_fence_before();
+    cluster_sync_all();  // both CTAs' barriers are initialised before either signals the other
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t s_base = smem_u32(smem);
+
+    if (warp == 0) {
+        // ================================ TMA producers ================================
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0;
+            int32_t pending[kPairStages];
+            for (uint32_t s = 0; s < kPairStages; ++s) pending[s] = -1;
+            bool ok = true, issued = false;
+            for (uint32_t t = cluster; t < p.num_tiles && ok; t += clusters) {
+                uint32_t tm, tn;
+                pair_tile(p, t, tm, tn);
+                const int32_t a_row = static_cast<int32_t>(tm * 256 + rank * 128);
+                const int32_t b_row = static_cast<int32_t>(tn * 256 + rank * 128);
+                for (uint32_t kb = 0; kb < p.kb; ++kb) {
+                    if (!mbar_wait_bounded(&bars->empty[stage], phase ^ 1, abort_flag, &g_mm8_error_word, kErrProducer)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* st = smem + stage * kPairStageBytes;
+                    const uint32_t full_even = mapa_shared(smem_u32(&bars->full[stage]), 0);
+                    if (rank == 0) mbar_arrive_expect_tx(&bars->full[stage], 2 * kPairStageBytes);
+                    tma_load_2d_pair(st, &tm_a, full_even, static_cast<int32_t>(kb * kBK), a_row);
+                    tma_load_2d_pair(st + kPanel, &tm_b, full_even, static_cast<int32_t>(kb * kBK), b_row);
+                    issued = true;
+                    pending[stage] = static_cast<int32_t>(phase);
+                    if (++stage == kPairStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+            if (!ok) {
+                if (rank == 0) {
+                    volatile uint32_t never = 0;
+                    for (uint32_t s = 0; s < kPairStages; ++s)
+                        if (pending[s] >= 0)
+                            mbar_wait_bounded(&bars->full[s], static_cast<uint32_t>(pending[s]), &never,
+                                              &g_mm8_error_word, kErrDrain, 1000000000ull);
+                } else if (issued) {
+                    spin_ns(2000000ull);  // this CTA cannot observe its last copies, which complete on the peer
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ====================== MMA issuer (even CTA, for the pair) =====================
+        if (rank == 0 && lane == 0) {
+            const uint32_t idesc = make_idesc_e4m3(256, 256);
+            uint32_t stage = 0, phase = 0, g = 0;  // g counts K blocks over all tiles
+            bool ok = true;
+            for (uint32_t t = cluster; t < p.num_tiles && ok; t += clusters) {
+                for (uint32_t kb = 0; kb < p.kb; ++kb, ++g) {
+                    const uint32_t ab = g & 1;
+                    if (!mbar_wait_bounded_cluster(&bars->acc_empty[ab], ((g >> 1) & 1) ^ 1, abort_flag,
+                                                   &g_mm8_error_word, kErrMmaAcc) ||
+                        !mbar_wait_bounded_cluster(&bars->full[stage], phase, abort_flag, &g_mm8_error_word,
+                                                   kErrMmaFull)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    Sw128Desc ad = make_sw128_desc2(s_base + stage * kPairStageBytes, 16, 1024);
+                    Sw128Desc bd = make_sw128_desc2(s_base + stage * kPairStageBytes + kPanel, 16, 1024);
+#pragma unroll
+                    for (uint32_t kk = 0; kk < kBK / 32; ++kk) {
+                        mma_f8_ss2_pair(tmem_base + ab * 256, ad, bd, idesc, kk > 0 ? 1u : 0u);
+                        ad.lo += 2;  // 32 bytes along K
+                        bd.lo += 2;
+                    }
+                    tc_commit_pair(&bars->empty[stage], 0x3);
+                    tc_commit_pair(&bars->acc_full[ab], 0x3);
+                    if (++stage == kPairStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+            // All issued MMAs complete before TMEM is freed (normal and error paths alike).
+            tc_commit_pair(&bars->mma_done, 0x1);
+            volatile uint32_t never = 0;
+            mbar_wait_bounded(&bars->mma_done, 0, &never, &g_mm8_error_word, kErrDrain, 1000000000ull);
+        }
+    } else {
+        // ================================== promotion ==================================
+        const uint32_t quarter = warp & 3, half = (warp - 2) / 4;
+        const uint32_t lane_field = (quarter * 32) << 16;
+        float* turn = reinterpret_cast<float*>(smem + kPairOffTile) + (warp - 2) * 32 * 33;
+        const uint32_t empty_even[2] = {mapa_shared(smem_u32(&bars->acc_empty[0]), 0),
+                                        mapa_shared(smem_u32(&bars->acc_empty[1]), 0)};
+        uint32_t g = 0;
+        bool ok = true;
+        for (uint32_t t = cluster; t < p.num_tiles && ok; t += clusters) {
+            uint32_t tm, tn;
+            pair_tile(p, t, tm, tn);
+            const uint32_t row0 = tm * 256 + rank * 128 + quarter * 32;
+            const uint32_t row = row0 + lane, n0 = tn * 256 + half * 128;
+            // rows and columns behind the end: any valid scale, nothing of them is stored
+            const float* sa = p.a_scale + static_cast<uint64_t>(min(row, p.M - 1)) * p.kb;
+            const float* sb = p.b_scale + static_cast<uint64_t>(min(n0 / 128, p.nb - 1)) * p.kb;
+            float2 acc[64];
+#pragma unroll
+            for (int i = 0; i < 64; ++i) acc[i] = make_float2(0.f, 0.f);
+            float sa_next = __ldg(sa), sb_next = __ldg(sb);
+            for (uint32_t kb = 0; kb < p.kb; ++kb, ++g) {
+                const uint32_t ab = g & 1;
+                const float s = sa_next * sb_next;
+                const uint32_t next = min(kb + 1, p.kb - 1);
+                sa_next = __ldg(sa + next);
+                sb_next = __ldg(sb + next);
+                ok = mbar_wait_bounded_cluster(&bars->acc_full[ab], (g >> 1) & 1, abort_flag, &g_mm8_error_word, kErrEpi);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t base = tmem_base + ab * 256 + half * 128 + lane_field;
+                uint32_t d[2][16];
+                tmem_ld16(base, d[0]);
+                tmem_wait_ld16(d[0]);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {  // the next 16 columns are on their way during the multiply-adds
+                    if (c < 7) {
+                        tmem_ld16(base + (c + 1) * 16, d[(c + 1) & 1]);
+                    } else {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(empty_even[ab]);
+                    }
+                    scale_add16(acc + c * 8, d[c & 1], s);
+                    if (c < 7) tmem_wait_ld16(d[(c + 1) & 1]);
+                }
+            }
+            if (!ok) break;
+            if (p.vec_store) {
+                if (row < p.M) store_row<T>(p, acc, row, n0);
+            } else {
+                store_turned<T>(p, acc, turn, row0, n0, lane);
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncwarp();
+    cluster_sync_all();  // neither CTA frees TMEM or exits while the pair still uses its memory
+    tc_fence_after();
+    if (warp == 1) {
+        __syncwarp();
+        tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+// ======================================================================================
+// Few tokens: the transposed product.  A CTA takes 128 rows of the weight as the M operand, TN tokens
+// as the N operand and every S-th run of K blocks; the S CTAs of a cluster then add their sums in
+// rank order through distributed shared memory.  Reading the weight is the work (N K bytes), so S is
+// chosen to give every SM a part of it, and the ring holds all that fits beside a second CTA.
+//   warp 0      TMA producer: 16 KB of weight and TN x 128 bytes of tokens per K block
+//   warp 1      issues M=128, N=TN, K=32 MMAs into one of kAcc accumulators of TN columns
+//   warps 2-5   thread = weight row: acc[t] += d[t] * (token scale * weight scale), the products of
+//               the scales staged in shared memory a block ahead
+// ======================================================================================
+constexpr uint32_t kFewThreads = 192;
+
+template <uint32_t TN>
+struct Few {
+    static constexpr uint32_t kAcc = TN <= 64 ? 4 : 2;
+    static constexpr uint32_t kTokBytes = TN * kBK;
+    static constexpr uint32_t kStageBytes = kPanel + kTokBytes;
+    static constexpr uint32_t kStages = 100 * 1024 / kStageBytes;  // two CTAs per SM
+    static constexpr uint32_t kOffScale = kStages * kStageBytes;   // [2][TN] products of scales
+    static constexpr uint32_t kOffBar = kOffScale + 2 * TN * 4;
+    static constexpr uint32_t kSmem = kOffBar + 512 + 1024;
+    static_assert(TN * 128 * 4 <= kOffScale, "the joined sums reuse the ring");
+};
+
+template <uint32_t TN>
+struct FewBars {
+    uint64_t full[Few<TN>::kStages], empty[Few<TN>::kStages];
+    uint64_t acc_full[Few<TN>::kAcc], acc_empty[Few<TN>::kAcc];
+    uint64_t mma_done;
+};
+
+template <typename T, uint32_t TN>
+__global__ void __launch_bounds__(kFewThreads)
+    mm8_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const Params p,
+                   const uint32_t splits) {
+    using F = Few<TN>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    FewBars<TN>* bars = reinterpret_cast<FewBars<TN>*>(smem + F::kOffBar);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + F::kOffBar + sizeof(FewBars<TN>));
+    volatile uint32_t* abort_flag = tmem_slot + 1;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const uint32_t rank = blockIdx.x;  // grid.x = splits = the cluster
+    const uint32_t n0 = blockIdx.y * 128, m0 = blockIdx.z * TN;
+    // this CTA's K blocks: a contiguous run, lengths differ by one at most
+    const uint32_t kb0 = static_cast<uint32_t>(static_cast<uint64_t>(p.kb) * rank / splits);
+    const uint32_t kb1 = static_cast<uint32_t>(static_cast<uint64_t>(p.kb) * (rank + 1) / splits);
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < F::kStages; ++s) {
+            mbar_init(&bars->full[s], 1);
+            mbar_init(&bars->empty[s], 1);
+        }
+        for (uint32_t b = 0; b < F::kAcc; ++b) {
+            mbar_init(&bars->acc_full[b], 1);
+            mbar_init(&bars->acc_empty[b], 4);
+        }
+        mbar_init(&bars->mma_done, 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, F::kAcc * TN);
+        tmem_relinquish();
+    }
+    if (warp == 0 && lane == 0) {
+        prefetch_tmap(&tm_a);
+        prefetch_tmap(&tm_b);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t s_base = smem_u32(smem);
+
+    float2 acc[TN / 2];
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0;
+            int32_t pending[F::kStages];
+            for (uint32_t s = 0; s < F::kStages; ++s) pending[s] = -1;
+            for (uint32_t kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait_bounded(&bars->empty[stage], phase ^ 1, abort_flag, &g_mm8_error_word, kErrProducer)) {
+                    ok = false;
+                    break;
+                }
+                uint8_t* st = smem + stage * F::kStageBytes;
+                mbar_arrive_expect_tx(&bars->full[stage], F::kStageBytes);
+                tma_load_2d(st, &tm_b, &bars->full[stage], static_cast<int32_t>(kb * kBK), static_cast<int32_t>(n0));
+                tma_load_2d(st + kPanel, &tm_a, &bars->full[stage], static_cast<int32_t>(kb * kBK),
+                            static_cast<int32_t>(m0));
+                pending[stage] = static_cast<int32_t>(phase);
+                if (++stage == F::kStages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+            if (!ok) {
+                volatile uint32_t never = 0;
+                for (uint32_t s = 0; s < F::kStages; ++s)
+                    if (pending[s] >= 0)
+                        mbar_wait_bounded(&bars->full[s], static_cast<uint32_t>(pending[s]), &never, &g_mm8_error_word,
+                                          kErrDrain, 1000000000ull);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t idesc = make_idesc_e4m3(128, TN);
+            uint32_t stage = 0, phase = 0, g = 0;
+            for (uint32_t kb = kb0; kb < kb1; ++kb, ++g) {
+                const uint32_t ab = g % F::kAcc;
+                if (!mbar_wait_bounded(&bars->acc_empty[ab], ((g / F::kAcc) & 1) ^ 1, abort_flag, &g_mm8_error_word,
+                                       kErrMmaAcc) ||
+                    !mbar_wait_bounded(&bars->full[stage], phase, abort_flag, &g_mm8_error_word, kErrMmaFull))
+                    break;
+                tc_fence_after();
+                Sw128Desc wd = make_sw128_desc2(s_base + stage * F::kStageBytes, 16, 1024);
+                Sw128Desc td = make_sw128_desc2(s_base + stage * F::kStageBytes + kPanel, 16, 1024);
+#pragma unroll
+                for (uint32_t kk = 0; kk < kBK / 32; ++kk) {
+                    mma_f8_ss2(tmem_base + ab * TN, wd, td, idesc, kk > 0 ? 1u : 0u);
+                    wd.lo += 2;
+                    td.lo += 2;
+                }
+                tc_commit(&bars->empty[stage]);
+                tc_commit(&bars->acc_full[ab]);
+                if (++stage == F::kStages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+            tc_commit(&bars->mma_done);
+            volatile uint32_t never = 0;
+            mbar_wait_bounded(&bars->mma_done, 0, &never, &g_mm8_error_word, kErrDrain, 1000000000ull);
+        }
+    } else {
+        const uint32_t quarter = warp & 3;
+        const uint32_t lane_field = (quarter * 32) << 16;
+        const uint32_t tid = threadIdx.x - 64;  // 0..127
+        float* prod = reinterpret_cast<float*>(smem + F::kOffScale);
+        const float* sa = p.a_scale + static_cast<uint64_t>(min(m0 + tid, p.M - 1)) * p.kb;
+        const float* sb = p.b_scale + static_cast<uint64_t>(blockIdx.y) * p.kb;
+#pragma unroll
+        for (uint32_t i = 0; i < TN / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+        float next = tid < TN && kb0 < kb1 ? __ldg(sa + kb0) * __ldg(sb + kb0) : 0.f;
+        uint32_t g = 0;
+        for (uint32_t kb = kb0; kb < kb1; ++kb, ++g) {
+            const uint32_t ab = g % F::kAcc;
+            float* sp = prod + (g & 1) * TN;
+            if (tid < TN) {
+                sp[tid] = next;
+                const uint32_t k2 = min(kb + 1, kb1 - 1);
+                next = __ldg(sa + k2) * __ldg(sb + k2);
+            }
+            // the four warps alone; two buffers: a warp two blocks behind cannot be, it has to pass here
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&bars->acc_full[ab], (g / F::kAcc) & 1, abort_flag,
+                                                           &g_mm8_error_word, kErrEpi)))
+                ok = false;
+            if (ok) {
+                tc_fence_after();
+#pragma unroll
+                for (uint32_t c = 0; c < TN; c += 16) {
+                    uint32_t d[16];
+                    tmem_ld16(tmem_base + ab * TN + c + lane_field, d);
+                    tmem_wait_ld16(d);
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i)
+                        acc[c / 2 + i] =
+                            __ffma2_rn(make_float2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])),
+                                       *reinterpret_cast<const float2*>(sp + c + 2 * i), acc[c / 2 + i]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars->acc_empty[ab]);
+            }
+        }
+    }
+
+    // Every MMA and copy of this CTA is done once its promotion warps are through the last block (or
+    // the roles above have drained them), so the ring can hold the sums.
+    __syncwarp();
+    __syncthreads();
+    const uint32_t tid = threadIdx.x - 64;
+    const uint32_t row = (warp & 3) * 32 + lane;  // weight row of this thread's sums
+    float* part = reinterpret_cast<float*>(smem);  // [TN][128]
+    if (splits > 1) {
+        if (warp >= 2) {
+#pragma unroll
+            for (uint32_t i = 0; i < TN / 2; ++i) {
+                part[(2 * i) * 128 + row] = acc[i].x;
+                part[(2 * i + 1) * 128 + row] = acc[i].y;
+            }
+        }
+        cluster_sync_all();
+        // rank r joins and stores tokens r, r + splits, ...
+        if (warp >= 2) {
+            const uint32_t n = n0 + tid;
+            const T* bias = static_cast<const T*>(p.bias);
+            const float b = bias && n < p.N ? elem<T>::to_f(bias[n]) : 0.f;
+            for (uint32_t t = rank; t < TN && m0 + t < p.M; t += splits) {
+                float v = 0.f;
+                for (uint32_t r = 0; r < splits; ++r)
+                    v += ld_cluster_f32(mapa_shared(smem_u32(part + t * 128 + tid), r));
+                if (bias) v += b;
+                if (n < p.N) static_cast<T*>(p.c)[static_cast<uint64_t>(m0 + t) * p.N + n] = elem<T>::from_f(v);
+            }
+        }
+        cluster_sync_all();  // no CTA leaves while its sums may still be read
+    } else if (warp >= 2) {
+        const uint32_t n = n0 + row;
+        const T* bias = static_cast<const T*>(p.bias);
+        const float b = bias && n < p.N ? elem<T>::to_f(bias[n]) : 0.f;
+#pragma unroll
+        for (uint32_t t = 0; t < TN; ++t) {
+            float v = (t & 1) ? acc[t / 2].y : acc[t / 2].x;
+            if (bias) v += b;
+            if (n < p.N && m0 + t < p.M) static_cast<T*>(p.c)[static_cast<uint64_t>(m0 + t) * p.N + n] = elem<T>::from_f(v);
+        }
+    }
+    if (warp == 1) {
+        __syncwarp();
+        tmem_dealloc(tmem_base, F::kAcc * TN);
+    }
+}
 
 template <typename T>
 __global__ void __launch_bounds__(256) mm8_simt_kernel(const Params p) {
@@ -76,15 +614,129 @@ __global__ void __launch_bounds__(256) mm8_simt_kernel(const Params p) {
     }
 }
 
+uint32_t read_error_word(const char** name) {
+    *name = "matmul_fp8_block";
+    uint32_t word = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&word, g_mm8_error_word, sizeof(word)) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    if (word) cudaMemcpyToSymbol(g_mm8_error_word, &zero, sizeof(zero));
+    return word;
+}
+
 thread_local int t_last_path = 0;
 
 template <typename T>
-int launch(const Params& p, cudaStream_t s) {
+int launch_simt(const Params& p, cudaStream_t s) {
     const uint64_t mt = (static_cast<uint64_t>(p.M) + 63) / 64;
     const dim3 grid(static_cast<unsigned>((static_cast<uint64_t>(p.N) + 63) / 64), mt < 65535 ? static_cast<unsigned>(mt) : 65535);
     mm8_simt_kernel<T><<<grid, 256, 0, s>>>(p);
     t_last_path = 2;
     return check_launch("mm8_simt_kernel");
+}
+
+int operand_map(CUtensorMap* out, const uint8_t* base, uint32_t rows, uint32_t K, uint32_t box_rows) {
+    uint64_t dims[2] = {K, rows};
+    uint64_t strides[1] = {K};
+    uint32_t box[2] = {kBK, box_rows};
+    return encode_tmap(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// CTA pairs that fit on the current device at once (cached per device).
+int pair_clusters() {
+    static std::mutex mu;
+    static int cache[64] = {0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+        cudaGetLastError();
+        return 0;
+    }
+    std::lock_guard<std::mutex> lock(mu);
+    if (cache[dev] == 0) {
+        int n = sm_count() / 2;
+        if (set_max_dynamic_smem(reinterpret_cast<const void*>(mm8_pair_kernel<bf16_t>), kPairSmem, "mm8_pair_kernel") ==
+            HC_OK) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(2 * n);
+            cfg.blockDim = dim3(kPairThreads);
+            cfg.dynamicSmemBytes = kPairSmem;
+            int active = 0;
+            if (cudaOccupancyMaxActiveClusters(&active, mm8_pair_kernel<bf16_t>, &cfg) == cudaSuccess && active > 0)
+                n = active < n ? active : n;
+            else
+                cudaGetLastError();
+        }
+        cache[dev] = n > 0 ? n : -1;
+    }
+    return cache[dev] > 0 ? cache[dev] : 0;
+}
+
+template <typename T>
+int launch_pair(Params p, int pairs, cudaStream_t s) {
+    CUtensorMap tma, tmb;
+    if (int rc = operand_map(&tma, p.a, p.M, p.K, 128)) return rc;
+    if (int rc = operand_map(&tmb, p.b, p.N, p.K, 128)) return rc;
+    auto* k = mm8_pair_kernel<T>;
+    if (int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(k), kPairSmem, "mm8_pair_kernel")) return rc;
+    const uint32_t clusters = static_cast<uint32_t>(pairs) < p.num_tiles ? static_cast<uint32_t>(pairs) : p.num_tiles;
+    k<<<2 * clusters, kPairThreads, kPairSmem, s>>>(tma, tmb, p);
+    t_last_path = 3;
+    return check_launch("mm8_pair_kernel");
+}
+
+template <typename T, uint32_t TN>
+int launch_few(const Params& p, cudaStream_t s) {
+    CUtensorMap tma, tmb;
+    if (int rc = operand_map(&tma, p.a, p.M, p.K, TN)) return rc;
+    if (int rc = operand_map(&tmb, p.b, p.N, p.K, 128)) return rc;
+    auto* k = mm8_few_kernel<T, TN>;
+    if (int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(k), Few<TN>::kSmem, "mm8_few_kernel")) return rc;
+    const uint32_t token_tiles = (p.M + TN - 1) / TN;
+    // Splits of K: double while the grid leaves half of the two CTAs per SM free and each split keeps
+    // two blocks.
+    const uint64_t tiles = static_cast<uint64_t>(p.nb) * token_tiles;
+    uint32_t splits = 1;
+    while (splits < 8 && tiles * splits * 2 <= 2ull * sm_count() && p.kb >= 4 * splits) splits *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(splits, p.nb, token_tiles);
+    cfg.blockDim = dim3(kFewThreads);
+    cfg.dynamicSmemBytes = Few<TN>::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = splits;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, k, tma, tmb, p, splits);
+    t_last_path = 1;
+    return check_launch("mm8_few_kernel");
+}
+
+template <typename T>
+int launch(Params p, cudaStream_t s) {
+    const bool tc = p.K % 16 == 0 && aligned16(p.a) && aligned16(p.b);
+    if (!tc) return launch_simt<T>(p, s);
+    static std::once_flag reg_once;
+    std::call_once(reg_once, [] { register_error_word(read_error_word); });
+    p.tiles_m = (p.M + 255) / 256;
+    p.tiles_n = (p.N + 255) / 256;
+    const uint64_t tiles = static_cast<uint64_t>(p.tiles_m) * p.tiles_n;
+    p.vec_store = aligned16(p.c) && (static_cast<uint64_t>(p.N) * sizeof(T)) % 16 == 0;
+    const int pairs = pair_clusters();
+    // grid limits of the few-token kernel: 65535 weight tiles and token tiles
+    const bool few_fits = p.nb <= 65535 && (p.M + 127) / 128 <= 65535;
+    if (tiles > 0x7FFFFFFFull) return launch_simt<T>(p, s);
+    p.num_tiles = static_cast<uint32_t>(tiles);
+    if (pairs > 0 && (!few_fits || (p.M > 128 && tiles * 4 >= static_cast<uint64_t>(pairs) * 3)))
+        return launch_pair<T>(p, pairs, s);
+    if (!few_fits) return launch_simt<T>(p, s);
+    if (p.M <= 16) return launch_few<T, 16>(p, s);
+    if (p.M <= 32) return launch_few<T, 32>(p, s);
+    if (p.M <= 64) return launch_few<T, 64>(p, s);
+    return launch_few<T, 128>(p, s);
 }
 
 }  // namespace mm8
@@ -105,7 +757,7 @@ extern "C" int hc_matmul_fp8_block_launch(const void* a, const float* a_scale, c
     if (!a || !a_scale || !b || !b_scale || !c) return fail(HC_ERR_INVALID, "matmul_fp8_block: null pointer");
     if (fault_hit("launch")) return fail(HC_ERR_INJECTED, "matmul_fp8_block: injected launch failure");
     mm8::Params p{static_cast<const uint8_t*>(a), a_scale, static_cast<const uint8_t*>(b), b_scale, bias, c,
-                  t->M, t->N, t->K, (t->K + kFp8Block - 1) / kFp8Block};
+                  t->M, t->N, t->K, (t->K + kFp8Block - 1) / kFp8Block, (t->N + kFp8Block - 1) / kFp8Block, 0, 0, 0, 0};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (dtype) {
         case HC_DTYPE_F32: return mm8::launch<float>(p, s);

@@ -3,8 +3,8 @@
 // plus the shared-memory matrix descriptors and instruction descriptors tcgen05.mma consumes.
 //
 // Encodings follow the public PTX ISA (tcgen05 "Matrix Descriptors" and "Instruction
-// Descriptor" tables): operands here are 16-bit (bf16/fp16), accumulators fp32, shared-memory
-// tiles use the 128-byte swizzle that TMA writes with CU_TENSOR_MAP_SWIZZLE_128B.
+// Descriptor" tables): operands here are 16-bit (bf16/fp16) or 8-bit (e4m3), accumulators fp32,
+// shared-memory tiles use the 128-byte swizzle that TMA writes with CU_TENSOR_MAP_SWIZZLE_128B.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -236,6 +236,16 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
         : "r"(taddr));
 }
 
+// tcgen05.wait::ld that the 16 registers of an earlier load pass through, so that no use of them can
+// be scheduled before the wait when several loads are in flight.
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -405,6 +415,29 @@ __device__ __forceinline__ void mma_ss2(uint32_t d_tmem, Sw128Desc a, Sw128Desc 
         : "memory");
 }
 
+// The 8-bit forms (kind::f8f6f4, K = 32 per instruction, fp32 accumulation); in the second, A holds
+// 128 rows in each CTA of the pair and B half of the columns.
+__device__ __forceinline__ void mma_f8_ss2(uint32_t d_tmem, Sw128Desc a, Sw128Desc b, uint32_t idesc,
+                                           uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %5, p;\n\t}" ::"r"(d_tmem),
+        "r"(a.lo), "r"(a.hi), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_f8_ss2_pair(uint32_t d_tmem, Sw128Desc a, Sw128Desc b, uint32_t idesc,
+                                                uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %5, p;\n\t}" ::"r"(d_tmem),
+        "r"(a.lo), "r"(a.hi), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 // D(tmem) (+)= A(tmem) * B(smem desc), the descriptor given as words.
 __device__ __forceinline__ void mma_ts2(uint32_t d_tmem, uint32_t a_tmem, Sw128Desc b, uint32_t idesc,
                                         uint32_t accumulate) {
@@ -458,6 +491,18 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(bool bf16, uint32_t M, uin
                                                       bool b_mn_major) {
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_mn_major ? 1u : 0u) << 15) |
            ((b_mn_major ? 1u : 0u) << 16) | ((N >> 3) << 17) | ((M >> 4) << 24);
+}
+
+// The same for kind::f8f6f4 with e4m3 operands (format 0), both K-major, fp32 accumulation.
+__host__ __device__ constexpr uint32_t make_idesc_e4m3(uint32_t M, uint32_t N) {
+    return (1u << 4) | ((N >> 3) << 17) | ((M >> 4) << 24);
+}
+
+// fp32 read of another CTA's shared memory, by its shared::cluster address.
+__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+    return v;
 }
 
 }  // namespace sm100
