@@ -39,6 +39,7 @@ enum : uint32_t {
     kErrMmaAcc = 1u << 2,
     kErrEpi = 1u << 3,
     kErrDrain = 1u << 4,
+    kErrScale = 1u << 5,
 };
 
 __device__ uint32_t g_mm8_error_word;
@@ -64,26 +65,36 @@ constexpr uint32_t kPanel = 128 * kBK;  // 16 KB: 128 rows of either operand
 // CTA pairs: 256x256 tiles of C, cta_group::2.  CTA rank r of the pair holds rows
 // [128 r, 128 r + 128) of A and of the result and stages columns [128 r, 128 r + 128) of B.
 //   warp 0      TMA producer: A and B panel of a K block, 32 KB per stage, 6 stages
-//   warp 1      issues the four K=32 MMAs of a block (even CTA, for the pair) into one of two TMEM
-//               accumulators of 256 columns
-//   warps 2-9   promotion: warp w reads TMEM lanes 32 (w % 4) .. + 31 (thread = row) and 128 of the 256
-//               columns, so both scales are one number per thread and block: 128 running sums per
-//               thread, one multiply-add each (as f32x2 pairs)
-// A block costs the tensor core 512 cycles (256 x 256 x 128 at 2 x 8192 products per cycle); reading
-// 128 x 256 accumulators takes 256 (512 B/cycle/SM) and the multiply-adds 256, side by side.
+//   warp 1      issues the MMAs of a block (even CTA, for the pair): M=256, N=128, K=32, first for the
+//               lower 64 columns of each CTA's B panel, then for the upper 64
+//   warps 2-17  promotion: warp w reads TMEM lanes 32 (w % 4) .. + 31 (thread = row) and 64 columns of one
+//               half, which lie in one 128-block of N, so both scales are one number per thread
+//               and block: 64 running sums per thread, one multiply-add each (as f32x2 pairs)
+//   warps 18-19 products of the scales for four K blocks at a time, row by row into shared memory:
+//               read by the promoting threads themselves (32 rows, 32 lines each) they cost a third
+//               of the time
+// "Accumulator read" goes straight to the even CTA's barrier with a release at CTA scope (no data in
+// memory hangs on it: the TMEM reads are complete and ordered by the tcgen05 fences); a release
+// at cluster scope takes about 1000 cycles here, several times the block itself.
+// TMEM holds four accumulators of 128 columns: two halves, two blocks.  A half costs the tensor
+// core 256 cycles (256 x 128 x 128 products at 2 x 8192 per cycle) and its accumulator is needed
+// again 1024 cycles after, which leaves 768 for the commit, the read (128 cycles at 512 B/cycle/SM)
+// and the arrival from both CTAs.
 // ======================================================================================
 constexpr uint32_t kPairStages = 6;
-constexpr uint32_t kPairThreads = 320;
-constexpr uint32_t kPairEpiWarps = 8;
+constexpr uint32_t kPairEpiWarps = 16;
+constexpr uint32_t kPairThreads = 64 + 32 * kPairEpiWarps + 64;
 constexpr uint32_t kPairStageBytes = 2 * kPanel;
-constexpr uint32_t kPairOffTile = kPairStages * kPairStageBytes;                // transposing tiles of the epilogue warps
-constexpr uint32_t kPairOffBar = kPairOffTile + kPairEpiWarps * 32 * 33 * 4;
+constexpr uint32_t kPairOffTurn = kPairStages * kPairStageBytes;             // turning tiles of the promoting warps
+constexpr uint32_t kPairOffScale = kPairOffTurn + kPairEpiWarps * 32 * 8 * 4;  // [2 groups][4 blocks][2 panels][128]
+constexpr uint32_t kPairOffBar = kPairOffScale + 2 * 4 * 256 * 4;
 constexpr uint32_t kPairSmem = kPairOffBar + 256 + 1024;
 constexpr uint32_t kPairGroupM = 8;  // pair-tile rows per rasterisation group (A and B panels shared in L2)
 
 struct PairBars {
     uint64_t full[kPairStages], empty[kPairStages];
-    uint64_t acc_full[2], acc_empty[2];
+    uint64_t acc_full[4], acc_empty[4];  // [block & 1][half]
+    uint64_t sc_full[2], sc_empty[2];    // [group of four blocks & 1]
     uint64_t mma_done;
 };
 
@@ -105,14 +116,14 @@ __device__ __forceinline__ void scale_add16(float2* acc, const uint32_t* d, floa
         acc[i] = __ffma2_rn(make_float2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), s2, acc[i]);
 }
 
-// One row's 128 sums to C (vec_store): packs of 16 bytes, the last columns one by one.
+// 64 sums of one row to C (vec_store): packs of 16 bytes, the last columns one by one.
 template <typename T>
 __device__ __forceinline__ void store_row(const Params& p, const float2* acc, uint64_t row, uint32_t n0) {
     constexpr uint32_t P = elem<T>::kPack;
     const T* bias = static_cast<const T*>(p.bias);
     T* crow = static_cast<T*>(p.c) + row * p.N;
 #pragma unroll
-    for (uint32_t j = 0; j < 128; j += P) {
+    for (uint32_t j = 0; j < 64; j += P) {
         float v[P];
 #pragma unroll
         for (uint32_t e = 0; e < P; ++e) {
@@ -130,24 +141,27 @@ __device__ __forceinline__ void store_row(const Params& p, const float2* acc, ui
     }
 }
 
-// A warp's 32 rows x 128 sums to C for any row alignment: 32 x 32 tiles are turned in shared memory
-// so that a store instruction writes 32 neighbouring columns of one row.
+// A warp's 32 rows x 64 sums to C for any row alignment: 32 x 8 tiles are turned in shared memory so
+// that a store instruction writes 8 neighbouring columns of four rows; row r is rotated by r / 4
+// columns, which spreads both the writes and the reads over all banks.
 template <typename T>
 __device__ __forceinline__ void store_turned(const Params& p, const float2* acc, float* tile, uint32_t row0, uint32_t n0,
                                              uint32_t lane) {
     const T* bias = static_cast<const T*>(p.bias);
 #pragma unroll
-    for (uint32_t c = 0; c < 4; ++c) {
+    for (uint32_t c = 0; c < 8; ++c) {
 #pragma unroll
-        for (uint32_t j = 0; j < 32; ++j) tile[lane * 33 + j] = (j & 1) ? acc[c * 16 + j / 2].y : acc[c * 16 + j / 2].x;
+        for (uint32_t j = 0; j < 8; ++j)
+            tile[lane * 8 + (j + lane / 4) % 8] = (j & 1) ? acc[c * 4 + j / 2].y : acc[c * 4 + j / 2].x;
         __syncwarp();
-        const uint32_t n = n0 + c * 32 + lane;
+        const uint32_t n = n0 + c * 8 + lane % 8;
         const float b = bias && n < p.N ? elem<T>::to_f(bias[n]) : 0.f;
 #pragma unroll 4
-        for (uint32_t r = 0; r < 32; ++r)
-            if (row0 + r < p.M && n < p.N)
-                static_cast<T*>(p.c)[static_cast<uint64_t>(row0 + r) * p.N + n] =
-                    elem<T>::from_f(bias ? tile[r * 33 + lane] + b : tile[r * 33 + lane]);
+        for (uint32_t r = lane / 8; r < 32; r += 4)
+            if (row0 + r < p.M && n < p.N) {
+                const float v = tile[r * 8 + (lane + r / 4) % 8];
+                static_cast<T*>(p.c)[static_cast<uint64_t>(row0 + r) * p.N + n] = elem<T>::from_f(bias ? v + b : v);
+            }
         __syncwarp();
     }
 }
@@ -169,9 +183,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             mbar_init(&bars->full[s], 1);
             mbar_init(&bars->empty[s], 1);
         }
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < 4; ++b) {
             mbar_init(&bars->acc_full[b], 1);
-            mbar_init(&bars->acc_empty[b], 2 * kPairEpiWarps);
+            mbar_init(&bars->acc_empty[b], kPairEpiWarps);  // half of each CTA's promoting warps
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&bars->sc_full[b], 2);
+            mbar_init(&bars->sc_empty[b], kPairEpiWarps);
         }
         mbar_init(&bars->mma_done, 1);
         *abort_flag = 0;
@@ -236,30 +254,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     } else if (warp == 1) {
         // ====================== MMA issuer (even CTA, for the pair) =====================
         if (rank == 0 && lane == 0) {
-            const uint32_t idesc = make_idesc_e4m3(256, 256);
+            const uint32_t idesc = make_idesc_e4m3(256, 128);
             uint32_t stage = 0, phase = 0, g = 0;  // g counts K blocks over all tiles
             bool ok = true;
             for (uint32_t t = cluster; t < p.num_tiles && ok; t += clusters) {
-                for (uint32_t kb = 0; kb < p.kb; ++kb, ++g) {
-                    const uint32_t ab = g & 1;
-                    if (!mbar_wait_bounded_cluster(&bars->acc_empty[ab], ((g >> 1) & 1) ^ 1, abort_flag,
-                                                   &g_mm8_error_word, kErrMmaAcc) ||
-                        !mbar_wait_bounded_cluster(&bars->full[stage], phase, abort_flag, &g_mm8_error_word,
-                                                   kErrMmaFull)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    Sw128Desc ad = make_sw128_desc2(s_base + stage * kPairStageBytes, 16, 1024);
-                    Sw128Desc bd = make_sw128_desc2(s_base + stage * kPairStageBytes + kPanel, 16, 1024);
+                for (uint32_t kb = 0; kb < p.kb && ok; ++kb, ++g) {
+                    const Sw128Desc a0 = make_sw128_desc2(s_base + stage * kPairStageBytes, 16, 1024);
 #pragma unroll
-                    for (uint32_t kk = 0; kk < kBK / 32; ++kk) {
-                        mma_f8_ss2_pair(tmem_base + ab * 256, ad, bd, idesc, kk > 0 ? 1u : 0u);
-                        ad.lo += 2;  // 32 bytes along K
-                        bd.lo += 2;
+                    for (uint32_t h = 0; h < 2; ++h) {
+                        const uint32_t ab = (g & 1) * 2 + h;
+                        if (!mbar_wait_bounded(&bars->acc_empty[ab], ((g >> 1) & 1) ^ 1, abort_flag,
+                                                       &g_mm8_error_word, kErrMmaAcc) ||
+                            (h == 0 && !mbar_wait_bounded(&bars->full[stage], phase, abort_flag,
+                                                                  &g_mm8_error_word, kErrMmaFull))) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        Sw128Desc ad = a0, bd = a0;
+                        bd.lo += (kPanel + h * 64 * kBK) >> 4;
+#pragma unroll
+                        for (uint32_t kk = 0; kk < kBK / 32; ++kk) {
+                            mma_f8_ss2_pair(tmem_base + ab * 128, ad, bd, idesc, kk > 0 ? 1u : 0u);
+                            ad.lo += 2;  // 32 bytes along K
+                            bd.lo += 2;
+                        }
+                        if (h == 1) tc_commit_pair(&bars->empty[stage], 0x3);
+                        tc_commit_pair(&bars->acc_full[ab], 0x3);
                     }
-                    tc_commit_pair(&bars->empty[stage], 0x3);
-                    tc_commit_pair(&bars->acc_full[ab], 0x3);
                     if (++stage == kPairStages) {
                         stage = 0;
                         phase ^= 1;
@@ -271,52 +293,93 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             volatile uint32_t never = 0;
             mbar_wait_bounded(&bars->mma_done, 0, &never, &g_mm8_error_word, kErrDrain, 1000000000ull);
         }
+    } else if (warp >= 2 + kPairEpiWarps) {
+        // ============================= products of the scales =============================
+        // two rows per thread; the loads of the next four blocks are under way while the last are read
+        const uint32_t r = (warp - 2 - kPairEpiWarps) * 32 + lane;
+        float* ring = reinterpret_cast<float*>(smem + kPairOffScale);
+        uint32_t sg = 0;
+        bool ok = true;
+        for (uint32_t t = cluster; t < p.num_tiles && ok; t += clusters) {
+            uint32_t tm, tn;
+            pair_tile(p, t, tm, tn);
+            // rows and columns behind the end: any valid scale, nothing of them is stored
+            const uint32_t row = tm * 256 + rank * 128 + r;
+            const float* sa[2] = {p.a_scale + static_cast<uint64_t>(min(row, p.M - 1)) * p.kb,
+                                  p.a_scale + static_cast<uint64_t>(min(row + 64, p.M - 1)) * p.kb};
+            const float* sb[2] = {p.b_scale + static_cast<uint64_t>(min(tn * 2, p.nb - 1)) * p.kb,
+                                  p.b_scale + static_cast<uint64_t>(min(tn * 2 + 1, p.nb - 1)) * p.kb};
+            for (uint32_t kb = 0; kb < p.kb; kb += 4, ++sg) {
+                float va[2][4], vb[2][4];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const uint32_t k = min(kb + i, p.kb - 1);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        va[j][i] = __ldg(sa[j] + k);
+                        vb[j][i] = __ldg(sb[j] + k);
+                    }
+                }
+                ok = mbar_wait_bounded(&bars->sc_empty[sg & 1], ((sg >> 1) & 1) ^ 1, abort_flag, &g_mm8_error_word,
+                                       kErrScale);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                float* out = ring + (sg & 1) * 1024 + r;
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int pn = 0; pn < 2; ++pn) {
+                        out[i * 256 + pn * 128] = va[0][i] * vb[pn][i];
+                        out[i * 256 + pn * 128 + 64] = va[1][i] * vb[pn][i];
+                    }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars->sc_full[sg & 1]);
+            }
+        }
     } else {
         // ================================== promotion ==================================
-        const uint32_t quarter = warp & 3, half = (warp - 2) / 4;
+        const uint32_t quarter = warp & 3, part = (warp - 2) / 4;  // part: 64 of the 256 columns
+        const uint32_t half = part & 1, panel = part / 2;
         const uint32_t lane_field = (quarter * 32) << 16;
-        float* turn = reinterpret_cast<float*>(smem + kPairOffTile) + (warp - 2) * 32 * 33;
-        const uint32_t empty_even[2] = {mapa_shared(smem_u32(&bars->acc_empty[0]), 0),
-                                        mapa_shared(smem_u32(&bars->acc_empty[1]), 0)};
-        uint32_t g = 0;
+        const uint32_t empty_even = mapa_shared(smem_u32(&bars->acc_empty[half]), 0);
+        float* turn = reinterpret_cast<float*>(smem + kPairOffTurn) + (warp - 2) * 32 * 8;
+        const float* ring = reinterpret_cast<const float*>(smem + kPairOffScale) + panel * 128 + quarter * 32 + lane;
+        uint32_t g = 0, sg = 0;
         bool ok = true;
         for (uint32_t t = cluster; t < p.num_tiles && ok; t += clusters) {
             uint32_t tm, tn;
             pair_tile(p, t, tm, tn);
             const uint32_t row0 = tm * 256 + rank * 128 + quarter * 32;
-            const uint32_t row = row0 + lane, n0 = tn * 256 + half * 128;
-            // rows and columns behind the end: any valid scale, nothing of them is stored
-            const float* sa = p.a_scale + static_cast<uint64_t>(min(row, p.M - 1)) * p.kb;
-            const float* sb = p.b_scale + static_cast<uint64_t>(min(n0 / 128, p.nb - 1)) * p.kb;
-            float2 acc[64];
+            // accumulator columns [64 panel, + 64) of a half are columns [64 half, + 64) of CTA `panel`'s B panel
+            const uint32_t row = row0 + lane, n0 = tn * 256 + panel * 128 + half * 64;
+            float2 acc[32];
 #pragma unroll
-            for (int i = 0; i < 64; ++i) acc[i] = make_float2(0.f, 0.f);
-            float sa_next = __ldg(sa), sb_next = __ldg(sb);
+            for (int i = 0; i < 32; ++i) acc[i] = make_float2(0.f, 0.f);
             for (uint32_t kb = 0; kb < p.kb; ++kb, ++g) {
-                const uint32_t ab = g & 1;
-                const float s = sa_next * sb_next;
-                const uint32_t next = min(kb + 1, p.kb - 1);
-                sa_next = __ldg(sa + next);
-                sb_next = __ldg(sb + next);
-                ok = mbar_wait_bounded_cluster(&bars->acc_full[ab], (g >> 1) & 1, abort_flag, &g_mm8_error_word, kErrEpi);
+                const uint32_t ab = (g & 1) * 2 + half;
+                if (kb % 4 == 0)
+                    ok = mbar_wait_bounded(&bars->sc_full[sg & 1], (sg >> 1) & 1, abort_flag, &g_mm8_error_word, kErrScale);
+                const float s = ring[(sg & 1) * 1024 + (kb % 4) * 256];
+                ok = ok && mbar_wait_bounded(&bars->acc_full[ab], (g >> 1) & 1, abort_flag, &g_mm8_error_word, kErrEpi);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t base = tmem_base + ab * 256 + half * 128 + lane_field;
-                uint32_t d[2][16];
-                tmem_ld16(base, d[0]);
-                tmem_wait_ld16(d[0]);
+                const uint32_t base = tmem_base + ab * 128 + panel * 64 + lane_field;
+                uint32_t d[16];  // 64 sums + 16: a block of 576 threads leaves a thread 96 registers
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {  // the next 16 columns are on their way during the multiply-adds
-                    if (c < 7) {
-                        tmem_ld16(base + (c + 1) * 16, d[(c + 1) & 1]);
-                    } else {
+                for (uint32_t c = 0; c < 4; ++c) {
+                    tmem_ld16(base + c * 16, d);
+                    tmem_wait_ld16(d);
+                    if (c == 3) {
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(empty_even[ab]);
+                        if (lane == 0) mbar_arrive_peer(empty_even + (g & 1) * 16);
                     }
-                    scale_add16(acc + c * 8, d[c & 1], s);
-                    if (c < 7) tmem_wait_ld16(d[(c + 1) & 1]);
+                    scale_add16(acc + c * 8, d, s);
+                }
+                if (kb % 4 == 3 || kb + 1 == p.kb) {
+                    if (lane == 0) mbar_arrive(&bars->sc_empty[sg & 1]);  // after the __syncwarp above
+                    ++sg;
                 }
             }
             if (!ok) break;
