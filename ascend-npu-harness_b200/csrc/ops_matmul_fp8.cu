@@ -67,12 +67,14 @@ constexpr uint32_t kPanel = 128 * kBK;  // 16 KB: 128 rows of either operand
 //   warp 0      TMA producer: A and B panel of a K block, 32 KB per stage, 6 stages
 //   warp 1      issues the MMAs of a block (even CTA, for the pair): M=256, N=128, K=32, first for the
 //               lower 64 columns of each CTA's B panel, then for the upper 64
-//   warps 2-17  promotion: warp w reads TMEM lanes 32 (w % 4) .. + 31 (thread = row) and 64 columns of one
-//               half, which lie in one 128-block of N, so both scales are one number per thread
-//               and block: 64 running sums per thread, one multiply-add each (as f32x2 pairs)
-//   warps 18-19 products of the scales for four K blocks at a time, row by row into shared memory:
-//               read by the promoting threads themselves (32 rows, 32 lines each) they cost a third
-//               of the time
+//   warps 2-3   products of the scales for four K blocks at a time, row by row into shared memory: read
+//               by the promoting threads themselves (32 rows, 32 lines each) they cost a third of the time
+//   warps 4-11  promotion: warp w reads TMEM lanes 32 (w % 4) .. + 31 (thread = row) and the 128 columns of
+//               one half, 64 of either 128-block of N, so a thread has two scales per block: 128
+//               running sums per thread, one multiply-add each (as f32x2 pairs), the next 32 columns
+//               on their way meanwhile.  Registers: 72 / 216 per thread of the two kinds of warps
+//               (4 x 32 x 72 + 8 x 32 x 216 = 384 x 168, what the block is launched with).  Sixteen
+//               warps of 64 columns each spent more on waits than on sums: 748 us at 8192^3.
 // "Accumulator read" goes straight to the even CTA's barrier with a release at CTA scope (no data in
 // memory hangs on it: the TMEM reads are complete and ordered by the tcgen05 fences); a release
 // at cluster scope takes about 1000 cycles here, several times the block itself.
@@ -82,11 +84,11 @@ constexpr uint32_t kPanel = 128 * kBK;  // 16 KB: 128 rows of either operand
 // and the arrival from both CTAs.
 // ======================================================================================
 constexpr uint32_t kPairStages = 6;
-constexpr uint32_t kPairEpiWarps = 16;
-constexpr uint32_t kPairThreads = 64 + 32 * kPairEpiWarps + 64;
+constexpr uint32_t kPairEpiWarps = 8;
+constexpr uint32_t kPairThreads = 128 + 32 * kPairEpiWarps;
 constexpr uint32_t kPairStageBytes = 2 * kPanel;
 constexpr uint32_t kPairOffTurn = kPairStages * kPairStageBytes;             // turning tiles of the promoting warps
-constexpr uint32_t kPairOffScale = kPairOffTurn + kPairEpiWarps * 32 * 8 * 4;  // [2 groups][4 blocks][2 panels][128]
+constexpr uint32_t kPairOffScale = kPairOffTurn + kPairEpiWarps * 32 * 16 * 4;  // [2 groups][4 blocks][2 panels][128]
 constexpr uint32_t kPairOffBar = kPairOffScale + 2 * 4 * 256 * 4;
 constexpr uint32_t kPairSmem = kPairOffBar + 256 + 1024;
 constexpr uint32_t kPairGroupM = 8;  // pair-tile rows per rasterisation group (A and B panels shared in L2)
@@ -108,11 +110,11 @@ __device__ __forceinline__ void pair_tile(const Params& p, uint32_t t, uint32_t&
     tn = r / gsize;
 }
 
-// acc[0..15] += d[0..15] * s, two at a time.
-__device__ __forceinline__ void scale_add16(float2* acc, const uint32_t* d, float s) {
+// acc += d * s over 32 columns, two at a time.
+__device__ __forceinline__ void scale_add32(float2* acc, const uint32_t (&d)[32], float s) {
     const float2 s2 = make_float2(s, s);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 16; ++i)
         acc[i] = __ffma2_rn(make_float2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), s2, acc[i]);
 }
 
@@ -141,25 +143,25 @@ __device__ __forceinline__ void store_row(const Params& p, const float2* acc, ui
     }
 }
 
-// A warp's 32 rows x 64 sums to C for any row alignment: 32 x 8 tiles are turned in shared memory so
-// that a store instruction writes 8 neighbouring columns of four rows; row r is rotated by r / 4
+// A warp's 32 rows x 64 sums to C for any row alignment: 32 x 16 tiles are turned in shared memory so
+// that a store instruction writes 16 neighbouring columns of two rows; row r is rotated by r / 2
 // columns, which spreads both the writes and the reads over all banks.
 template <typename T>
 __device__ __forceinline__ void store_turned(const Params& p, const float2* acc, float* tile, uint32_t row0, uint32_t n0,
                                              uint32_t lane) {
     const T* bias = static_cast<const T*>(p.bias);
 #pragma unroll
-    for (uint32_t c = 0; c < 8; ++c) {
+    for (uint32_t c = 0; c < 4; ++c) {
 #pragma unroll
-        for (uint32_t j = 0; j < 8; ++j)
-            tile[lane * 8 + (j + lane / 4) % 8] = (j & 1) ? acc[c * 4 + j / 2].y : acc[c * 4 + j / 2].x;
+        for (uint32_t j = 0; j < 16; ++j)
+            tile[lane * 16 + (j + lane / 2) % 16] = (j & 1) ? acc[c * 8 + j / 2].y : acc[c * 8 + j / 2].x;
         __syncwarp();
-        const uint32_t n = n0 + c * 8 + lane % 8;
+        const uint32_t n = n0 + c * 16 + lane % 16;
         const float b = bias && n < p.N ? elem<T>::to_f(bias[n]) : 0.f;
 #pragma unroll 4
-        for (uint32_t r = lane / 8; r < 32; r += 4)
+        for (uint32_t r = lane / 16; r < 32; r += 2)
             if (row0 + r < p.M && n < p.N) {
-                const float v = tile[r * 8 + (lane + r / 4) % 8];
+                const float v = tile[r * 16 + (lane + r / 2) % 16];
                 static_cast<T*>(p.c)[static_cast<uint64_t>(row0 + r) * p.N + n] = elem<T>::from_f(bias ? v + b : v);
             }
         __syncwarp();
@@ -185,7 +187,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         }
         for (int b = 0; b < 4; ++b) {
             mbar_init(&bars->acc_full[b], 1);
-            mbar_init(&bars->acc_empty[b], kPairEpiWarps);  // half of each CTA's promoting warps
+            mbar_init(&bars->acc_empty[b], kPairEpiWarps);  // those of one half in either CTA
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&bars->sc_full[b], 2);
@@ -209,184 +211,194 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const uint32_t tmem_base = *tmem_slot;
     const uint32_t s_base = smem_u32(smem);
 
-    if (warp == 0) {
-        // ================================ TMA producers ================================
-        if (lane == 0) {
-            uint32_t stage = 0, phase = 0;
-            int32_t pending[kPairStages];
-            for (uint32_t s = 0; s < kPairStages; ++s) pending[s] = -1;
-            bool ok = true, issued = false;
-            for (uint32_t t = cluster; t < p.num_tiles && ok; t += clusters) {
-                uint32_t tm, tn;
-                pair_tile(p, t, tm, tn);
-                const int32_t a_row = static_cast<int32_t>(tm * 256 + rank * 128);
-                const int32_t b_row = static_cast<int32_t>(tn * 256 + rank * 128);
-                for (uint32_t kb = 0; kb < p.kb; ++kb) {
-                    if (!mbar_wait_bounded(&bars->empty[stage], phase ^ 1, abort_flag, &g_mm8_error_word, kErrProducer)) {
-                        ok = false;
-                        break;
-                    }
-                    uint8_t* st = smem + stage * kPairStageBytes;
-                    const uint32_t full_even = mapa_shared(smem_u32(&bars->full[stage]), 0);
-                    if (rank == 0) mbar_arrive_expect_tx(&bars->full[stage], 2 * kPairStageBytes);
-                    tma_load_2d_pair(st, &tm_a, full_even, static_cast<int32_t>(kb * kBK), a_row);
-                    tma_load_2d_pair(st + kPanel, &tm_b, full_even, static_cast<int32_t>(kb * kBK), b_row);
-                    issued = true;
-                    pending[stage] = static_cast<int32_t>(phase);
-                    if (++stage == kPairStages) {
-                        stage = 0;
-                        phase ^= 1;
-                    }
-                }
-            }
-            if (!ok) {
-                if (rank == 0) {
-                    volatile uint32_t never = 0;
-                    for (uint32_t s = 0; s < kPairStages; ++s)
-                        if (pending[s] >= 0)
-                            mbar_wait_bounded(&bars->full[s], static_cast<uint32_t>(pending[s]), &never,
-                                              &g_mm8_error_word, kErrDrain, 1000000000ull);
-                } else if (issued) {
-                    spin_ns(2000000ull);  // this CTA cannot observe its last copies, which complete on the peer
-                }
-            }
-        }
-    } else if (warp == 1) {
-        // ====================== MMA issuer (even CTA, for the pair) =====================
-        if (rank == 0 && lane == 0) {
-            const uint32_t idesc = make_idesc_e4m3(256, 128);
-            uint32_t stage = 0, phase = 0, g = 0;  // g counts K blocks over all tiles
-            bool ok = true;
-            for (uint32_t t = cluster; t < p.num_tiles && ok; t += clusters) {
-                for (uint32_t kb = 0; kb < p.kb && ok; ++kb, ++g) {
-                    const Sw128Desc a0 = make_sw128_desc2(s_base + stage * kPairStageBytes, 16, 1024);
-#pragma unroll
-                    for (uint32_t h = 0; h < 2; ++h) {
-                        const uint32_t ab = (g & 1) * 2 + h;
-                        if (!mbar_wait_bounded(&bars->acc_empty[ab], ((g >> 1) & 1) ^ 1, abort_flag,
-                                                       &g_mm8_error_word, kErrMmaAcc) ||
-                            (h == 0 && !mbar_wait_bounded(&bars->full[stage], phase, abort_flag,
-                                                                  &g_mm8_error_word, kErrMmaFull))) {
+    if (warp < 4) {
+        setmaxnreg_dec<72>();
+        if (warp == 0) {
+            // ================================ TMA producers ================================
+            if (lane == 0) {
+                uint32_t stage = 0, phase = 0;
+                int32_t pending[kPairStages];
+                for (uint32_t s = 0; s < kPairStages; ++s) pending[s] = -1;
+                bool ok = true, issued = false;
+                for (uint32_t t = cluster; t < p.num_tiles && ok; t += clusters) {
+                    uint32_t tm, tn;
+                    pair_tile(p, t, tm, tn);
+                    const int32_t a_row = static_cast<int32_t>(tm * 256 + rank * 128);
+                    const int32_t b_row = static_cast<int32_t>(tn * 256 + rank * 128);
+                    for (uint32_t kb = 0; kb < p.kb; ++kb) {
+                        if (!mbar_wait_bounded(&bars->empty[stage], phase ^ 1, abort_flag, &g_mm8_error_word, kErrProducer)) {
                             ok = false;
                             break;
                         }
-                        tc_fence_after();
-                        Sw128Desc ad = a0, bd = a0;
-                        bd.lo += (kPanel + h * 64 * kBK) >> 4;
-#pragma unroll
-                        for (uint32_t kk = 0; kk < kBK / 32; ++kk) {
-                            mma_f8_ss2_pair(tmem_base + ab * 128, ad, bd, idesc, kk > 0 ? 1u : 0u);
-                            ad.lo += 2;  // 32 bytes along K
-                            bd.lo += 2;
+                        uint8_t* st = smem + stage * kPairStageBytes;
+                        const uint32_t full_even = mapa_shared(smem_u32(&bars->full[stage]), 0);
+                        if (rank == 0) mbar_arrive_expect_tx(&bars->full[stage], 2 * kPairStageBytes);
+                        tma_load_2d_pair(st, &tm_a, full_even, static_cast<int32_t>(kb * kBK), a_row);
+                        tma_load_2d_pair(st + kPanel, &tm_b, full_even, static_cast<int32_t>(kb * kBK), b_row);
+                        issued = true;
+                        pending[stage] = static_cast<int32_t>(phase);
+                        if (++stage == kPairStages) {
+                            stage = 0;
+                            phase ^= 1;
                         }
-                        if (h == 1) tc_commit_pair(&bars->empty[stage], 0x3);
-                        tc_commit_pair(&bars->acc_full[ab], 0x3);
                     }
-                    if (++stage == kPairStages) {
-                        stage = 0;
-                        phase ^= 1;
+                }
+                if (!ok) {
+                    if (rank == 0) {
+                        volatile uint32_t never = 0;
+                        for (uint32_t s = 0; s < kPairStages; ++s)
+                            if (pending[s] >= 0)
+                                mbar_wait_bounded(&bars->full[s], static_cast<uint32_t>(pending[s]), &never,
+                                                  &g_mm8_error_word, kErrDrain, 1000000000ull);
+                    } else if (issued) {
+                        spin_ns(2000000ull);  // this CTA cannot observe its last copies, which complete on the peer
                     }
                 }
             }
-            // All issued MMAs complete before TMEM is freed (normal and error paths alike).
-            tc_commit_pair(&bars->mma_done, 0x1);
-            volatile uint32_t never = 0;
-            mbar_wait_bounded(&bars->mma_done, 0, &never, &g_mm8_error_word, kErrDrain, 1000000000ull);
-        }
-    } else if (warp >= 2 + kPairEpiWarps) {
-        // ============================= products of the scales =============================
-        // two rows per thread; the loads of the next four blocks are under way while the last are read
-        const uint32_t r = (warp - 2 - kPairEpiWarps) * 32 + lane;
-        float* ring = reinterpret_cast<float*>(smem + kPairOffScale);
-        uint32_t sg = 0;
-        bool ok = true;
-        for (uint32_t t = cluster; t < p.num_tiles && ok; t += clusters) {
-            uint32_t tm, tn;
-            pair_tile(p, t, tm, tn);
-            // rows and columns behind the end: any valid scale, nothing of them is stored
-            const uint32_t row = tm * 256 + rank * 128 + r;
-            const float* sa[2] = {p.a_scale + static_cast<uint64_t>(min(row, p.M - 1)) * p.kb,
-                                  p.a_scale + static_cast<uint64_t>(min(row + 64, p.M - 1)) * p.kb};
-            const float* sb[2] = {p.b_scale + static_cast<uint64_t>(min(tn * 2, p.nb - 1)) * p.kb,
-                                  p.b_scale + static_cast<uint64_t>(min(tn * 2 + 1, p.nb - 1)) * p.kb};
-            for (uint32_t kb = 0; kb < p.kb; kb += 4, ++sg) {
-                float va[2][4], vb[2][4];
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    const uint32_t k = min(kb + i, p.kb - 1);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        va[j][i] = __ldg(sa[j] + k);
-                        vb[j][i] = __ldg(sb[j] + k);
+        } else if (warp == 1) {
+            // ====================== MMA issuer (even CTA, for the pair) =====================
+            if (rank == 0 && lane == 0) {
+                const uint32_t idesc = make_idesc_e4m3(256, 128);
+                uint32_t stage = 0, phase = 0, g = 0;  // g counts K blocks over all tiles
+                bool ok = true;
+                for (uint32_t t = cluster; t < p.num_tiles && ok; t += clusters) {
+                    for (uint32_t kb = 0; kb < p.kb && ok; ++kb, ++g) {
+                        const Sw128Desc a0 = make_sw128_desc2(s_base + stage * kPairStageBytes, 16, 1024);
+    #pragma unroll
+                        for (uint32_t h = 0; h < 2; ++h) {
+                            const uint32_t ab = (g & 1) * 2 + h;
+                            if (!mbar_wait_bounded(&bars->acc_empty[ab], ((g >> 1) & 1) ^ 1, abort_flag,
+                                                           &g_mm8_error_word, kErrMmaAcc) ||
+                                (h == 0 && !mbar_wait_bounded(&bars->full[stage], phase, abort_flag,
+                                                                      &g_mm8_error_word, kErrMmaFull))) {
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after();
+                            Sw128Desc ad = a0, bd = a0;
+                            bd.lo += (kPanel + h * 64 * kBK) >> 4;
+    #pragma unroll
+                            for (uint32_t kk = 0; kk < kBK / 32; ++kk) {
+                                mma_f8_ss2_pair(tmem_base + ab * 128, ad, bd, idesc, kk > 0 ? 1u : 0u);
+                                ad.lo += 2;  // 32 bytes along K
+                                bd.lo += 2;
+                            }
+                            if (h == 1) tc_commit_pair(&bars->empty[stage], 0x3);
+                            tc_commit_pair(&bars->acc_full[ab], 0x3);
+                        }
+                        if (++stage == kPairStages) {
+                            stage = 0;
+                            phase ^= 1;
+                        }
                     }
                 }
-                ok = mbar_wait_bounded(&bars->sc_empty[sg & 1], ((sg >> 1) & 1) ^ 1, abort_flag, &g_mm8_error_word,
-                                       kErrScale);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                float* out = ring + (sg & 1) * 1024 + r;
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int pn = 0; pn < 2; ++pn) {
-                        out[i * 256 + pn * 128] = va[0][i] * vb[pn][i];
-                        out[i * 256 + pn * 128 + 64] = va[1][i] * vb[pn][i];
+                // All issued MMAs complete before TMEM is freed (normal and error paths alike).
+                tc_commit_pair(&bars->mma_done, 0x1);
+                volatile uint32_t never = 0;
+                mbar_wait_bounded(&bars->mma_done, 0, &never, &g_mm8_error_word, kErrDrain, 1000000000ull);
+            }
+        } else if (warp < 4) {
+            // ============================= products of the scales =============================
+            // two rows per thread; the loads of the next four blocks are under way while the last are read
+            const uint32_t r = (warp - 2) * 32 + lane;
+            float* ring = reinterpret_cast<float*>(smem + kPairOffScale);
+            uint32_t sg = 0;
+            bool ok = true;
+            for (uint32_t t = cluster; t < p.num_tiles && ok; t += clusters) {
+                uint32_t tm, tn;
+                pair_tile(p, t, tm, tn);
+                // rows and columns behind the end: any valid scale, nothing of them is stored
+                const uint32_t row = tm * 256 + rank * 128 + r;
+                const float* sa[2] = {p.a_scale + static_cast<uint64_t>(min(row, p.M - 1)) * p.kb,
+                                      p.a_scale + static_cast<uint64_t>(min(row + 64, p.M - 1)) * p.kb};
+                const float* sb[2] = {p.b_scale + static_cast<uint64_t>(min(tn * 2, p.nb - 1)) * p.kb,
+                                      p.b_scale + static_cast<uint64_t>(min(tn * 2 + 1, p.nb - 1)) * p.kb};
+                for (uint32_t kb = 0; kb < p.kb; kb += 4, ++sg) {
+                    float va[2][4], vb[2][4];
+    #pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        const uint32_t k = min(kb + i, p.kb - 1);
+    #pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            va[j][i] = __ldg(sa[j] + k);
+                            vb[j][i] = __ldg(sb[j] + k);
+                        }
                     }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars->sc_full[sg & 1]);
+                    ok = mbar_wait_bounded(&bars->sc_empty[sg & 1], ((sg >> 1) & 1) ^ 1, abort_flag, &g_mm8_error_word,
+                                           kErrScale);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    float* out = ring + (sg & 1) * 1024 + r;
+    #pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i)
+    #pragma unroll
+                        for (int pn = 0; pn < 2; ++pn) {
+                            out[i * 256 + pn * 128] = va[0][i] * vb[pn][i];
+                            out[i * 256 + pn * 128 + 64] = va[1][i] * vb[pn][i];
+                        }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars->sc_full[sg & 1]);
+                }
             }
         }
     } else {
         // ================================== promotion ==================================
-        const uint32_t quarter = warp & 3, part = (warp - 2) / 4;  // part: 64 of the 256 columns
-        const uint32_t half = part & 1, panel = part / 2;
-        const uint32_t lane_field = (quarter * 32) << 16;
+        setmaxnreg_inc<216>();
+        const uint32_t quarter = warp & 3, half = (warp - 4) / 4;
+        const uint32_t tmem_half = tmem_base + half * 128 + ((quarter * 32) << 16);
         const uint32_t empty_even = mapa_shared(smem_u32(&bars->acc_empty[half]), 0);
-        float* turn = reinterpret_cast<float*>(smem + kPairOffTurn) + (warp - 2) * 32 * 8;
-        const float* ring = reinterpret_cast<const float*>(smem + kPairOffScale) + panel * 128 + quarter * 32 + lane;
+        float* turn = reinterpret_cast<float*>(smem + kPairOffTurn) + (warp - 4) * 32 * 16;
+        const float* ring = reinterpret_cast<const float*>(smem + kPairOffScale) + quarter * 32 + lane;
         uint32_t g = 0, sg = 0;
         bool ok = true;
         for (uint32_t t = cluster; t < p.num_tiles && ok; t += clusters) {
-            uint32_t tm, tn;
-            pair_tile(p, t, tm, tn);
-            const uint32_t row0 = tm * 256 + rank * 128 + quarter * 32;
-            // accumulator columns [64 panel, + 64) of a half are columns [64 half, + 64) of CTA `panel`'s B panel
-            const uint32_t row = row0 + lane, n0 = tn * 256 + panel * 128 + half * 64;
-            float2 acc[32];
+            float2 acc[64];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) acc[i] = make_float2(0.f, 0.f);
+            for (int i = 0; i < 64; ++i) acc[i] = make_float2(0.f, 0.f);
             for (uint32_t kb = 0; kb < p.kb; ++kb, ++g) {
                 const uint32_t ab = (g & 1) * 2 + half;
                 if (kb % 4 == 0)
                     ok = mbar_wait_bounded(&bars->sc_full[sg & 1], (sg >> 1) & 1, abort_flag, &g_mm8_error_word, kErrScale);
-                const float s = ring[(sg & 1) * 1024 + (kb % 4) * 256];
+                const float s0 = ring[(sg & 1) * 1024 + (kb % 4) * 256], s1 = ring[(sg & 1) * 1024 + (kb % 4) * 256 + 128];
                 ok = ok && mbar_wait_bounded(&bars->acc_full[ab], (g >> 1) & 1, abort_flag, &g_mm8_error_word, kErrEpi);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t base = tmem_base + ab * 128 + panel * 64 + lane_field;
-                uint32_t d[16];  // 64 sums + 16: a block of 576 threads leaves a thread 96 registers
-#pragma unroll
-                for (uint32_t c = 0; c < 4; ++c) {
-                    tmem_ld16(base + c * 16, d);
-                    tmem_wait_ld16(d);
-                    if (c == 3) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_peer(empty_even + (g & 1) * 16);
-                    }
-                    scale_add16(acc + c * 8, d, s);
+                const uint32_t base = tmem_half + (g & 1) * 256;
+                uint32_t d0[32], d1[32];
+                tmem_ld32(base, d0);
+                tmem_wait_ld32(d0);
+                tmem_ld32(base + 32, d1);
+                scale_add32(acc, d0, s0);
+                tmem_wait_ld32(d1);
+                tmem_ld32(base + 64, d0);
+                scale_add32(acc + 16, d1, s0);
+                tmem_wait_ld32(d0);
+                tmem_ld32(base + 96, d1);
+                scale_add32(acc + 32, d0, s1);
+                tmem_wait_ld32(d1);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive_peer(empty_even + (g & 1) * 16);
+                    if (kb % 4 == 3 || kb + 1 == p.kb) mbar_arrive(&bars->sc_empty[sg & 1]);
                 }
-                if (kb % 4 == 3 || kb + 1 == p.kb) {
-                    if (lane == 0) mbar_arrive(&bars->sc_empty[sg & 1]);  // after the __syncwarp above
-                    ++sg;
-                }
+                if (kb % 4 == 3 || kb + 1 == p.kb) ++sg;
+                scale_add32(acc + 48, d1, s1);
             }
             if (!ok) break;
-            if (p.vec_store) {
-                if (row < p.M) store_row<T>(p, acc, row, n0);
-            } else {
-                store_turned<T>(p, acc, turn, row0, n0, lane);
+            uint32_t tm, tn;
+            pair_tile(p, t, tm, tn);
+            const uint32_t row0 = tm * 256 + rank * 128 + quarter * 32;
+#pragma unroll
+            for (uint32_t pn = 0; pn < 2; ++pn) {
+                // accumulator columns [64 pn, + 64) of a half are columns [64 half, + 64) of CTA pn's B panel
+                const uint32_t n0 = tn * 256 + pn * 128 + half * 64;
+                if (p.vec_store) {
+                    if (row0 + lane < p.M) store_row<T>(p, acc + pn * 32, row0 + lane, n0);
+                } else {
+                    store_turned<T>(p, acc + pn * 32, turn, row0, n0, lane);
+                }
             }
         }
     }
