@@ -349,24 +349,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const uint32_t empty_even = mapa_shared(smem_u32(&bars->acc_empty[half]), 0);
         float* turn = reinterpret_cast<float*>(smem + kPairOffTurn) + (warp - 4) * 32 * 16;
         const float* ring = reinterpret_cast<const float*>(smem + kPairOffScale) + quarter * 32 + lane;
+        // A wait that gave up has set the error word and the abort flag: the rest runs through, without
+        // waiting again, on whatever the accumulators hold.
         uint32_t g = 0, sg = 0;
-        bool ok = true;
-        for (uint32_t t = cluster; t < p.num_tiles && ok; t += clusters) {
+        uint32_t d0[32], d1[32];
+        float s0, s1;
+        // scales and the first 32 columns of the next block (kb of its tile)
+        auto fetch = [&](uint32_t kb) {
+            if (kb % 4 == 0)
+                mbar_wait_bounded(&bars->sc_full[sg & 1], (sg >> 1) & 1, abort_flag, &g_mm8_error_word, kErrScale);
+            s0 = ring[(sg & 1) * 1024 + (kb % 4) * 256];
+            s1 = ring[(sg & 1) * 1024 + (kb % 4) * 256 + 128];
+            mbar_wait_bounded(&bars->acc_full[(g & 1) * 2 + half], (g >> 1) & 1, abort_flag, &g_mm8_error_word, kErrEpi);
+            __syncwarp();
+            tc_fence_after();
+            tmem_ld32(tmem_half + (g & 1) * 256, d0);
+        };
+        for (uint32_t t = cluster; t < p.num_tiles; t += clusters) {
             float2 acc[64];
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = make_float2(0.f, 0.f);
-            for (uint32_t kb = 0; kb < p.kb; ++kb, ++g) {
-                const uint32_t ab = (g & 1) * 2 + half;
-                if (kb % 4 == 0)
-                    ok = mbar_wait_bounded(&bars->sc_full[sg & 1], (sg >> 1) & 1, abort_flag, &g_mm8_error_word, kErrScale);
-                const float s0 = ring[(sg & 1) * 1024 + (kb % 4) * 256], s1 = ring[(sg & 1) * 1024 + (kb % 4) * 256 + 128];
-                ok = ok && mbar_wait_bounded(&bars->acc_full[ab], (g >> 1) & 1, abort_flag, &g_mm8_error_word, kErrEpi);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tc_fence_after();
+            fetch(0);
+            for (uint32_t kb = 0; kb < p.kb; ++kb) {
                 const uint32_t base = tmem_half + (g & 1) * 256;
-                uint32_t d0[32], d1[32];
-                tmem_ld32(base, d0);
                 tmem_wait_ld32(d0);
                 tmem_ld32(base + 32, d1);
                 scale_add32(acc, d0, s0);
@@ -379,14 +384,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 tmem_wait_ld32(d1);
                 tc_fence_before();
                 __syncwarp();
+                const bool group_end = kb % 4 == 3 || kb + 1 == p.kb;
                 if (lane == 0) {
                     mbar_arrive_peer(empty_even + (g & 1) * 16);
-                    if (kb % 4 == 3 || kb + 1 == p.kb) mbar_arrive(&bars->sc_empty[sg & 1]);
+                    if (group_end) mbar_arrive(&bars->sc_empty[sg & 1]);
                 }
-                if (kb % 4 == 3 || kb + 1 == p.kb) ++sg;
-                scale_add32(acc + 48, d1, s1);
+                if (group_end) ++sg;
+                ++g;
+                const float s_last = s1;
+                if (kb + 1 < p.kb) fetch(kb + 1);  // under way while the last 32 columns are added
+                scale_add32(acc + 48, d1, s_last);
             }
-            if (!ok) break;
             uint32_t tm, tn;
             pair_tile(p, t, tm, tn);
             const uint32_t row0 = tm * 256 + rank * 128 + quarter * 32;
