@@ -65,23 +65,22 @@ constexpr uint32_t kPanel = 128 * kBK;  // 16 KB: 128 rows of either operand
 // CTA pairs: 256x256 tiles of C, cta_group::2.  CTA rank r of the pair holds rows
 // [128 r, 128 r + 128) of A and of the result and stages columns [128 r, 128 r + 128) of B.
 //   warp 0      TMA producer: A and B panel of a K block, 32 KB per stage, 6 stages
-//   warp 1      issues the MMAs of a block (even CTA, for the pair): M=256, N=128, K=32, first for the
-//               lower 64 columns of each CTA's B panel, then for the upper 64
+//   warp 1      issues the four M=256, N=256, K=32 MMAs of a block (even CTA, for the pair) into one of
+//               two TMEM accumulators of 256 columns.  Two N=128 halves with accumulators of their
+//               own would hand over sooner but read A twice: with the TMA writes 80 KB of shared
+//               memory per block instead of 64, and 128 B/cycle make that 640 cycles instead of 512
 //   warps 2-3   products of the scales for four K blocks at a time, row by row into shared memory: read
 //               by the promoting threads themselves (32 rows, 32 lines each) they cost a third of the time
-//   warps 4-11  promotion: warp w reads TMEM lanes 32 (w % 4) .. + 31 (thread = row) and the 128 columns of
-//               one half, 64 of either 128-block of N, so a thread has two scales per block: 128
-//               running sums per thread, one multiply-add each (as f32x2 pairs), the next 32 columns
-//               on their way meanwhile.  Registers: 72 / 216 per thread of the two kinds of warps
-//               (4 x 32 x 72 + 8 x 32 x 216 = 384 x 168, what the block is launched with).  Sixteen
-//               warps of 64 columns each spent more on waits than on sums: 748 us at 8192^3.
+//   warps 4-11  promotion: warp w reads TMEM lanes 32 (w % 4) .. + 31 (thread = row) and 128 columns, one
+//               128-block of N: 128 running sums per thread, one multiply-add each (as f32x2 pairs)
+//               with one product of scales per block, the next 32 columns on their way meanwhile.
+//               Registers: 72 / 216 per thread of the two kinds of warps (4 x 32 x 72 + 8 x 32 x 216
+//               = 384 x 168, what the block is launched with).  Sixteen warps of 64 columns spent more
+//               on waits than on sums.
 // "Accumulator read" goes straight to the even CTA's barrier with a release at CTA scope (no data in
 // memory hangs on it: the TMEM reads are complete and ordered by the tcgen05 fences); a release
 // at cluster scope takes about 1000 cycles here, several times the block itself.
-// TMEM holds four accumulators of 128 columns: two halves, two blocks.  A half costs the tensor
-// core 256 cycles (256 x 128 x 128 products at 2 x 8192 per cycle) and its accumulator is needed
-// again 1024 cycles after, which leaves 768 for the commit, the read (128 cycles at 512 B/cycle/SM)
-// and the arrival from both CTAs.
+// A block costs the tensor core 512 cycles (256 x 256 x 128 products at 2 x 8192 per cycle).
 // ======================================================================================
 constexpr uint32_t kPairStages = 6;
 constexpr uint32_t kPairEpiWarps = 8;
@@ -95,7 +94,7 @@ constexpr uint32_t kPairGroupM = 8;  // pair-tile rows per rasterisation group (
 
 struct PairBars {
     uint64_t full[kPairStages], empty[kPairStages];
-    uint64_t acc_full[4], acc_empty[4];  // [block & 1][half]
+    uint64_t acc_full[2], acc_empty[2];  // [block & 1]
     uint64_t sc_full[2], sc_empty[2];    // [group of four blocks & 1]
     uint64_t mma_done;
 };
@@ -118,14 +117,14 @@ __device__ __forceinline__ void scale_add32(float2* acc, const uint32_t (&d)[32]
         acc[i] = __ffma2_rn(make_float2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), s2, acc[i]);
 }
 
-// 64 sums of one row to C (vec_store): packs of 16 bytes, the last columns one by one.
+// 128 sums of one row to C (vec_store): packs of 16 bytes, the last columns one by one.
 template <typename T>
 __device__ __forceinline__ void store_row(const Params& p, const float2* acc, uint64_t row, uint32_t n0) {
     constexpr uint32_t P = elem<T>::kPack;
     const T* bias = static_cast<const T*>(p.bias);
     T* crow = static_cast<T*>(p.c) + row * p.N;
 #pragma unroll
-    for (uint32_t j = 0; j < 64; j += P) {
+    for (uint32_t j = 0; j < 128; j += P) {
         float v[P];
 #pragma unroll
         for (uint32_t e = 0; e < P; ++e) {
@@ -143,7 +142,7 @@ __device__ __forceinline__ void store_row(const Params& p, const float2* acc, ui
     }
 }
 
-// A warp's 32 rows x 64 sums to C for any row alignment: 32 x 16 tiles are turned in shared memory so
+// A warp's 32 rows x 128 sums to C for any row alignment: 32 x 16 tiles are turned in shared memory so
 // that a store instruction writes 16 neighbouring columns of two rows; row r is rotated by r / 2
 // columns, which spreads both the writes and the reads over all banks.
 template <typename T>
@@ -151,7 +150,7 @@ __device__ __forceinline__ void store_turned(const Params& p, const float2* acc,
                                              uint32_t lane) {
     const T* bias = static_cast<const T*>(p.bias);
 #pragma unroll
-    for (uint32_t c = 0; c < 4; ++c) {
+    for (uint32_t c = 0; c < 8; ++c) {
 #pragma unroll
         for (uint32_t j = 0; j < 16; ++j)
             tile[lane * 16 + (j + lane / 2) % 16] = (j & 1) ? acc[c * 8 + j / 2].y : acc[c * 8 + j / 2].x;
@@ -185,11 +184,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             mbar_init(&bars->full[s], 1);
             mbar_init(&bars->empty[s], 1);
         }
-        for (int b = 0; b < 4; ++b) {
-            mbar_init(&bars->acc_full[b], 1);
-            mbar_init(&bars->acc_empty[b], kPairEpiWarps);  // those of one half in either CTA
-        }
         for (int b = 0; b < 2; ++b) {
+            mbar_init(&bars->acc_full[b], 1);
+            mbar_init(&bars->acc_empty[b], 2 * kPairEpiWarps);  // both CTAs
             mbar_init(&bars->sc_full[b], 2);
             mbar_init(&bars->sc_empty[b], kPairEpiWarps);
         }
@@ -257,35 +254,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             }
         } else if (warp == 1) {
             // ====================== MMA issuer (even CTA, for the pair) =====================
-            if (rank == 0 && lane == 0) {
-                const uint32_t idesc = make_idesc_e4m3(256, 128);
+            // The warp stays converged and an elected lane issues: the time between two MMAs is tensor
+            // time lost.
+            if (rank == 0) {
+                const uint32_t leader = elect_one() ? 1u : 0u;
+                const uint32_t idesc = make_idesc_e4m3(256, 256);
+                const Sw128Desc desc0 = make_sw128_desc2(s_base, 16, 1024);
                 uint32_t stage = 0, phase = 0, g = 0;  // g counts K blocks over all tiles
                 bool ok = true;
                 for (uint32_t t = cluster; t < p.num_tiles && ok; t += clusters) {
-                    for (uint32_t kb = 0; kb < p.kb && ok; ++kb, ++g) {
-                        const Sw128Desc a0 = make_sw128_desc2(s_base + stage * kPairStageBytes, 16, 1024);
-    #pragma unroll
-                        for (uint32_t h = 0; h < 2; ++h) {
-                            const uint32_t ab = (g & 1) * 2 + h;
-                            if (!mbar_wait_bounded(&bars->acc_empty[ab], ((g >> 1) & 1) ^ 1, abort_flag,
-                                                           &g_mm8_error_word, kErrMmaAcc) ||
-                                (h == 0 && !mbar_wait_bounded(&bars->full[stage], phase, abort_flag,
-                                                                      &g_mm8_error_word, kErrMmaFull))) {
-                                ok = false;
-                                break;
-                            }
-                            tc_fence_after();
-                            Sw128Desc ad = a0, bd = a0;
-                            bd.lo += (kPanel + h * 64 * kBK) >> 4;
-    #pragma unroll
-                            for (uint32_t kk = 0; kk < kBK / 32; ++kk) {
-                                mma_f8_ss2_pair(tmem_base + ab * 128, ad, bd, idesc, kk > 0 ? 1u : 0u);
-                                ad.lo += 2;  // 32 bytes along K
-                                bd.lo += 2;
-                            }
-                            if (h == 1) tc_commit_pair(&bars->empty[stage], 0x3);
-                            tc_commit_pair(&bars->acc_full[ab], 0x3);
+                    for (uint32_t kb = 0; kb < p.kb; ++kb, ++g) {
+                        ok = mbar_wait_bounded(&bars->full[stage], phase, abort_flag, &g_mm8_error_word, kErrMmaFull) &&
+                             mbar_wait_bounded(&bars->acc_empty[g & 1], ((g >> 1) & 1) ^ 1, abort_flag,
+                                               &g_mm8_error_word, kErrMmaAcc);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        tc_fence_after();
+                        Sw128Desc ad = desc0, bd = desc0;
+                        ad.lo += stage * (kPairStageBytes >> 4);
+                        bd.lo = ad.lo + (kPanel >> 4);
+#pragma unroll
+                        for (uint32_t kk = 0; kk < kBK / 32; ++kk) {
+                            mma_f8_ss2_pair_if(leader, tmem_base + (g & 1) * 256, ad, bd, idesc, kk > 0 ? 1u : 0u);
+                            ad.lo += 2;  // 32 bytes along K
+                            bd.lo += 2;
                         }
+                        tc_commit_pair_if(leader, &bars->acc_full[g & 1], 0x3);
+                        tc_commit_pair_if(leader, &bars->empty[stage], 0x3);
                         if (++stage == kPairStages) {
                             stage = 0;
                             phase ^= 1;
@@ -293,7 +288,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     }
                 }
                 // All issued MMAs complete before TMEM is freed (normal and error paths alike).
-                tc_commit_pair(&bars->mma_done, 0x1);
+                tc_commit_pair_if(leader, &bars->mma_done, 0x1);
                 volatile uint32_t never = 0;
                 mbar_wait_bounded(&bars->mma_done, 0, &never, &g_mm8_error_word, kErrDrain, 1000000000ull);
             }
@@ -344,26 +339,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     } else {
         // ================================== promotion ==================================
         setmaxnreg_inc<216>();
-        const uint32_t quarter = warp & 3, half = (warp - 4) / 4;
-        const uint32_t tmem_half = tmem_base + half * 128 + ((quarter * 32) << 16);
-        const uint32_t empty_even = mapa_shared(smem_u32(&bars->acc_empty[half]), 0);
+        const uint32_t quarter = warp & 3, panel = (warp - 4) / 4;
+        const uint32_t tmem_cols = tmem_base + panel * 128 + ((quarter * 32) << 16);
+        const uint32_t empty_even = mapa_shared(smem_u32(&bars->acc_empty[0]), 0);
         float* turn = reinterpret_cast<float*>(smem + kPairOffTurn) + (warp - 4) * 32 * 16;
-        const float* ring = reinterpret_cast<const float*>(smem + kPairOffScale) + quarter * 32 + lane;
+        const float* ring = reinterpret_cast<const float*>(smem + kPairOffScale) + panel * 128 + quarter * 32 + lane;
         // A wait that gave up has set the error word and the abort flag: the rest runs through, without
         // waiting again, on whatever the accumulators hold.
         uint32_t g = 0, sg = 0;
         uint32_t d0[32], d1[32];
-        float s0, s1;
-        // scales and the first 32 columns of the next block (kb of its tile)
+        float s;
+        // scale and the first 32 columns of the next block (kb of its tile)
         auto fetch = [&](uint32_t kb) {
             if (kb % 4 == 0)
                 mbar_wait_bounded(&bars->sc_full[sg & 1], (sg >> 1) & 1, abort_flag, &g_mm8_error_word, kErrScale);
-            s0 = ring[(sg & 1) * 1024 + (kb % 4) * 256];
-            s1 = ring[(sg & 1) * 1024 + (kb % 4) * 256 + 128];
-            mbar_wait_bounded(&bars->acc_full[(g & 1) * 2 + half], (g >> 1) & 1, abort_flag, &g_mm8_error_word, kErrEpi);
+            s = ring[(sg & 1) * 1024 + (kb % 4) * 256];
+            mbar_wait_bounded(&bars->acc_full[g & 1], (g >> 1) & 1, abort_flag, &g_mm8_error_word, kErrEpi);
             __syncwarp();
             tc_fence_after();
-            tmem_ld32(tmem_half + (g & 1) * 256, d0);
+            tmem_ld32(tmem_cols + (g & 1) * 256, d0);
         };
         for (uint32_t t = cluster; t < p.num_tiles; t += clusters) {
             float2 acc[64];
@@ -371,42 +365,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             for (int i = 0; i < 64; ++i) acc[i] = make_float2(0.f, 0.f);
             fetch(0);
             for (uint32_t kb = 0; kb < p.kb; ++kb) {
-                const uint32_t base = tmem_half + (g & 1) * 256;
+                const uint32_t base = tmem_cols + (g & 1) * 256;
                 tmem_wait_ld32(d0);
                 tmem_ld32(base + 32, d1);
-                scale_add32(acc, d0, s0);
+                scale_add32(acc, d0, s);
                 tmem_wait_ld32(d1);
                 tmem_ld32(base + 64, d0);
-                scale_add32(acc + 16, d1, s0);
+                scale_add32(acc + 16, d1, s);
                 tmem_wait_ld32(d0);
                 tmem_ld32(base + 96, d1);
-                scale_add32(acc + 32, d0, s1);
+                scale_add32(acc + 32, d0, s);
                 tmem_wait_ld32(d1);
                 tc_fence_before();
                 __syncwarp();
                 const bool group_end = kb % 4 == 3 || kb + 1 == p.kb;
                 if (lane == 0) {
-                    mbar_arrive_peer(empty_even + (g & 1) * 16);
+                    mbar_arrive_peer(empty_even + (g & 1) * 8);
                     if (group_end) mbar_arrive(&bars->sc_empty[sg & 1]);
                 }
                 if (group_end) ++sg;
                 ++g;
-                const float s_last = s1;
+                const float s_last = s;
                 if (kb + 1 < p.kb) fetch(kb + 1);  // under way while the last 32 columns are added
                 scale_add32(acc + 48, d1, s_last);
             }
             uint32_t tm, tn;
             pair_tile(p, t, tm, tn);
-            const uint32_t row0 = tm * 256 + rank * 128 + quarter * 32;
-#pragma unroll
-            for (uint32_t pn = 0; pn < 2; ++pn) {
-                // accumulator columns [64 pn, + 64) of a half are columns [64 half, + 64) of CTA pn's B panel
-                const uint32_t n0 = tn * 256 + pn * 128 + half * 64;
-                if (p.vec_store) {
-                    if (row0 + lane < p.M) store_row<T>(p, acc + pn * 32, row0 + lane, n0);
-                } else {
-                    store_turned<T>(p, acc + pn * 32, turn, row0, n0, lane);
-                }
+            const uint32_t row0 = tm * 256 + rank * 128 + quarter * 32, n0 = tn * 256 + panel * 128;
+            if (p.vec_store) {
+                if (row0 + lane < p.M) store_row<T>(p, acc, row0 + lane, n0);
+            } else {
+                store_turned<T>(p, acc, turn, row0, n0, lane);
             }
         }
     }

@@ -453,14 +453,16 @@ __device__ __forceinline__ void mma_f8_ss2(uint32_t d_tmem, Sw128Desc a, Sw128De
         "r"(a.lo), "r"(a.hi), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void mma_f8_ss2_pair(uint32_t d_tmem, Sw128Desc a, Sw128Desc b, uint32_t idesc,
-                                                uint32_t accumulate) {
+// For an MMA warp that runs converged (see mma_ss2_if below).
+__device__ __forceinline__ void mma_f8_ss2_pair_if(uint32_t leader, uint32_t d_tmem, Sw128Desc a, Sw128Desc b,
+                                                   uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+        "setp.ne.b32 q, %7, 0;\n\t"
         "mov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"
         "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %5, p;\n\t}" ::"r"(d_tmem),
-        "r"(a.lo), "r"(a.hi), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"(accumulate)
+        "@q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %5, p;\n\t}" ::"r"(d_tmem),
+        "r"(a.lo), "r"(a.hi), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"(accumulate), "r"(leader)
         : "memory");
 }
 
@@ -507,6 +509,16 @@ __device__ __forceinline__ void tc_commit_if(uint32_t leader, uint64_t* bar) {
         "setp.ne.b32 q, %1, 0;\n\t"
         "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
         "r"(leader)
+        : "memory");
+}
+
+__device__ __forceinline__ void tc_commit_pair_if(uint32_t leader, uint64_t* bar, uint16_t cta_mask) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %2, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(
+            smem_u32(bar)),
+        "h"(cta_mask), "r"(leader)
         : "memory");
 }
 
