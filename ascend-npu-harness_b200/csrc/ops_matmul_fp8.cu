@@ -417,17 +417,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 // chosen to give every SM a part of it, and the ring holds all that fits beside a second CTA.
 //   warp 0      TMA producer: 16 KB of weight and TN x 128 bytes of tokens per K block
 //   warp 1      issues M=128, N=TN, K=32 MMAs into one of kAcc accumulators of TN columns
-//   warps 2-5   thread = weight row: acc[t] += d[t] * (token scale * weight scale), the products of
-//               the scales staged in shared memory a block ahead
+//   warps 2 on  promotion, kEpi = 4 or 8 warps: thread = weight row (TMEM lane), kCols of the tokens:
+//               acc[t] += d[t] * (token scale * weight scale), the products of the scales staged in
+//               shared memory a block ahead
 // ======================================================================================
-constexpr uint32_t kFewThreads = 192;
-
 template <uint32_t TN>
 struct Few {
+    static constexpr uint32_t kEpi = TN <= 32 ? 4 : 8;       // promoting warps
+    static constexpr uint32_t kCols = TN / (kEpi / 4);       // tokens of a promoting warp
+    static constexpr uint32_t kThreads = 64 + 32 * kEpi;
     static constexpr uint32_t kAcc = TN <= 64 ? 4 : 2;
+    static constexpr uint32_t kTmem = kAcc * TN <= 64 ? 64 : kAcc * TN <= 128 ? 128 : 256;
+    static constexpr uint32_t kPerSm = TN <= 64 ? 2 : 1;     // CTAs that share an SM
     static constexpr uint32_t kTokBytes = TN * kBK;
     static constexpr uint32_t kStageBytes = kPanel + kTokBytes;
-    static constexpr uint32_t kStages = 100 * 1024 / kStageBytes;  // two CTAs per SM
+    static constexpr uint32_t kStages = (kPerSm == 2 ? 100 : 210) * 1024 / kStageBytes;
     static constexpr uint32_t kOffScale = kStages * kStageBytes;   // [2][TN] products of scales
     static constexpr uint32_t kOffBar = kOffScale + 2 * TN * 4;
     static constexpr uint32_t kSmem = kOffBar + 512 + 1024;
@@ -442,7 +446,7 @@ struct FewBars {
 };
 
 template <typename T, uint32_t TN>
-__global__ void __launch_bounds__(kFewThreads)
+__global__ void __launch_bounds__(Few<TN>::kThreads, Few<TN>::kPerSm)
     mm8_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const Params p,
                    const uint32_t splits) {
     using F = Few<TN>;
@@ -465,14 +469,14 @@ __global__ void __launch_bounds__(kFewThreads)
         }
         for (uint32_t b = 0; b < F::kAcc; ++b) {
             mbar_init(&bars->acc_full[b], 1);
-            mbar_init(&bars->acc_empty[b], 4);
+            mbar_init(&bars->acc_empty[b], F::kEpi);
         }
         mbar_init(&bars->mma_done, 1);
         *abort_flag = 0;
         fence_mbar_init();
     }
     if (warp == 1) {
-        tmem_alloc(tmem_slot, F::kAcc * TN);
+        tmem_alloc(tmem_slot, F::kTmem);
         tmem_relinquish();
     }
     if (warp == 0 && lane == 0) {
@@ -485,7 +489,7 @@ __global__ void __launch_bounds__(kFewThreads)
     const uint32_t tmem_base = *tmem_slot;
     const uint32_t s_base = smem_u32(smem);
 
-    float2 acc[TN / 2];
+    float2 acc[F::kCols / 2];
     bool ok = true;
     if (warp == 0) {
         if (lane == 0) {
@@ -547,15 +551,15 @@ __global__ void __launch_bounds__(kFewThreads)
             mbar_wait_bounded(&bars->mma_done, 0, &never, &g_mm8_error_word, kErrDrain, 1000000000ull);
         }
     } else {
-        const uint32_t quarter = warp & 3;
-        const uint32_t lane_field = (quarter * 32) << 16;
-        const uint32_t tid = threadIdx.x - 64;  // 0..127
+        const uint32_t tid = threadIdx.x - 64;
+        const uint32_t col0 = (warp - 2) / 4 * F::kCols;
+        const uint32_t tmem_cols = tmem_base + col0 + (((warp & 3) * 32) << 16);
         float* prod = reinterpret_cast<float*>(smem + F::kOffScale);
         const float* sa = p.a_scale + static_cast<uint64_t>(min(m0 + tid, p.M - 1)) * p.kb;
         const float* sb = p.b_scale + static_cast<uint64_t>(blockIdx.y) * p.kb;
 #pragma unroll
-        for (uint32_t i = 0; i < TN / 2; ++i) acc[i] = make_float2(0.f, 0.f);
-        float next = tid < TN && kb0 < kb1 ? __ldg(sa + kb0) * __ldg(sb + kb0) : 0.f;
+        for (uint32_t i = 0; i < F::kCols / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+        float next = tid < TN ? __ldg(sa + kb0) * __ldg(sb + kb0) : 0.f;
         uint32_t g = 0;
         for (uint32_t kb = kb0; kb < kb1; ++kb, ++g) {
             const uint32_t ab = g % F::kAcc;
@@ -565,75 +569,100 @@ __global__ void __launch_bounds__(kFewThreads)
                 const uint32_t k2 = min(kb + 1, kb1 - 1);
                 next = __ldg(sa + k2) * __ldg(sb + k2);
             }
-            // the four warps alone; two buffers: a warp two blocks behind cannot be, it has to pass here
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&bars->acc_full[ab], (g / F::kAcc) & 1, abort_flag,
-                                                           &g_mm8_error_word, kErrEpi)))
-                ok = false;
-            if (ok) {
-                tc_fence_after();
+            // the promoting warps alone; two buffers of products are enough, since a warp that still reads
+            // the one before last has not been here
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * F::kEpi) : "memory");
+            // after a wait that gave up (the error word is set) the rest runs through without waiting
+            mbar_wait_bounded(&bars->acc_full[ab], (g / F::kAcc) & 1, abort_flag, &g_mm8_error_word, kErrEpi);
+            __syncwarp();
+            tc_fence_after();
 #pragma unroll
-                for (uint32_t c = 0; c < TN; c += 16) {
-                    uint32_t d[16];
-                    tmem_ld16(tmem_base + ab * TN + c + lane_field, d);
-                    tmem_wait_ld16(d);
+            for (uint32_t c = 0; c < F::kCols; c += 16) {
+                uint32_t d[16];
+                tmem_ld16(tmem_cols + ab * TN + c, d);
+                tmem_wait_ld16(d);
 #pragma unroll
-                    for (uint32_t i = 0; i < 8; ++i)
-                        acc[c / 2 + i] =
-                            __ffma2_rn(make_float2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])),
-                                       *reinterpret_cast<const float2*>(sp + c + 2 * i), acc[c / 2 + i]);
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const float4 f = *reinterpret_cast<const float4*>(sp + col0 + c + 4 * i);
+                    float2& a0 = acc[c / 2 + 2 * i];
+                    float2& a1 = acc[c / 2 + 2 * i + 1];
+                    a0 = __ffma2_rn(make_float2(__uint_as_float(d[4 * i]), __uint_as_float(d[4 * i + 1])),
+                                    make_float2(f.x, f.y), a0);
+                    a1 = __ffma2_rn(make_float2(__uint_as_float(d[4 * i + 2]), __uint_as_float(d[4 * i + 3])),
+                                    make_float2(f.z, f.w), a1);
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars->acc_empty[ab]);
             }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->acc_empty[ab]);
         }
     }
 
-    // Every MMA and copy of this CTA is done once its promotion warps are through the last block (or
+    // Every MMA and copy of this CTA is done once its promoting warps are through the last block (or
     // the roles above have drained them), so the ring can hold the sums.
     __syncwarp();
     __syncthreads();
-    const uint32_t tid = threadIdx.x - 64;
-    const uint32_t row = (warp & 3) * 32 + lane;  // weight row of this thread's sums
-    float* part = reinterpret_cast<float*>(smem);  // [TN][128]
+    const uint32_t row = (warp & 3) * 32 + lane;                            // weight row of this thread's sums
+    const uint32_t t0 = warp >= 2 ? (warp - 2) / 4 * F::kCols : 0;          // and their first token
+    const T* bias = static_cast<const T*>(p.bias);
     if (splits > 1) {
+        float* part = reinterpret_cast<float*>(smem);  // [TN][128]
         if (warp >= 2) {
 #pragma unroll
-            for (uint32_t i = 0; i < TN / 2; ++i) {
-                part[(2 * i) * 128 + row] = acc[i].x;
-                part[(2 * i + 1) * 128 + row] = acc[i].y;
+            for (uint32_t i = 0; i < F::kCols / 2; ++i) {
+                part[(t0 + 2 * i) * 128 + row] = acc[i].x;
+                part[(t0 + 2 * i + 1) * 128 + row] = acc[i].y;
             }
         }
         cluster_sync_all();
-        // rank r joins and stores tokens r, r + splits, ...
+        // rank r joins and stores tokens r, r + splits, ...: a warp takes one token, a lane four rows
         if (warp >= 2) {
-            const uint32_t n = n0 + tid;
-            const T* bias = static_cast<const T*>(p.bias);
-            const float b = bias && n < p.N ? elem<T>::to_f(bias[n]) : 0.f;
-            for (uint32_t t = rank; t < TN && m0 + t < p.M; t += splits) {
-                float v = 0.f;
-                for (uint32_t r = 0; r < splits; ++r)
-                    v += ld_cluster_f32(mapa_shared(smem_u32(part + t * 128 + tid), r));
-                if (bias) v += b;
-                if (n < p.N) static_cast<T*>(p.c)[static_cast<uint64_t>(m0 + t) * p.N + n] = elem<T>::from_f(v);
+            const uint32_t n = n0 + lane * 4;
+            float b[4];
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) b[e] = bias && n + e < p.N ? elem<T>::to_f(bias[n + e]) : 0.f;
+            for (uint32_t t = rank + splits * (warp - 2); t < TN && m0 + t < p.M; t += splits * F::kEpi) {
+                const uint32_t at = smem_u32(part + t * 128 + lane * 4);
+                float4 v[8];
+#pragma unroll
+                for (uint32_t r = 0; r < 8; ++r)
+                    if (r < splits) v[r] = ld_cluster_f32x4(mapa_shared(at, r));
+                float o[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+                for (uint32_t r = 1; r < 8; ++r)
+                    if (r < splits) {
+                        o[0] += v[r].x; o[1] += v[r].y; o[2] += v[r].z; o[3] += v[r].w;
+                    }
+                T* c = static_cast<T*>(p.c) + static_cast<uint64_t>(m0 + t) * p.N + n;
+                alignas(16) T h[4];
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) h[e] = elem<T>::from_f(bias ? o[e] + b[e] : o[e]);
+                if (p.vec_store && n < p.N) {  // N is a multiple of 4 then
+                    if constexpr (sizeof(T) == 4)
+                        *reinterpret_cast<uint4*>(c) = *reinterpret_cast<const uint4*>(h);
+                    else
+                        *reinterpret_cast<uint2*>(c) = *reinterpret_cast<const uint2*>(h);
+                } else {
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e)
+                        if (n + e < p.N) c[e] = h[e];
+                }
             }
         }
         cluster_sync_all();  // no CTA leaves while its sums may still be read
     } else if (warp >= 2) {
         const uint32_t n = n0 + row;
-        const T* bias = static_cast<const T*>(p.bias);
         const float b = bias && n < p.N ? elem<T>::to_f(bias[n]) : 0.f;
 #pragma unroll
-        for (uint32_t t = 0; t < TN; ++t) {
-            float v = (t & 1) ? acc[t / 2].y : acc[t / 2].x;
-            if (bias) v += b;
-            if (n < p.N && m0 + t < p.M) static_cast<T*>(p.c)[static_cast<uint64_t>(m0 + t) * p.N + n] = elem<T>::from_f(v);
+        for (uint32_t t = 0; t < F::kCols; ++t) {
+            const float v = (t & 1) ? acc[t / 2].y : acc[t / 2].x;
+            if (n < p.N && m0 + t0 + t < p.M)
+                static_cast<T*>(p.c)[static_cast<uint64_t>(m0 + t0 + t) * p.N + n] = elem<T>::from_f(bias ? v + b : v);
         }
     }
     if (warp == 1) {
         __syncwarp();
-        tmem_dealloc(tmem_base, F::kAcc * TN);
+        tmem_dealloc(tmem_base, F::kTmem);
     }
 }
 
@@ -765,14 +794,22 @@ int launch_few(const Params& p, cudaStream_t s) {
     auto* k = mm8_few_kernel<T, TN>;
     if (int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(k), Few<TN>::kSmem, "mm8_few_kernel")) return rc;
     const uint32_t token_tiles = (p.M + TN - 1) / TN;
-    // Splits of K: double while the grid leaves half of the two CTAs per SM free and each split keeps
-    // two blocks.
-    const uint64_t tiles = static_cast<uint64_t>(p.nb) * token_tiles;
+    // Splits of K: the least work of the busiest SM, in K blocks and a join that costs about as much as two;
+    // at most as many CTAs as are resident at once, unless even one split is more.
+    const uint64_t tiles = static_cast<uint64_t>(p.nb) * token_tiles, sms = sm_count();
     uint32_t splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= 2ull * sm_count() && p.kb >= 4 * splits) splits *= 2;
+    uint64_t best = ~0ull;
+    for (uint32_t c = 1; c <= 8 && c <= p.kb; ++c) {
+        if (c > 1 && tiles * c > sms * Few<TN>::kPerSm) break;
+        const uint64_t cost = (tiles * c + sms - 1) / sms * ((p.kb + c - 1) / c) + (c > 1 ? 2 : 0);
+        if (cost < best) {
+            best = cost;
+            splits = c;
+        }
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(splits, p.nb, token_tiles);
-    cfg.blockDim = dim3(kFewThreads);
+    cfg.blockDim = dim3(Few<TN>::kThreads);
     cfg.dynamicSmemBytes = Few<TN>::kSmem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
@@ -808,6 +845,7 @@ int launch(Params p, cudaStream_t s) {
     if (p.M <= 16) return launch_few<T, 16>(p, s);
     if (p.M <= 32) return launch_few<T, 32>(p, s);
     if (p.M <= 64) return launch_few<T, 64>(p, s);
+    if (p.M <= 96) return launch_few<T, 96>(p, s);
     return launch_few<T, 128>(p, s);
 }
 

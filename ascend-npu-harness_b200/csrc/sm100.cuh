@@ -536,10 +536,13 @@ __host__ __device__ constexpr uint32_t make_idesc_e4m3(uint32_t M, uint32_t N) {
     return (1u << 4) | ((N >> 3) << 17) | ((M >> 4) << 24);
 }
 
-// fp32 read of another CTA's shared memory, by its shared::cluster address.
-__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+// 16-byte read of another CTA's shared memory, by its shared::cluster address (volatile, so that it stays
+// behind the cluster barrier that makes the data visible).
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t cluster_addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(cluster_addr));
     return v;
 }
 
