@@ -96,6 +96,160 @@ __global__ void __launch_bounds__(kThreads) block_bwd_kernel(const T* __restrict
 }
 
 // ---------------------------------------------------------------------------------------
+// Rows of whole 16-byte packs: G = 16 lanes (32 for fp32) own a block, one pack each, so the block's
+// maximum is a shuffle tree over the group; a group has kUnroll blocks in flight.  One CTA per
+// kUnroll * groups blocks: nothing is kept from block to block.
+// ---------------------------------------------------------------------------------------
+constexpr int kUnroll = 4;
+
+template <typename T>
+struct Vec {
+    static constexpr uint32_t P = elem<T>::kPack;
+    static constexpr uint32_t G = kFp8Block / P;
+    static constexpr uint32_t kGroups = kThreads / G;
+    static constexpr uint32_t kPerCta = kGroups * kUnroll;  // blocks
+};
+
+// Where block b starts, and how many of its columns there are.
+struct BlockMap {
+    FastDiv row_blocks;
+    uint32_t cols;
+    bool whole;  // rows are whole blocks: block b starts at 128 b
+    __device__ __forceinline__ uint64_t start(uint32_t b, uint32_t& n) const {
+        if (whole) {
+            n = kFp8Block;
+            return static_cast<uint64_t>(b) * kFp8Block;
+        }
+        const uint32_t row = row_blocks.div(b), c0 = (b - row * row_blocks.d) * kFp8Block;
+        n = min(kFp8Block, cols - c0);
+        return static_cast<uint64_t>(row) * cols + c0;
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ void unpack(const pack<T>& p, float* f) {
+#pragma unroll
+    for (int e = 0; e < elem<T>::kPack; ++e) f[e] = elem<T>::to_f(p.v[e]);
+}
+
+// A pack's codes, as one store.
+__device__ __forceinline__ void store_codes(uint8_t* q, const float (&v)[8]) {
+    const uint32_t lo = fp8_encode2(v[0], v[1]) | fp8_encode2(v[2], v[3]) << 16;
+    const uint32_t hi = fp8_encode2(v[4], v[5]) | fp8_encode2(v[6], v[7]) << 16;
+    __stcs(reinterpret_cast<uint2*>(q), make_uint2(lo, hi));
+}
+__device__ __forceinline__ void store_codes(uint8_t* q, const float (&v)[4]) {
+    __stcs(reinterpret_cast<uint32_t*>(q), fp8_encode2(v[0], v[1]) | fp8_encode2(v[2], v[3]) << 16);
+}
+
+template <typename Op, int N>
+__device__ __forceinline__ void apply_act(const Op& op, const float (&v)[N], float (&y)[N]) {
+    if constexpr (std::is_same<Op, FastActOp>::value) {
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+            const float2 r = op.apply2(make_float2(v[e], v[e + 1]));
+            y[e] = r.x;
+            y[e + 1] = r.y;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) y[e] = op.apply(v[e], 0.f);
+    }
+}
+
+template <typename T, bool HasAct>
+__global__ void __launch_bounds__(kThreads) block_fwd_vec_kernel(const T* __restrict__ x, T* __restrict__ y,
+                                                                 uint8_t* __restrict__ q, float* __restrict__ scale,
+                                                                 uint32_t blocks, const BlockMap map,
+                                                                 typename ActOf<T>::Op op) {
+    using V = Vec<T>;
+    const uint32_t gl = threadIdx.x % V::G, c = gl * V::P;
+    const uint32_t b0 = blockIdx.x * V::kPerCta + threadIdx.x / V::G;
+    pack<T> in[kUnroll];
+    uint64_t at[kUnroll];
+    bool have[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        const uint32_t b = b0 + u * V::kGroups;
+        uint32_t n = 0;
+        at[u] = b < blocks ? map.start(b, n) + c : 0;
+        have[u] = c < n;  // rows are whole packs, so a pack is in or out
+        if (have[u]) in[u] = ld_stream(reinterpret_cast<const pack<T>*>(x + at[u]));
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        const uint32_t b = b0 + u * V::kGroups;
+        float v[V::P];
+        uint32_t m = 0;
+        if (have[u]) {
+            unpack<T>(in[u], v);
+#pragma unroll
+            for (uint32_t e = 0; e < V::P; ++e) m = max(m, abs_bits(v[e]));
+        }
+#pragma unroll
+        for (uint32_t o = V::G / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        float inv, s;
+        fp8_block_scale(m, inv, s);
+        if (!have[u]) continue;
+        if (gl == 0) scale[b] = s;
+        float w[V::P];
+#pragma unroll
+        for (uint32_t e = 0; e < V::P; ++e) w[e] = __fmul_rn(v[e], inv);
+        store_codes(q + at[u], w);
+        if (HasAct) {
+            apply_act(op, v, w);
+            st_stream(reinterpret_cast<pack<T>*>(y + at[u]), pack_from_f<T>(w));
+        }
+    }
+}
+
+template <typename T, bool HasAct>
+__global__ void __launch_bounds__(kThreads) block_bwd_vec_kernel(const T* __restrict__ dy, const uint8_t* __restrict__ q,
+                                                                 const float* __restrict__ scale, T* __restrict__ out,
+                                                                 uint32_t blocks, const BlockMap map,
+                                                                 ActSlope<sizeof(T) == 4> slope) {
+    using V = Vec<T>;
+    const uint32_t c = threadIdx.x % V::G * V::P;
+    const uint32_t b0 = blockIdx.x * V::kPerCta + threadIdx.x / V::G;
+    pack<T> in[kUnroll];
+    uint2 codes[kUnroll];
+    float s[kUnroll];
+    uint64_t at[kUnroll];
+    bool have[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        const uint32_t b = b0 + u * V::kGroups;
+        uint32_t n = 0;
+        at[u] = b < blocks ? map.start(b, n) + c : 0;
+        have[u] = c < n;
+        if (!have[u]) continue;
+        if (HasAct) in[u] = ld_stream(reinterpret_cast<const pack<T>*>(dy + at[u]));
+        if (V::P == 8)
+            codes[u] = __ldcs(reinterpret_cast<const uint2*>(q + at[u]));
+        else
+            codes[u].x = __ldcs(reinterpret_cast<const uint32_t*>(q + at[u]));
+        s[u] = __ldg(scale + b);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        if (!have[u]) continue;
+        float v[V::P], g[V::P];
+#pragma unroll
+        for (uint32_t e = 0; e < V::P; e += 2) {
+            const float2 f = fp8_decode2((e < 4 ? codes[u].x : codes[u].y) >> (e % 4 * 8));
+            v[e] = __fmul_rn(f.x, s[u]);
+            v[e + 1] = __fmul_rn(f.y, s[u]);
+        }
+        if (HasAct) {
+            unpack<T>(in[u], g);
+#pragma unroll
+            for (uint32_t e = 0; e < V::P; ++e) v[e] = __fmul_rn(g[e], slope(v[e]));
+        }
+        st_stream(reinterpret_cast<pack<T>*>(out + at[u]), pack_from_f<T>(v));
+    }
+}
+
+// ---------------------------------------------------------------------------------------
 // 128 x 128 tiles (weights: laid out once, so plain): one CTA per tile, two passes, the second
 // from cache.
 // ---------------------------------------------------------------------------------------
@@ -156,12 +310,35 @@ unsigned grid_of(K kernel, uint64_t items, uint64_t per_block) {
     return static_cast<unsigned>(blocks < cap ? blocks : (cap ? cap : 1));
 }
 
+// Whether the pack kernels take these buffers: rows of whole packs, 16-byte aligned (codes: a pack's), and
+// a block count that 32 bits hold with a CTA's worth to spare.
+template <typename T>
+bool vec_ok(const void* a, const void* b, const void* q, uint32_t rows, uint32_t cols, uint32_t nb) {
+    return cols % Vec<T>::P == 0 && aligned16(a) && aligned16(b) && reinterpret_cast<uintptr_t>(q) % Vec<T>::P == 0 &&
+           static_cast<uint64_t>(rows) * nb <= 0xFFFFFFFFull - Vec<T>::kPerCta;
+}
+
+BlockMap block_map(uint32_t cols, uint32_t nb) {
+    BlockMap m;
+    m.row_blocks.init(nb);
+    m.cols = cols;
+    m.whole = cols % kFp8Block == 0;
+    return m;
+}
+
 template <typename T, bool HasAct>
 int launch_fwd(const void* x, void* y, void* q, float* scale, uint32_t rows, uint32_t cols, uint32_t act,
                cudaStream_t s, const char* name) {
     const uint32_t nb = (cols + kFp8Block - 1) / kFp8Block;
     const auto op = ActOf<T>::make(act);
     const uint64_t blocks = static_cast<uint64_t>(rows) * nb;
+    if (vec_ok<T>(x, HasAct ? y : x, q, rows, cols, nb)) {
+        const unsigned grid = static_cast<unsigned>((blocks + Vec<T>::kPerCta - 1) / Vec<T>::kPerCta);
+        block_fwd_vec_kernel<T, HasAct><<<grid, kThreads, 0, s>>>(static_cast<const T*>(x), static_cast<T*>(y),
+                                                                  static_cast<uint8_t*>(q), scale,
+                                                                  static_cast<uint32_t>(blocks), block_map(cols, nb), op);
+        return check_launch(name);
+    }
     auto* k = block_fwd_kernel<T, HasAct>;
     k<<<grid_of(k, blocks, kThreads / 32), kThreads, 0, s>>>(static_cast<const T*>(x), static_cast<T*>(y),
                                                              static_cast<uint8_t*>(q), scale, rows, cols, nb, op);
@@ -174,6 +351,13 @@ int launch_bwd(const void* dy, const void* q, const float* scale, void* out, uin
     const uint32_t nb = (cols + kFp8Block - 1) / kFp8Block;
     const auto slope = ActSlope<sizeof(T) == 4>::make(act);
     const uint64_t blocks = static_cast<uint64_t>(rows) * nb;
+    if (vec_ok<T>(out, HasAct ? dy : out, q, rows, cols, nb)) {
+        const unsigned grid = static_cast<unsigned>((blocks + Vec<T>::kPerCta - 1) / Vec<T>::kPerCta);
+        block_bwd_vec_kernel<T, HasAct><<<grid, kThreads, 0, s>>>(static_cast<const T*>(dy), static_cast<const uint8_t*>(q),
+                                                                  scale, static_cast<T*>(out),
+                                                                  static_cast<uint32_t>(blocks), block_map(cols, nb), slope);
+        return check_launch(name);
+    }
     auto* k = block_bwd_kernel<T, HasAct>;
     k<<<grid_of(k, blocks, kThreads / 32), kThreads, 0, s>>>(static_cast<const T*>(dy), static_cast<const uint8_t*>(q),
                                                              scale, static_cast<T*>(out), rows, cols, nb, slope);

@@ -419,7 +419,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 //   warp 1      issues M=128, N=TN, K=32 MMAs into one of kAcc accumulators of TN columns
 //   warps 2 on  promotion, kEpi = 4 or 8 warps: thread = weight row (TMEM lane), kCols of the tokens:
 //               acc[t] += d[t] * (token scale * weight scale), the products of the scales staged in
-//               shared memory a block ahead
+//               shared memory for four blocks at a time; the accumulator is read as a whole and given
+//               back before the sums, so that the tensor core waits for the read alone
 // ======================================================================================
 template <uint32_t TN>
 struct Few {
@@ -432,8 +433,8 @@ struct Few {
     static constexpr uint32_t kTokBytes = TN * kBK;
     static constexpr uint32_t kStageBytes = kPanel + kTokBytes;
     static constexpr uint32_t kStages = (kPerSm == 2 ? 100 : 210) * 1024 / kStageBytes;
-    static constexpr uint32_t kOffScale = kStages * kStageBytes;   // [2][TN] products of scales
-    static constexpr uint32_t kOffBar = kOffScale + 2 * TN * 4;
+    static constexpr uint32_t kOffScale = kStages * kStageBytes;   // [2][4][TN] products of scales
+    static constexpr uint32_t kOffBar = kOffScale + 8 * TN * 4;
     static constexpr uint32_t kSmem = kOffBar + 512 + 1024;
     static_assert(TN * 128 * 4 <= kOffScale, "the joined sums reuse the ring");
 };
@@ -559,42 +560,53 @@ __global__ void __launch_bounds__(Few<TN>::kThreads, Few<TN>::kPerSm)
         const float* sb = p.b_scale + static_cast<uint64_t>(blockIdx.y) * p.kb;
 #pragma unroll
         for (uint32_t i = 0; i < F::kCols / 2; ++i) acc[i] = make_float2(0.f, 0.f);
-        float next = tid < TN ? __ldg(sa + kb0) * __ldg(sb + kb0) : 0.f;
+        float next[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t k = min(kb0 + i, kb1 - 1);
+            next[i] = tid < TN ? __ldg(sa + k) * __ldg(sb + k) : 0.f;
+        }
         uint32_t g = 0;
         for (uint32_t kb = kb0; kb < kb1; ++kb, ++g) {
             const uint32_t ab = g % F::kAcc;
-            float* sp = prod + (g & 1) * TN;
-            if (tid < TN) {
-                sp[tid] = next;
-                const uint32_t k2 = min(kb + 1, kb1 - 1);
-                next = __ldg(sa + k2) * __ldg(sb + k2);
+            const float* sp = prod + (g & 7) * TN + col0;
+            if (g % 4 == 0) {
+                if (tid < TN) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        prod[((g & 4) + i) * TN + tid] = next[i];
+                        const uint32_t k = min(kb + 4 + i, kb1 - 1);
+                        next[i] = __ldg(sa + k) * __ldg(sb + k);
+                    }
+                }
+                // the promoting warps alone; two groups are enough, since a warp that still reads the one
+                // before last has not been here
+                asm volatile("bar.sync 1, %0;" ::"n"(32 * F::kEpi) : "memory");
             }
-            // the promoting warps alone; two buffers of products are enough, since a warp that still reads
-            // the one before last has not been here
-            asm volatile("bar.sync 1, %0;" ::"n"(32 * F::kEpi) : "memory");
             // after a wait that gave up (the error word is set) the rest runs through without waiting
             mbar_wait_bounded(&bars->acc_full[ab], (g / F::kAcc) & 1, abort_flag, &g_mm8_error_word, kErrEpi);
             __syncwarp();
             tc_fence_after();
+            uint32_t d[F::kCols / 16][16];
 #pragma unroll
-            for (uint32_t c = 0; c < F::kCols; c += 16) {
-                uint32_t d[16];
-                tmem_ld16(tmem_cols + ab * TN + c, d);
-                tmem_wait_ld16(d);
+            for (uint32_t c = 0; c < F::kCols / 16; ++c) tmem_ld16(tmem_cols + ab * TN + c * 16, d[c]);
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    const float4 f = *reinterpret_cast<const float4*>(sp + col0 + c + 4 * i);
-                    float2& a0 = acc[c / 2 + 2 * i];
-                    float2& a1 = acc[c / 2 + 2 * i + 1];
-                    a0 = __ffma2_rn(make_float2(__uint_as_float(d[4 * i]), __uint_as_float(d[4 * i + 1])),
-                                    make_float2(f.x, f.y), a0);
-                    a1 = __ffma2_rn(make_float2(__uint_as_float(d[4 * i + 2]), __uint_as_float(d[4 * i + 3])),
-                                    make_float2(f.z, f.w), a1);
-                }
-            }
+            for (uint32_t c = 0; c < F::kCols / 16; ++c) tmem_wait_ld16(d[c]);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars->acc_empty[ab]);
+#pragma unroll
+            for (uint32_t c = 0; c < F::kCols / 16; ++c)
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const float4 f = *reinterpret_cast<const float4*>(sp + c * 16 + 4 * i);
+                    float2& a0 = acc[c * 8 + 2 * i];
+                    float2& a1 = acc[c * 8 + 2 * i + 1];
+                    a0 = __ffma2_rn(make_float2(__uint_as_float(d[c][4 * i]), __uint_as_float(d[c][4 * i + 1])),
+                                    make_float2(f.x, f.y), a0);
+                    a1 = __ffma2_rn(make_float2(__uint_as_float(d[c][4 * i + 2]), __uint_as_float(d[c][4 * i + 3])),
+                                    make_float2(f.z, f.w), a1);
+                }
         }
     }
 
@@ -786,6 +798,23 @@ int launch_pair(Params p, int pairs, cudaStream_t s) {
     return check_launch("mm8_pair_kernel");
 }
 
+// Splits of K for the few-token kernel: the least work of the busiest SM, in K blocks and a join that
+// costs about as much as two; at most as many CTAs as are resident at once, unless one split is more.
+struct FewPlan {
+    uint32_t splits;
+    uint64_t cost;  // K blocks of the busiest SM
+};
+FewPlan few_plan(uint64_t tiles, uint32_t kb, uint32_t per_sm) {
+    const uint64_t sms = sm_count();
+    FewPlan best{1, ~0ull};
+    for (uint32_t c = 1; c <= 8 && c <= kb; ++c) {
+        if (c > 1 && tiles * c > sms * per_sm) break;
+        const uint64_t cost = (tiles * c + sms - 1) / sms * ((kb + c - 1) / c) + (c > 1 ? 2 : 0);
+        if (cost < best.cost) best = FewPlan{c, cost};
+    }
+    return best;
+}
+
 template <typename T, uint32_t TN>
 int launch_few(const Params& p, cudaStream_t s) {
     CUtensorMap tma, tmb;
@@ -794,19 +823,7 @@ int launch_few(const Params& p, cudaStream_t s) {
     auto* k = mm8_few_kernel<T, TN>;
     if (int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(k), Few<TN>::kSmem, "mm8_few_kernel")) return rc;
     const uint32_t token_tiles = (p.M + TN - 1) / TN;
-    // Splits of K: the least work of the busiest SM, in K blocks and a join that costs about as much as two;
-    // at most as many CTAs as are resident at once, unless even one split is more.
-    const uint64_t tiles = static_cast<uint64_t>(p.nb) * token_tiles, sms = sm_count();
-    uint32_t splits = 1;
-    uint64_t best = ~0ull;
-    for (uint32_t c = 1; c <= 8 && c <= p.kb; ++c) {
-        if (c > 1 && tiles * c > sms * Few<TN>::kPerSm) break;
-        const uint64_t cost = (tiles * c + sms - 1) / sms * ((p.kb + c - 1) / c) + (c > 1 ? 2 : 0);
-        if (cost < best) {
-            best = cost;
-            splits = c;
-        }
-    }
+    const uint32_t splits = few_plan(static_cast<uint64_t>(p.nb) * token_tiles, p.kb, Few<TN>::kPerSm).splits;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(splits, p.nb, token_tiles);
     cfg.blockDim = dim3(Few<TN>::kThreads);
@@ -839,7 +856,12 @@ int launch(Params p, cudaStream_t s) {
     const bool few_fits = p.nb <= 65535 && (p.M + 127) / 128 <= 65535;
     if (tiles > 0x7FFFFFFFull) return launch_simt<T>(p, s);
     p.num_tiles = static_cast<uint32_t>(tiles);
-    if (pairs > 0 && (!few_fits || (p.M > 128 && tiles * 4 >= static_cast<uint64_t>(pairs) * 3)))
+    // Pairs where a busy SM has no more K blocks to go through than with 128-token tiles: a block costs
+    // both about the same time, 0.65 us (4096 x 4096 weight: M = 256 15.7 us against 24 in pairs, M = 512
+    // 24 either way, M = 1024 49 against 25).
+    const uint64_t pair_cost = pairs > 0 ? (tiles + pairs - 1) / pairs * p.kb : ~0ull;
+    if (pairs > 0 && (!few_fits || (p.M > 128 && pair_cost <= few_plan(static_cast<uint64_t>(p.nb) * ((p.M + 127) / 128),
+                                                                       p.kb, Few<128>::kPerSm).cost)))
         return launch_pair<T>(p, pairs, s);
     if (!few_fits) return launch_simt<T>(p, s);
     if (p.M <= 16) return launch_few<T, 16>(p, s);
