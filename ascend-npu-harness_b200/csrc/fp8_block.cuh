@@ -28,9 +28,13 @@ constexpr uint32_t kFp8FloorBits = 0x0D800000u;  // 2^-100
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
-// amax bits (unfloored) -> multiplier 448 / amax and scale amax / 448.
+// The block's amax from the bits of its largest magnitude.
+__device__ __forceinline__ float fp8_amax(uint32_t bits) {
+    return __uint_as_float(bits < kFp8FloorBits ? kFp8FloorBits : bits);
+}
+// Multiplier 448 / amax and scale amax / 448.
 __device__ __forceinline__ void fp8_block_scale(uint32_t bits, float& inv, float& scale) {
-    const float amax = __uint_as_float(bits < kFp8FloorBits ? kFp8FloorBits : bits);
+    const float amax = fp8_amax(bits);
     inv = __fdiv_rn(kFp8Max, amax);
     scale = __fdiv_rn(amax, kFp8Max);
 }

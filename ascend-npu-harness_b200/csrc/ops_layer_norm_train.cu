@@ -187,13 +187,345 @@ __global__ void __launch_bounds__(kThreads) ln_bwd_join_kernel(const float* __re
     }
 }
 
+// ---------------------------------------------------------------------------------------
+// Rows of up to 8192 elements: W warps own a row, 16 columns per thread in registers, the next row's
+// loads issued before the current row is worked on.
+//
+// Rows of whole, aligned 16-byte packs (Vec): thread t holds packs t + 32 W j, so 16 (fp32: 32)
+// neighbouring lanes hold a block of 128 and its maximum is a shuffle tree.  Other rows: thread t
+// holds elements t + 32 W i.  Columns behind the row's end hold zeros and are not stored.
+// ---------------------------------------------------------------------------------------
+constexpr int kCpt = 16;
+constexpr uint32_t kMaxFastH = 32 * 16 * kCpt;
+
+constexpr int group_threads(int W) { return W <= 8 ? 256 : 32 * W; }
+constexpr int row_groups(int W) { return group_threads(W) / (32 * W); }
+
+// Raw bits of a thread's 16 columns of one row, and their values.
+template <typename T, int W, bool Vec>
+struct RowPart {
+    static constexpr int P = elem<T>::kPack, N = Vec ? kCpt / P : kCpt;
+    using Raw = typename std::conditional<Vec, pack<T>, T>::type;
+    Raw r[N];
+    __device__ __forceinline__ static uint32_t first(uint32_t t, int i) { return Vec ? (t + 32 * W * i) * P : t + 32 * W * i; }
+    __device__ __forceinline__ void load(const T* row, uint32_t t, uint32_t H) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (first(t, i) >= H) continue;
+            if constexpr (Vec) r[i] = ld_stream(reinterpret_cast<const pack<T>*>(row + first(t, i)));
+            else r[i] = row[first(t, i)];
+        }
+    }
+    __device__ __forceinline__ void values(float (&v)[kCpt], uint32_t t, uint32_t H) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int e = 0; e < kCpt / N; ++e) {
+                T x;
+                if constexpr (Vec) x = r[i].v[e];
+                else x = r[i];
+                v[i * (kCpt / N) + e] = first(t, i) < H ? elem<T>::to_f(x) : 0.f;
+            }
+    }
+    __device__ __forceinline__ static void store(T* row, const float (&v)[kCpt], uint32_t t, uint32_t H) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (first(t, i) >= H) continue;
+            if constexpr (Vec) st_stream(reinterpret_cast<pack<T>*>(row + first(t, i)), pack_from_f<T>(v + i * P));
+            else row[first(t, i)] = elem<T>::from_f(v[i]);
+        }
+    }
+    // Parameters of the thread's columns (read once per thread; zeros behind the end).
+    __device__ __forceinline__ static void params(const float* p, float (&v)[kCpt], uint32_t t, uint32_t H) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int e = 0; e < kCpt / N; ++e)
+                v[i * (kCpt / N) + e] = first(t, i) < H ? __ldg(p + first(t, i) + e) : 0.f;
+    }
+};
+
+// Sums of two values over the W warps of a row, the same bits in every thread.  `sh` alternates
+// between two buffers from call to call: whoever writes one again has passed the barrier that
+// everybody reached after reading it.
+template <int W>
+__device__ __forceinline__ float2 row_sum2(float2 v, float2* sh, uint32_t group, uint32_t warp_in_row) {
+    v.x = warp_sum(v.x);
+    v.y = warp_sum(v.y);
+    if (W == 1) return v;
+    if ((threadIdx.x & 31) == 0) sh[warp_in_row] = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * W) : "memory");
+    float2 s = sh[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+        s.x += sh[w].x;
+        s.y += sh[w].y;
+    }
+    return s;
+}
+
+template <typename T, int W, bool Vec, bool Ckpt>
+__global__ void __launch_bounds__(group_threads(W)) ln_fwd_row_kernel(const FwdArgs a) {
+    using Row = RowPart<T, W, Vec>;
+    constexpr int G = row_groups(W), P = Row::P;
+    __shared__ float2 sh[G][2][W];
+    __shared__ alignas(16) uint32_t quarter[Ckpt && !Vec ? G : 1][Ckpt && !Vec ? W * kCpt : 4];
+    const uint32_t group = threadIdx.x / (32 * W), t = threadIdx.x % (32 * W), wir = t / 32;
+    const uint32_t stride = gridDim.x * G;
+    const float H = static_cast<float>(a.H);
+    float gamma[kCpt], beta[kCpt];
+    Row::params(a.gamma, gamma, t, a.H);
+    Row::params(a.beta, beta, t, a.H);
+    uint64_t row = static_cast<uint64_t>(blockIdx.x) * G + group;
+    const T* x = static_cast<const T*>(a.x);
+    Row next;
+    float k_next = 0.f;
+    if (row < a.rows) {
+        next.load(x + row * a.H, t, a.H);
+        k_next = elem<T>::to_f(x[row * a.H]);
+    }
+    for (; row < a.rows; row += stride) {
+        float v[kCpt];
+        next.values(v, t, a.H);
+        const float K = k_next;
+        if (row + stride < a.rows) {
+            next.load(x + (row + stride) * a.H, t, a.H);
+            k_next = elem<T>::to_f(x[(row + stride) * a.H]);
+        }
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < Row::N; ++i)
+            if (Row::first(t, i) < a.H)
+#pragma unroll
+                for (int e = 0; e < kCpt / Row::N; ++e) s += v[i * (kCpt / Row::N) + e] - K;
+        const float mean = K + __fdiv_rn(row_sum2<W>(make_float2(s, 0.f), sh[group][0], group, wir).x, H);
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < Row::N; ++i)
+#pragma unroll
+            for (int e = 0; e < kCpt / Row::N; ++e) {
+                float& d = v[i * (kCpt / Row::N) + e];
+                d = Row::first(t, i) < a.H ? d - mean : 0.f;
+                s = fmaf(d, d, s);
+            }
+        const float var = __fdiv_rn(row_sum2<W>(make_float2(s, 0.f), sh[group][1], group, wir).x, H);
+        const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(var + a.eps));
+        if (t == 0) {
+            if (a.mean) a.mean[row] = mean;
+            a.rstd[row] = rstd;
+        }
+#pragma unroll
+        for (int i = 0; i < kCpt; ++i) v[i] *= rstd;
+        if constexpr (Ckpt && Vec) {
+#pragma unroll
+            for (int i = 0; i < Row::N; ++i) {
+                uint32_t m = 0;
+#pragma unroll
+                for (int e = 0; e < P; ++e) m = max(m, abs_bits(v[i * P + e]));
+#pragma unroll
+                for (uint32_t o = kFp8Block / P / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                float inv, sc;
+                fp8_block_scale(m, inv, sc);
+                const uint32_t c = Row::first(t, i);
+                if (c >= a.H) continue;
+                if (c % kFp8Block == 0) a.scale[row * a.row_blocks + c / kFp8Block] = sc;
+                uint32_t w[P / 4];
+#pragma unroll
+                for (int e = 0; e < P; e += 4)
+                    w[e / 4] = fp8_encode2(__fmul_rn(v[i * P + e], inv), __fmul_rn(v[i * P + e + 1], inv)) |
+                               fp8_encode2(__fmul_rn(v[i * P + e + 2], inv), __fmul_rn(v[i * P + e + 3], inv)) << 16;
+                uint8_t* q = a.q + row * a.H + c;
+                if constexpr (P == 8) __stcs(reinterpret_cast<uint2*>(q), make_uint2(w[0], w[1]));
+                else __stcs(reinterpret_cast<uint32_t*>(q), w[0]);
+            }
+        } else if constexpr (Ckpt) {
+            // a warp's 32 neighbouring columns are a quarter of a block: its maximum from four of them
+#pragma unroll
+            for (int i = 0; i < kCpt; ++i) {
+                const uint32_t m = warp_umax(abs_bits(v[i]));
+                if (t % 32 == 0) quarter[group][W * i + wir] = m;
+            }
+            if (W == 1) __syncwarp();
+            else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * W) : "memory");
+#pragma unroll
+            for (int i = 0; i < kCpt; ++i) {
+                const uint32_t b = (W * i + wir) / 4;
+                const uint4 m = *reinterpret_cast<const uint4*>(&quarter[group][b * 4]);
+                float inv, sc;
+                fp8_block_scale(max(max(m.x, m.y), max(m.z, m.w)), inv, sc);
+                const uint32_t c = Row::first(t, i);
+                if (c >= a.H) continue;
+                if (c % kFp8Block == 0) a.scale[row * a.row_blocks + b] = sc;
+                a.q[row * a.H + c] = fp8_encode(__fmul_rn(v[i], inv));
+            }
+            if (W == 1) __syncwarp();  // with more warps, the next row's sums lie between this read and the next write
+        }
+#pragma unroll
+        for (int i = 0; i < kCpt; ++i) v[i] = fmaf(v[i], gamma[i], beta[i]);
+        Row::store(static_cast<T*>(a.y) + row * a.H, v, t, a.H);
+    }
+}
+
+// A thread's 16 columns of xh from the checkpoint: codes and scales, loaded like RowPart.
+template <int W, bool Vec, int P>
+struct CkptPart {
+    static constexpr int N = Vec ? kCpt / P : kCpt;
+    uint32_t code[N * (Vec ? P / 4 : 1)];
+    float s[N];
+    __device__ __forceinline__ void load(const uint8_t* q, const float* scale, uint32_t t, uint32_t H) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t c = Vec ? (t + 32 * W * i) * P : t + 32 * W * i;
+            if (c >= H) continue;
+            if constexpr (!Vec) code[i] = q[c];
+            else if constexpr (P == 8) {
+                const uint2 v = __ldcs(reinterpret_cast<const uint2*>(q + c));
+                code[2 * i] = v.x;
+                code[2 * i + 1] = v.y;
+            } else code[i] = __ldcs(reinterpret_cast<const uint32_t*>(q + c));
+            s[i] = __ldg(scale + c / kFp8Block);
+        }
+    }
+    __device__ __forceinline__ void values(float (&v)[kCpt], uint32_t t, uint32_t H) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bool in = (Vec ? (t + 32 * W * i) * P : t + 32 * W * i) < H;
+            if constexpr (Vec) {
+#pragma unroll
+                for (int e = 0; e < P; e += 2) {
+                    const float2 f = fp8_decode2(code[i * (P / 4) + e / 4] >> (e % 4 * 8));
+                    v[i * P + e] = in ? __fmul_rn(f.x, s[i]) : 0.f;
+                    v[i * P + e + 1] = in ? __fmul_rn(f.y, s[i]) : 0.f;
+                }
+            } else {
+                v[i] = in ? __fmul_rn(fp8_decode(static_cast<uint8_t>(code[i])), s[i]) : 0.f;
+            }
+        }
+    }
+};
+
+// dx of every row, and this CTA's sums over its rows of dy xh and dy: 16 columns per thread in
+// registers over all its rows, joined over the CTA's row groups at the end.
+template <typename T, int W, bool Vec, bool Ckpt>
+__global__ void __launch_bounds__(group_threads(W), W <= 8 ? 2 : 1) ln_bwd_row_kernel(const BwdArgs a) {
+    using Row = RowPart<T, W, Vec>;
+    using Part = typename std::conditional<Ckpt, CkptPart<W, Vec, Row::P>, Row>::type;
+    constexpr int G = row_groups(W);
+    __shared__ float2 sh[G][2][W];
+    __shared__ float joined[G > 1 ? G * 2 * 32 * W * kCpt : 1];
+    const uint32_t group = threadIdx.x / (32 * W), t = threadIdx.x % (32 * W), wir = t / 32;
+    const uint32_t stride = gridDim.x * G;
+    const float inv_h = 1.0f / static_cast<float>(a.H);
+    float gamma[kCpt], dgamma[kCpt], dbeta[kCpt];
+    Row::params(a.gamma, gamma, t, a.H);
+#pragma unroll
+    for (int i = 0; i < kCpt; ++i) dgamma[i] = dbeta[i] = 0.f;
+    uint64_t row = static_cast<uint64_t>(blockIdx.x) * G + group;
+    Row dy_next;
+    Part x_next;
+    float mean_next = 0.f, rstd_next = 0.f;
+    auto fetch = [&](uint64_t r) {
+        dy_next.load(static_cast<const T*>(a.dy) + r * a.H, t, a.H);
+        if constexpr (Ckpt) {
+            x_next.load(a.q + r * a.H, a.scale + r * a.row_blocks, t, a.H);
+        } else {
+            x_next.load(static_cast<const T*>(a.x) + r * a.H, t, a.H);
+            mean_next = __ldg(a.mean + r);
+        }
+        rstd_next = __ldg(a.rstd + r);
+    };
+    if (row < a.rows) fetch(row);
+    uint32_t flip = 0;
+    for (; row < a.rows; row += stride, flip ^= 1) {
+        float g[kCpt], xh[kCpt];
+        dy_next.values(g, t, a.H);
+        x_next.values(xh, t, a.H);
+        const float mean = mean_next, rstd = rstd_next;
+        if (row + stride < a.rows) fetch(row + stride);
+        float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < kCpt; ++i) {
+            if constexpr (!Ckpt) xh[i] = (xh[i] - mean) * rstd;  // meets g = 0 behind the row's end
+            dgamma[i] = fmaf(g[i], xh[i], dgamma[i]);
+            dbeta[i] += g[i];
+            g[i] *= gamma[i];
+            s.x += g[i];
+            s.y = fmaf(g[i], xh[i], s.y);
+        }
+        s = row_sum2<W>(s, sh[group][flip], group, wir);
+        const float c1 = s.x * inv_h, c2 = s.y * inv_h;
+#pragma unroll
+        for (int i = 0; i < kCpt; ++i) g[i] = rstd * (g[i] - c1 - xh[i] * c2);
+        Row::store(static_cast<T*>(a.dx) + row * a.H, g, t, a.H);
+    }
+    float* part = a.parts + static_cast<uint64_t>(blockIdx.x) * 2 * a.H;
+    if constexpr (G > 1) {  // columns in thread order: [group][dgamma, dbeta][i][t]
+        float* mine = joined + group * 2 * 32 * W * kCpt;
+#pragma unroll
+        for (int i = 0; i < kCpt; ++i) {
+            mine[i * 32 * W + t] = dgamma[i];
+            mine[(kCpt + i) * 32 * W + t] = dbeta[i];
+        }
+        __syncthreads();
+        if (group != 0) return;
+#pragma unroll
+        for (int i = 0; i < kCpt; ++i)
+            for (int o = 1; o < G; ++o) {
+                dgamma[i] += joined[(o * 2 * kCpt + i) * 32 * W + t];
+                dbeta[i] += joined[((o * 2 + 1) * kCpt + i) * 32 * W + t];
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < Row::N; ++i) {
+        const uint32_t c = Row::first(t, i);
+        if (c >= a.H) continue;
+#pragma unroll
+        for (int e = 0; e < kCpt / Row::N; ++e) {
+            part[c + e] = dgamma[i * (kCpt / Row::N) + e];
+            part[a.H + c + e] = dbeta[i * (kCpt / Row::N) + e];
+        }
+    }
+}
+
+// Calls f with the number of warps that own a row of H <= kMaxFastH elements.
+template <typename F>
+int by_warps(uint32_t H, F f) {
+    if (H <= 32 * kCpt) return f(std::integral_constant<int, 1>{});
+    if (H <= 64 * kCpt) return f(std::integral_constant<int, 2>{});
+    if (H <= 128 * kCpt) return f(std::integral_constant<int, 4>{});
+    if (H <= 256 * kCpt) return f(std::integral_constant<int, 8>{});
+    return f(std::integral_constant<int, 16>{});
+}
+
 unsigned row_grid(const void* kernel, uint32_t rows) {
     const uint64_t cap = static_cast<uint64_t>(resident_blocks(kernel, kThreads, 0));
     return static_cast<unsigned>(rows < cap ? rows : (cap ? cap : 1));
 }
 
 template <typename T>
+bool packs_ok(uint32_t H, const void* a, const void* b) {
+    return H % elem<T>::kPack == 0 && aligned16(a) && aligned16(b);
+}
+
+template <typename T, bool Vec, bool Ckpt>
+int launch_fwd_rows(const FwdArgs& a, cudaStream_t s) {
+    return by_warps(a.H, [&](auto w) {
+        constexpr int W = decltype(w)::value;
+        auto* k = ln_fwd_row_kernel<T, W, Vec, Ckpt>;
+        const uint64_t groups = (static_cast<uint64_t>(a.rows) + row_groups(W) - 1) / row_groups(W);
+        const uint64_t cap = static_cast<uint64_t>(resident_blocks(reinterpret_cast<const void*>(k), group_threads(W), 0));
+        k<<<static_cast<unsigned>(groups < cap ? groups : (cap ? cap : 1)), group_threads(W), 0, s>>>(a);
+        return check_launch("layer_norm_fwd_train");
+    });
+}
+
+template <typename T>
 int launch_fwd(const FwdArgs& a, cudaStream_t s) {
+    const bool vec = packs_ok<T>(a.H, a.x, a.y) && reinterpret_cast<uintptr_t>(a.q) % elem<T>::kPack == 0;
+    if (a.H <= kMaxFastH) {
+        if (vec) return a.q ? launch_fwd_rows<T, true, true>(a, s) : launch_fwd_rows<T, true, false>(a, s);
+        return a.q ? launch_fwd_rows<T, false, true>(a, s) : launch_fwd_rows<T, false, false>(a, s);
+    }
     auto* k = ln_fwd_any_kernel<T>;
     k<<<row_grid(reinterpret_cast<const void*>(k), a.rows), kThreads, 0, s>>>(a);
     return check_launch("layer_norm_fwd_train");
@@ -201,15 +533,32 @@ int launch_fwd(const FwdArgs& a, cudaStream_t s) {
 
 uint32_t parts_of(uint32_t rows) { return rows < kMaxParts ? rows : kMaxParts; }
 
+template <typename T, bool Vec, bool Ckpt>
+int launch_bwd_rows(BwdArgs& a, cudaStream_t s) {
+    return by_warps(a.H, [&](auto w) {
+        constexpr int W = decltype(w)::value;
+        const uint32_t groups = (a.rows + row_groups(W) - 1) / row_groups(W);
+        a.parts_n = parts_of(groups);  // one per CTA
+        ln_bwd_row_kernel<T, W, Vec, Ckpt><<<a.parts_n, group_threads(W), 0, s>>>(a);
+        return check_launch("layer_norm_bwd");
+    });
+}
+
 template <typename T, bool Ckpt>
 int launch_bwd(BwdArgs a, float* dgamma, float* dbeta, cudaStream_t s) {
-    a.rows_per_part = (a.rows + parts_of(a.rows) - 1) / parts_of(a.rows);
-    a.parts_n = (a.rows + a.rows_per_part - 1) / a.rows_per_part;
-    auto* k = ln_bwd_dx_any_kernel<T, Ckpt>;
-    k<<<row_grid(reinterpret_cast<const void*>(k), a.rows), kThreads, 0, s>>>(a);
-    if (int rc = check_launch("layer_norm_bwd")) return rc;
-    ln_bwd_cols_any_kernel<T, Ckpt><<<dim3((a.H + 31) / 32, a.parts_n), kThreads, 0, s>>>(a);
-    if (int rc = check_launch("layer_norm_bwd")) return rc;
+    if (a.H <= kMaxFastH) {
+        const bool vec = packs_ok<T>(a.H, a.dy, a.dx) && (Ckpt || aligned16(a.x)) &&
+                         reinterpret_cast<uintptr_t>(a.q) % elem<T>::kPack == 0;
+        if (int rc = vec ? launch_bwd_rows<T, true, Ckpt>(a, s) : launch_bwd_rows<T, false, Ckpt>(a, s)) return rc;
+    } else {
+        a.rows_per_part = (a.rows + parts_of(a.rows) - 1) / parts_of(a.rows);
+        a.parts_n = (a.rows + a.rows_per_part - 1) / a.rows_per_part;
+        auto* k = ln_bwd_dx_any_kernel<T, Ckpt>;
+        k<<<row_grid(reinterpret_cast<const void*>(k), a.rows), kThreads, 0, s>>>(a);
+        if (int rc = check_launch("layer_norm_bwd")) return rc;
+        ln_bwd_cols_any_kernel<T, Ckpt><<<dim3((a.H + 31) / 32, a.parts_n), kThreads, 0, s>>>(a);
+        if (int rc = check_launch("layer_norm_bwd")) return rc;
+    }
     ln_bwd_join_kernel<<<dim3((a.H + 31) / 32, 2), kThreads, 0, s>>>(a.parts, a.parts_n, a.H, dgamma, dbeta);
     return check_launch("layer_norm_bwd");
 }
