@@ -201,47 +201,96 @@ constexpr uint32_t kMaxFastH = 32 * 16 * kCpt;
 constexpr int group_threads(int W) { return W <= 8 ? 256 : 32 * W; }
 constexpr int row_groups(int W) { return group_threads(W) / (32 * W); }
 
-// Raw bits of a thread's 16 columns of one row, and their values.
+// fp32 pairs: one instruction for two elements.
+__device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
+constexpr int kPairs = kCpt / 2;
+
+__device__ __forceinline__ float2 unpack2(uint32_t w, bf16_t) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w, f16_t) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+
+// Raw bits of a thread's 16 columns of one row, and their values.  Columns behind the end are zeros
+// from the start and never loaded.
 template <typename T, int W, bool Vec>
 struct RowPart {
     static constexpr int P = elem<T>::kPack, N = Vec ? kCpt / P : kCpt;
-    using Raw = typename std::conditional<Vec, pack<T>, T>::type;
+    static constexpr int kRun = kCpt / N;  // neighbouring columns of one load
+    using Raw = typename std::conditional<Vec, uint4, T>::type;
     Raw r[N];
     __device__ __forceinline__ static uint32_t first(uint32_t t, int i) { return Vec ? (t + 32 * W * i) * P : t + 32 * W * i; }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) r[i] = Raw{};
+    }
     __device__ __forceinline__ void load(const T* row, uint32_t t, uint32_t H) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             if (first(t, i) >= H) continue;
-            if constexpr (Vec) r[i] = ld_stream(reinterpret_cast<const pack<T>*>(row + first(t, i)));
+            if constexpr (Vec) r[i] = __ldcs(reinterpret_cast<const uint4*>(row + first(t, i)));
             else r[i] = row[first(t, i)];
         }
     }
-    __device__ __forceinline__ void values(float (&v)[kCpt], uint32_t t, uint32_t H) const {
+    __device__ __forceinline__ void values(float2 (&v)[kPairs]) const {
+        if constexpr (!Vec) {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
+            for (int i = 0; i < kPairs; ++i) v[i] = make_float2(elem<T>::to_f(r[2 * i]), elem<T>::to_f(r[2 * i + 1]));
+        } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int e = 0; e < kCpt / N; ++e) {
-                T x;
-                if constexpr (Vec) x = r[i].v[e];
-                else x = r[i];
-                v[i * (kCpt / N) + e] = first(t, i) < H ? elem<T>::to_f(x) : 0.f;
+            for (int i = 0; i < N; ++i) {
+                v[2 * i] = make_float2(__uint_as_float(r[i].x), __uint_as_float(r[i].y));
+                v[2 * i + 1] = make_float2(__uint_as_float(r[i].z), __uint_as_float(r[i].w));
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                v[4 * i] = unpack2(r[i].x, T{});
+                v[4 * i + 1] = unpack2(r[i].y, T{});
+                v[4 * i + 2] = unpack2(r[i].z, T{});
+                v[4 * i + 3] = unpack2(r[i].w, T{});
+            }
+        }
     }
-    __device__ __forceinline__ static void store(T* row, const float (&v)[kCpt], uint32_t t, uint32_t H) {
+    __device__ __forceinline__ static void store(T* row, const float2 (&v)[kPairs], uint32_t t, uint32_t H) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             if (first(t, i) >= H) continue;
-            if constexpr (Vec) st_stream(reinterpret_cast<pack<T>*>(row + first(t, i)), pack_from_f<T>(v + i * P));
-            else row[first(t, i)] = elem<T>::from_f(v[i]);
+            if constexpr (Vec)
+                st_stream(reinterpret_cast<pack<T>*>(row + first(t, i)), pack_from_f<T>(&v[i * P / 2].x));
+            else row[first(t, i)] = elem<T>::from_f(i & 1 ? v[i / 2].y : v[i / 2].x);
         }
     }
     // Parameters of the thread's columns (read once per thread; zeros behind the end).
-    __device__ __forceinline__ static void params(const float* p, float (&v)[kCpt], uint32_t t, uint32_t H) {
+    __device__ __forceinline__ static void params(const float* p, float2 (&v)[kPairs], uint32_t t, uint32_t H) {
+        float f[kCpt];
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int e = 0; e < kCpt / N; ++e)
-                v[i * (kCpt / N) + e] = first(t, i) < H ? __ldg(p + first(t, i) + e) : 0.f;
+            for (int e = 0; e < kRun; ++e) f[i * kRun + e] = first(t, i) < H ? __ldg(p + first(t, i) + e) : 0.f;
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) v[i] = make_float2(f[2 * i], f[2 * i + 1]);
+    }
+    // v -= m in the columns of the row, leaving zeros behind its end; the sum of what `f` makes of each
+    // pair, over the thread's columns.
+    template <typename F>
+    __device__ __forceinline__ static float sum_of(float2 (&v)[kPairs], uint32_t t, uint32_t H, F f) {
+        float2 s = f2(0.f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (Vec) {
+                if (first(t, i) >= H) continue;
+#pragma unroll
+                for (int e = 0; e < kRun / 2; ++e) s = f(v[i * kRun / 2 + e], s);
+            } else if (i % 2 == 0) {  // a pair's two columns end separately
+                if (first(t, i + 1) < H) s = f(v[i / 2], s);
+                else if (first(t, i) < H) {
+                    float2 one = v[i / 2];
+                    s.x = f(one, s).x;
+                    v[i / 2] = make_float2(one.x, 0.f);
+                }
+            }
+        }
+        return s.x + s.y;
     }
 };
 
@@ -264,76 +313,84 @@ __device__ __forceinline__ float2 row_sum2(float2 v, float2* sh, uint32_t group,
     return s;
 }
 
+template <int W>
+__device__ __forceinline__ float row_sum(float v, float* sh, uint32_t group, uint32_t warp_in_row) {
+    v = warp_sum(v);
+    if (W == 1) return v;
+    if ((threadIdx.x & 31) == 0) sh[warp_in_row] = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * W) : "memory");
+    float s = sh[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) s += sh[w];
+    return s;
+}
+
 template <typename T, int W, bool Vec, bool Ckpt>
 __global__ void __launch_bounds__(group_threads(W)) ln_fwd_row_kernel(const FwdArgs a) {
     using Row = RowPart<T, W, Vec>;
     constexpr int G = row_groups(W), P = Row::P;
-    __shared__ float2 sh[G][2][W];
+    __shared__ float sh[G][2][W];
     __shared__ alignas(16) uint32_t quarter[Ckpt && !Vec ? G : 1][Ckpt && !Vec ? W * kCpt : 4];
     const uint32_t group = threadIdx.x / (32 * W), t = threadIdx.x % (32 * W), wir = t / 32;
     const uint32_t stride = gridDim.x * G;
     const float H = static_cast<float>(a.H);
-    float gamma[kCpt], beta[kCpt];
+    float2 gamma[kPairs], beta[kPairs];
     Row::params(a.gamma, gamma, t, a.H);
     Row::params(a.beta, beta, t, a.H);
     uint64_t row = static_cast<uint64_t>(blockIdx.x) * G + group;
     const T* x = static_cast<const T*>(a.x);
     Row next;
+    next.clear();
     float k_next = 0.f;
     if (row < a.rows) {
         next.load(x + row * a.H, t, a.H);
         k_next = elem<T>::to_f(x[row * a.H]);
     }
     for (; row < a.rows; row += stride) {
-        float v[kCpt];
-        next.values(v, t, a.H);
+        float2 v[kPairs];
+        next.values(v);
         const float K = k_next;
         if (row + stride < a.rows) {
             next.load(x + (row + stride) * a.H, t, a.H);
             k_next = elem<T>::to_f(x[(row + stride) * a.H]);
         }
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < Row::N; ++i)
-            if (Row::first(t, i) < a.H)
-#pragma unroll
-                for (int e = 0; e < kCpt / Row::N; ++e) s += v[i * (kCpt / Row::N) + e] - K;
-        const float mean = K + __fdiv_rn(row_sum2<W>(make_float2(s, 0.f), sh[group][0], group, wir).x, H);
-        s = 0.f;
-#pragma unroll
-        for (int i = 0; i < Row::N; ++i)
-#pragma unroll
-            for (int e = 0; e < kCpt / Row::N; ++e) {
-                float& d = v[i * (kCpt / Row::N) + e];
-                d = Row::first(t, i) < a.H ? d - mean : 0.f;
-                s = fmaf(d, d, s);
-            }
-        const float var = __fdiv_rn(row_sum2<W>(make_float2(s, 0.f), sh[group][1], group, wir).x, H);
+        float s = Row::sum_of(v, t, a.H, [&](float2& p, float2 s) { return __fadd2_rn(s, __fadd2_rn(p, f2(-K))); });
+        const float mean = K + __fdiv_rn(row_sum<W>(s, sh[group][0], group, wir), H);
+        s = Row::sum_of(v, t, a.H, [&](float2& p, float2 s) {
+            p = __fadd2_rn(p, f2(-mean));
+            return __ffma2_rn(p, p, s);
+        });
+        const float var = __fdiv_rn(row_sum<W>(s, sh[group][1], group, wir), H);
         const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(var + a.eps));
         if (t == 0) {
             if (a.mean) a.mean[row] = mean;
             a.rstd[row] = rstd;
         }
 #pragma unroll
-        for (int i = 0; i < kCpt; ++i) v[i] *= rstd;
+        for (int i = 0; i < kPairs; ++i) v[i] = __fmul2_rn(v[i], f2(rstd));
         if constexpr (Ckpt && Vec) {
 #pragma unroll
             for (int i = 0; i < Row::N; ++i) {
+                const float2* h = v + i * P / 2;
                 uint32_t m = 0;
 #pragma unroll
-                for (int e = 0; e < P; ++e) m = max(m, abs_bits(v[i * P + e]));
+                for (int e = 0; e < P / 2; ++e) m = max(m, max(abs_bits(h[e].x), abs_bits(h[e].y)));
 #pragma unroll
                 for (uint32_t o = kFp8Block / P / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-                float inv, sc;
-                fp8_block_scale(m, inv, sc);
+                // one division for both quotients: even lanes 448 / amax, odd lanes the scale
+                const float amax = fp8_amax(m);
+                const float ratio = __fdiv_rn(t & 1 ? amax : kFp8Max, t & 1 ? kFp8Max : amax);
+                const float other = __shfl_xor_sync(0xffffffffu, ratio, 1);
+                const float inv = t & 1 ? other : ratio;
                 const uint32_t c = Row::first(t, i);
                 if (c >= a.H) continue;
-                if (c % kFp8Block == 0) a.scale[row * a.row_blocks + c / kFp8Block] = sc;
+                if (c % kFp8Block == 0) a.scale[row * a.row_blocks + c / kFp8Block] = other;
                 uint32_t w[P / 4];
 #pragma unroll
-                for (int e = 0; e < P; e += 4)
-                    w[e / 4] = fp8_encode2(__fmul_rn(v[i * P + e], inv), __fmul_rn(v[i * P + e + 1], inv)) |
-                               fp8_encode2(__fmul_rn(v[i * P + e + 2], inv), __fmul_rn(v[i * P + e + 3], inv)) << 16;
+                for (int e = 0; e < P / 2; e += 2) {
+                    const float2 lo = __fmul2_rn(h[e], f2(inv)), hi = __fmul2_rn(h[e + 1], f2(inv));
+                    w[e / 2] = fp8_encode2(lo.x, lo.y) | fp8_encode2(hi.x, hi.y) << 16;
+                }
                 uint8_t* q = a.q + row * a.H + c;
                 if constexpr (P == 8) __stcs(reinterpret_cast<uint2*>(q), make_uint2(w[0], w[1]));
                 else __stcs(reinterpret_cast<uint32_t*>(q), w[0]);
@@ -342,7 +399,7 @@ __global__ void __launch_bounds__(group_threads(W)) ln_fwd_row_kernel(const FwdA
             // a warp's 32 neighbouring columns are a quarter of a block: its maximum from four of them
 #pragma unroll
             for (int i = 0; i < kCpt; ++i) {
-                const uint32_t m = warp_umax(abs_bits(v[i]));
+                const uint32_t m = warp_umax(abs_bits(i & 1 ? v[i / 2].y : v[i / 2].x));
                 if (t % 32 == 0) quarter[group][W * i + wir] = m;
             }
             if (W == 1) __syncwarp();
@@ -356,12 +413,12 @@ __global__ void __launch_bounds__(group_threads(W)) ln_fwd_row_kernel(const FwdA
                 const uint32_t c = Row::first(t, i);
                 if (c >= a.H) continue;
                 if (c % kFp8Block == 0) a.scale[row * a.row_blocks + b] = sc;
-                a.q[row * a.H + c] = fp8_encode(__fmul_rn(v[i], inv));
+                a.q[row * a.H + c] = fp8_encode(__fmul_rn(i & 1 ? v[i / 2].y : v[i / 2].x, inv));
             }
             if (W == 1) __syncwarp();  // with more warps, the next row's sums lie between this read and the next write
         }
 #pragma unroll
-        for (int i = 0; i < kCpt; ++i) v[i] = fmaf(v[i], gamma[i], beta[i]);
+        for (int i = 0; i < kPairs; ++i) v[i] = __ffma2_rn(v[i], gamma[i], beta[i]);
         Row::store(static_cast<T*>(a.y) + row * a.H, v, t, a.H);
     }
 }
@@ -370,8 +427,14 @@ __global__ void __launch_bounds__(group_threads(W)) ln_fwd_row_kernel(const FwdA
 template <int W, bool Vec, int P>
 struct CkptPart {
     static constexpr int N = Vec ? kCpt / P : kCpt;
-    uint32_t code[N * (Vec ? P / 4 : 1)];
+    uint32_t code[Vec ? kCpt / 4 : kCpt];
     float s[N];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < (Vec ? kCpt / 4 : kCpt); ++i) code[i] = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] = 0.f;
+    }
     __device__ __forceinline__ void load(const uint8_t* q, const float* scale, uint32_t t, uint32_t H) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -386,20 +449,13 @@ struct CkptPart {
             s[i] = __ldg(scale + c / kFp8Block);
         }
     }
-    __device__ __forceinline__ void values(float (&v)[kCpt], uint32_t t, uint32_t H) const {
+    __device__ __forceinline__ void values(float2 (&v)[kPairs]) const {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const bool in = (Vec ? (t + 32 * W * i) * P : t + 32 * W * i) < H;
-            if constexpr (Vec) {
-#pragma unroll
-                for (int e = 0; e < P; e += 2) {
-                    const float2 f = fp8_decode2(code[i * (P / 4) + e / 4] >> (e % 4 * 8));
-                    v[i * P + e] = in ? __fmul_rn(f.x, s[i]) : 0.f;
-                    v[i * P + e + 1] = in ? __fmul_rn(f.y, s[i]) : 0.f;
-                }
-            } else {
-                v[i] = in ? __fmul_rn(fp8_decode(static_cast<uint8_t>(code[i])), s[i]) : 0.f;
-            }
+        for (int i = 0; i < kPairs; ++i) {
+            if constexpr (Vec)
+                v[i] = __fmul2_rn(fp8_decode2(code[i / 2] >> (i % 2 * 16)), f2(s[2 * i / P]));
+            else
+                v[i] = __fmul2_rn(fp8_decode2(code[2 * i] | code[2 * i + 1] << 8), make_float2(s[2 * i], s[2 * i + 1]));
         }
     }
 };
@@ -412,17 +468,19 @@ __global__ void __launch_bounds__(group_threads(W), W <= 8 ? 2 : 1) ln_bwd_row_k
     using Part = typename std::conditional<Ckpt, CkptPart<W, Vec, Row::P>, Row>::type;
     constexpr int G = row_groups(W);
     __shared__ float2 sh[G][2][W];
-    __shared__ float joined[G > 1 ? G * 2 * 32 * W * kCpt : 1];
+    __shared__ float2 joined[G > 1 ? G * 2 * 32 * W * kPairs : 1];
     const uint32_t group = threadIdx.x / (32 * W), t = threadIdx.x % (32 * W), wir = t / 32;
     const uint32_t stride = gridDim.x * G;
     const float inv_h = 1.0f / static_cast<float>(a.H);
-    float gamma[kCpt], dgamma[kCpt], dbeta[kCpt];
+    float2 gamma[kPairs], dgamma[kPairs], dbeta[kPairs];
     Row::params(a.gamma, gamma, t, a.H);
 #pragma unroll
-    for (int i = 0; i < kCpt; ++i) dgamma[i] = dbeta[i] = 0.f;
+    for (int i = 0; i < kPairs; ++i) dgamma[i] = dbeta[i] = f2(0.f);
     uint64_t row = static_cast<uint64_t>(blockIdx.x) * G + group;
     Row dy_next;
     Part x_next;
+    dy_next.clear();
+    x_next.clear();
     float mean_next = 0.f, rstd_next = 0.f;
     auto fetch = [&](uint64_t r) {
         dy_next.load(static_cast<const T*>(a.dy) + r * a.H, t, a.H);
@@ -437,42 +495,43 @@ __global__ void __launch_bounds__(group_threads(W), W <= 8 ? 2 : 1) ln_bwd_row_k
     if (row < a.rows) fetch(row);
     uint32_t flip = 0;
     for (; row < a.rows; row += stride, flip ^= 1) {
-        float g[kCpt], xh[kCpt];
-        dy_next.values(g, t, a.H);
-        x_next.values(xh, t, a.H);
+        float2 g[kPairs], xh[kPairs];
+        dy_next.values(g);
+        x_next.values(xh);
         const float mean = mean_next, rstd = rstd_next;
         if (row + stride < a.rows) fetch(row + stride);
-        float2 s = make_float2(0.f, 0.f);
+        float2 s1 = f2(0.f), s2 = f2(0.f);
 #pragma unroll
-        for (int i = 0; i < kCpt; ++i) {
-            if constexpr (!Ckpt) xh[i] = (xh[i] - mean) * rstd;  // meets g = 0 behind the row's end
-            dgamma[i] = fmaf(g[i], xh[i], dgamma[i]);
-            dbeta[i] += g[i];
-            g[i] *= gamma[i];
-            s.x += g[i];
-            s.y = fmaf(g[i], xh[i], s.y);
+        for (int i = 0; i < kPairs; ++i) {
+            if constexpr (!Ckpt) xh[i] = __fmul2_rn(__fadd2_rn(xh[i], f2(-mean)), f2(rstd));  // meets g = 0 behind the end
+            dgamma[i] = __ffma2_rn(g[i], xh[i], dgamma[i]);
+            dbeta[i] = __fadd2_rn(dbeta[i], g[i]);
+            g[i] = __fmul2_rn(g[i], gamma[i]);
+            s1 = __fadd2_rn(s1, g[i]);
+            s2 = __ffma2_rn(g[i], xh[i], s2);
         }
-        s = row_sum2<W>(s, sh[group][flip], group, wir);
-        const float c1 = s.x * inv_h, c2 = s.y * inv_h;
+        const float2 s = row_sum2<W>(make_float2(s1.x + s1.y, s2.x + s2.y), sh[group][flip], group, wir);
+        const float2 c1 = f2(-s.x * inv_h), c2 = f2(-s.y * inv_h);
 #pragma unroll
-        for (int i = 0; i < kCpt; ++i) g[i] = rstd * (g[i] - c1 - xh[i] * c2);
+        for (int i = 0; i < kPairs; ++i)
+            g[i] = __fmul2_rn(__ffma2_rn(xh[i], c2, __fadd2_rn(g[i], c1)), f2(rstd));
         Row::store(static_cast<T*>(a.dx) + row * a.H, g, t, a.H);
     }
     float* part = a.parts + static_cast<uint64_t>(blockIdx.x) * 2 * a.H;
-    if constexpr (G > 1) {  // columns in thread order: [group][dgamma, dbeta][i][t]
-        float* mine = joined + group * 2 * 32 * W * kCpt;
+    if constexpr (G > 1) {  // [group][dgamma, dbeta][pair][t]
+        float2* mine = joined + group * 2 * 32 * W * kPairs;
 #pragma unroll
-        for (int i = 0; i < kCpt; ++i) {
+        for (int i = 0; i < kPairs; ++i) {
             mine[i * 32 * W + t] = dgamma[i];
-            mine[(kCpt + i) * 32 * W + t] = dbeta[i];
+            mine[(kPairs + i) * 32 * W + t] = dbeta[i];
         }
         __syncthreads();
         if (group != 0) return;
 #pragma unroll
-        for (int i = 0; i < kCpt; ++i)
+        for (int i = 0; i < kPairs; ++i)
             for (int o = 1; o < G; ++o) {
-                dgamma[i] += joined[(o * 2 * kCpt + i) * 32 * W + t];
-                dbeta[i] += joined[((o * 2 + 1) * kCpt + i) * 32 * W + t];
+                dgamma[i] = __fadd2_rn(dgamma[i], joined[(o * 2 * kPairs + i) * 32 * W + t]);
+                dbeta[i] = __fadd2_rn(dbeta[i], joined[((o * 2 + 1) * kPairs + i) * 32 * W + t]);
             }
     }
 #pragma unroll
@@ -480,9 +539,10 @@ __global__ void __launch_bounds__(group_threads(W), W <= 8 ? 2 : 1) ln_bwd_row_k
         const uint32_t c = Row::first(t, i);
         if (c >= a.H) continue;
 #pragma unroll
-        for (int e = 0; e < kCpt / Row::N; ++e) {
-            part[c + e] = dgamma[i * (kCpt / Row::N) + e];
-            part[a.H + c + e] = dbeta[i * (kCpt / Row::N) + e];
+        for (int e = 0; e < Row::kRun; ++e) {
+            const int j = i * Row::kRun + e;
+            part[c + e] = j & 1 ? dgamma[j / 2].y : dgamma[j / 2].x;
+            part[a.H + c + e] = j & 1 ? dbeta[j / 2].y : dbeta[j / 2].x;
         }
     }
 }
