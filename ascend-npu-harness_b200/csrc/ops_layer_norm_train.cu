@@ -168,32 +168,44 @@ __global__ void __launch_bounds__(kThreads) ln_bwd_cols_any_kernel(const BwdArgs
     }
 }
 
-// dgamma and dbeta from the partial rows, always added in the same order.
-__global__ void __launch_bounds__(kThreads) ln_bwd_join_kernel(const float* __restrict__ parts, uint32_t parts_n,
-                                                               uint32_t H, float* __restrict__ dgamma,
-                                                               float* __restrict__ dbeta) {
-    __shared__ float sh[kWarps][32];
+// dgamma and dbeta from the partial rows, always added in the same order: a warp per 32nd partial row, its
+// loads all under way at once.  Launched to start while the kernel before drains.
+constexpr int kJoinWarps = 32;
+__global__ void __launch_bounds__(32 * kJoinWarps) ln_bwd_join_kernel(const float* __restrict__ parts, uint32_t parts_n,
+                                                                      uint32_t H, float* __restrict__ dgamma,
+                                                                      float* __restrict__ dbeta) {
+    __shared__ float sh[kJoinWarps][33];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     const uint32_t c = blockIdx.x * 32 + lane;
+    cudaGridDependencySynchronize();
+    float v[(kMaxParts + kJoinWarps - 1) / kJoinWarps];
+    constexpr int N = sizeof(v) / sizeof(v[0]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint32_t p = warp + i * kJoinWarps;
+        v[i] = c < H && p < parts_n ? __ldcg(parts + (static_cast<uint64_t>(p) * 2 + blockIdx.y) * H + c) : 0.f;
+    }
     float s = 0.f;
-    if (c < H)
-        for (uint32_t p = warp; p < parts_n; p += kWarps)
-            s += parts[(static_cast<uint64_t>(p) * 2 + blockIdx.y) * H + c];
+#pragma unroll
+    for (int i = 0; i < N; ++i) s += v[i];
     sh[warp][lane] = s;
     __syncthreads();
-    if (warp == 0 && c < H) {
-        for (int w = 1; w < kWarps; ++w) s += sh[w][lane];
-        (blockIdx.y ? dbeta : dgamma)[c] = s;
-    }
+    // warp w joins column w of the 32
+    s = warp_sum(sh[lane][warp]);
+    const uint32_t col = blockIdx.x * 32 + warp;
+    if (lane == 0 && col < H) (blockIdx.y ? dbeta : dgamma)[col] = s;
 }
 
 // ---------------------------------------------------------------------------------------
-// Rows of up to 8192 elements: W warps own a row, 16 columns per thread in registers, the next row's
-// loads issued before the current row is worked on.
+// Rows of up to 8192 elements: W warps own a row, 16 columns per thread in registers, the loads of the
+// next row (backward: of the next rows) under way while the current one is worked on.
 //
 // Rows of whole, aligned 16-byte packs (Vec): thread t holds packs t + 32 W j, so 16 (fp32: 32)
-// neighbouring lanes hold a block of 128 and its maximum is a shuffle tree.  Other rows: thread t
-// holds elements t + 32 W i.  Columns behind the row's end hold zeros and are not stored.
+// neighbouring lanes hold a block of 128 and its maximum is a shuffle tree.  In the backward each thread
+// copies its own packs into a ring in shared memory with cp.async and waits for its own copies
+// alone: no barrier and no registers, which the weight gradients need.
+// Other rows: thread t holds elements t + 32 W i, the next row's in registers.
+// Columns behind the row's end hold zeros and are not stored.
 // ---------------------------------------------------------------------------------------
 constexpr int kCpt = 16;
 constexpr uint32_t kMaxFastH = 32 * 16 * kCpt;
@@ -223,12 +235,14 @@ struct RowPart {
 #pragma unroll
         for (int i = 0; i < N; ++i) r[i] = Raw{};
     }
-    __device__ __forceinline__ void load(const T* row, uint32_t t, uint32_t H) {
+    // `mine` points at the thread's first column of the row; column i's distance from it is a constant
+    static constexpr int step(int i) { return 32 * W * i * (Vec ? P : 1); }
+    __device__ __forceinline__ void load(const T* mine, uint32_t t, uint32_t H) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             if (first(t, i) >= H) continue;
-            if constexpr (Vec) r[i] = __ldcs(reinterpret_cast<const uint4*>(row + first(t, i)));
-            else r[i] = row[first(t, i)];
+            if constexpr (Vec) r[i] = __ldcs(reinterpret_cast<const uint4*>(mine + step(i)));
+            else r[i] = mine[step(i)];
         }
     }
     __device__ __forceinline__ void values(float2 (&v)[kPairs]) const {
@@ -251,13 +265,13 @@ struct RowPart {
             }
         }
     }
-    __device__ __forceinline__ static void store(T* row, const float2 (&v)[kPairs], uint32_t t, uint32_t H) {
+    __device__ __forceinline__ static void store(T* mine, const float2 (&v)[kPairs], uint32_t t, uint32_t H) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             if (first(t, i) >= H) continue;
             if constexpr (Vec)
-                st_stream(reinterpret_cast<pack<T>*>(row + first(t, i)), pack_from_f<T>(&v[i * P / 2].x));
-            else row[first(t, i)] = elem<T>::from_f(i & 1 ? v[i / 2].y : v[i / 2].x);
+                st_stream(reinterpret_cast<pack<T>*>(mine + step(i)), pack_from_f<T>(&v[i * P / 2].x));
+            else mine[step(i)] = elem<T>::from_f(i & 1 ? v[i / 2].y : v[i / 2].x);
         }
     }
     // Parameters of the thread's columns (read once per thread; zeros behind the end).
@@ -270,8 +284,16 @@ struct RowPart {
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) v[i] = make_float2(f[2 * i], f[2 * i + 1]);
     }
-    // v -= m in the columns of the row, leaving zeros behind its end; the sum of what `f` makes of each
-    // pair, over the thread's columns.
+    // Zeros in the columns behind the end.
+    __device__ __forceinline__ static void clear_behind(float2 (&v)[kPairs], uint32_t t, uint32_t H) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (first(t, i) < H) continue;
+#pragma unroll
+            for (int e = 0; e < kRun; ++e) ((i * kRun + e) & 1 ? v[(i * kRun + e) / 2].y : v[(i * kRun + e) / 2].x) = 0.f;
+        }
+    }
+    // The sum of what `f` makes of each pair, over the thread's columns of the row; f may change them.
     template <typename F>
     __device__ __forceinline__ static float sum_of(float2 (&v)[kPairs], uint32_t t, uint32_t H, F f) {
         float2 s = f2(0.f);
@@ -294,6 +316,33 @@ struct RowPart {
     }
 };
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+template <int B>
+__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(B) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// The backward's ring of a CTA with `Threads` threads: of one row per thread N packs of dy, and N packs of
+// x or N codes of a pack and their scales; kStages rows, so that `CtasPerSm` rings fit an SM.
+template <typename T, int Threads, int CtasPerSm, bool Ckpt>
+struct RingShape {
+    static constexpr int P = elem<T>::kPack, N = kCpt / P;
+    static constexpr uint32_t kFirst = 16 * N * Threads;
+    static constexpr uint32_t kSecond = Ckpt ? (P + 4) * N * Threads : 16 * N * Threads;
+    static constexpr uint32_t kStage = kFirst + kSecond;
+    static constexpr uint32_t kFit = 192 * 1024 / CtasPerSm / kStage;
+    static constexpr uint32_t kStages = kFit > 6 ? 6 : kFit;
+    static_assert(kStages >= 2, "a ring of one row would not run ahead");
+    static constexpr uint32_t kBytes = kStages * kStage;
+};
+
 // Sums of two values over the W warps of a row, the same bits in every thread.  `sh` alternates
 // between two buffers from call to call: whoever writes one again has passed the barrier that
 // everybody reached after reading it.
@@ -313,61 +362,88 @@ __device__ __forceinline__ float2 row_sum2(float2 v, float2* sh, uint32_t group,
     return s;
 }
 
-template <int W>
-__device__ __forceinline__ float row_sum(float v, float* sh, uint32_t group, uint32_t warp_in_row) {
-    v = warp_sum(v);
-    if (W == 1) return v;
-    if ((threadIdx.x & 31) == 0) sh[warp_in_row] = v;
-    asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * W) : "memory");
-    float s = sh[0];
-#pragma unroll
-    for (int w = 1; w < W; ++w) s += sh[w];
-    return s;
-}
+constexpr int bwd_ctas(int W) { return W <= 8 ? 2 : 1; }
+template <typename T, int W, bool Ckpt>
+using BwdRing = RingShape<T, group_threads(W), bwd_ctas(W), Ckpt>;
 
+// Statistics: each warp takes the mean of its own columns (over deviations from its first one) and its
+// sum of squares around that, with shuffles alone; the row's follow from the W pairs behind one
+// barrier, M2 = sum_w M2_w + n_w (mean_w - mean)^2, which is as exact as two passes over the row.
 template <typename T, int W, bool Vec, bool Ckpt>
-__global__ void __launch_bounds__(group_threads(W)) ln_fwd_row_kernel(const FwdArgs a) {
+__global__ void __launch_bounds__(group_threads(W), W <= 8 ? 3 : 1) ln_fwd_row_kernel(const FwdArgs a) {
     using Row = RowPart<T, W, Vec>;
     constexpr int G = row_groups(W), P = Row::P;
-    __shared__ float sh[G][2][W];
+    __shared__ float2 sh[G][2][W];
     __shared__ alignas(16) uint32_t quarter[Ckpt && !Vec ? G : 1][Ckpt && !Vec ? W * kCpt : 4];
     const uint32_t group = threadIdx.x / (32 * W), t = threadIdx.x % (32 * W), wir = t / 32;
     const uint32_t stride = gridDim.x * G;
-    const float H = static_cast<float>(a.H);
+    const uint64_t step = static_cast<uint64_t>(stride) * a.H;
+    const float inv_h = 1.0f / static_cast<float>(a.H);
     float2 gamma[kPairs], beta[kPairs];
     Row::params(a.gamma, gamma, t, a.H);
     Row::params(a.beta, beta, t, a.H);
+    // columns of each warp of the row, and of this one
+    auto columns_of = [&](uint32_t w) {
+        uint32_t n = 0;
+#pragma unroll
+        for (int i = 0; i < Row::N; ++i) {
+            const uint32_t c = Row::first(32 * w, i), len = 32 * Row::kRun;
+            n += c >= a.H ? 0 : min(len, a.H - c);
+        }
+        return n;
+    };
+    const uint32_t n_mine = columns_of(wir);
+    const float inv_mine = n_mine ? 1.0f / static_cast<float>(n_mine) : 0.f;
     uint64_t row = static_cast<uint64_t>(blockIdx.x) * G + group;
-    const T* x = static_cast<const T*>(a.x);
+    const T* x = static_cast<const T*>(a.x) + row * a.H + Row::first(t, 0);
+    T* y = static_cast<T*>(a.y) + row * a.H + Row::first(t, 0);
     Row next;
     next.clear();
-    float k_next = 0.f;
-    if (row < a.rows) {
-        next.load(x + row * a.H, t, a.H);
-        k_next = elem<T>::to_f(x[row * a.H]);
-    }
-    for (; row < a.rows; row += stride) {
+    if (row < a.rows) next.load(x, t, a.H);
+    uint32_t flip = 0;
+    for (; row < a.rows; row += stride, y += step, flip ^= 1) {
         float2 v[kPairs];
         next.values(v);
-        const float K = k_next;
-        if (row + stride < a.rows) {
-            next.load(x + (row + stride) * a.H, t, a.H);
-            k_next = elem<T>::to_f(x[(row + stride) * a.H]);
-        }
-        float s = Row::sum_of(v, t, a.H, [&](float2& p, float2 s) { return __fadd2_rn(s, __fadd2_rn(p, f2(-K))); });
-        const float mean = K + __fdiv_rn(row_sum<W>(s, sh[group][0], group, wir), H);
+        x += step;
+        if (row + stride < a.rows) next.load(x, t, a.H);
+        const float K = __shfl_sync(0xffffffffu, v[0].x, 0);  // lane 0 holds the warp's first column
+        float s = Row::sum_of(v, t, a.H, [&](float2& p, float2 s) {
+            p = __fadd2_rn(p, f2(-K));
+            return __fadd2_rn(s, p);
+        });
+        const float shift = warp_sum(s) * inv_mine;  // the warp's mean is K + shift
         s = Row::sum_of(v, t, a.H, [&](float2& p, float2 s) {
-            p = __fadd2_rn(p, f2(-mean));
+            p = __fadd2_rn(p, f2(-shift));
             return __ffma2_rn(p, p, s);
         });
-        const float var = __fdiv_rn(row_sum<W>(s, sh[group][1], group, wir), H);
-        const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(var + a.eps));
+        float m2 = warp_sum(s), mean = K + shift, off = 0.f;  // v holds deviations from the warp's mean
+        if constexpr (W > 1) {
+            if (t % 32 == 0) sh[group][flip][wir] = make_float2(mean, m2);
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * W) : "memory");
+            float2 w[W];
+#pragma unroll
+            for (int i = 0; i < W; ++i) w[i] = sh[group][flip][i];
+            const float own = mean;
+            float d = 0.f;
+#pragma unroll
+            for (int i = 1; i < W; ++i) d = fmaf(static_cast<float>(columns_of(i)), w[i].x - w[0].x, d);
+            mean = fmaf(d, inv_h, w[0].x);
+            m2 = 0.f;
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const float e = w[i].x - mean;
+                m2 += fmaf(static_cast<float>(columns_of(i)) * e, e, w[i].y);
+            }
+            off = own - mean;
+        }
+        const float rstd = rsqrtf(fmaf(m2, inv_h, a.eps));
         if (t == 0) {
             if (a.mean) a.mean[row] = mean;
             a.rstd[row] = rstd;
         }
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) v[i] = __fmul2_rn(v[i], f2(rstd));
+        for (int i = 0; i < kPairs; ++i) v[i] = __fmul2_rn(__fadd2_rn(v[i], f2(off)), f2(rstd));
+        Row::clear_behind(v, t, a.H);
         if constexpr (Ckpt && Vec) {
 #pragma unroll
             for (int i = 0; i < Row::N; ++i) {
@@ -419,11 +495,11 @@ __global__ void __launch_bounds__(group_threads(W)) ln_fwd_row_kernel(const FwdA
         }
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) v[i] = __ffma2_rn(v[i], gamma[i], beta[i]);
-        Row::store(static_cast<T*>(a.y) + row * a.H, v, t, a.H);
+        Row::store(y, v, t, a.H);
     }
 }
 
-// A thread's 16 columns of xh from the checkpoint: codes and scales, loaded like RowPart.
+// A thread's 16 columns of xh from the checkpoint: codes and scales (load: rows without a ring).
 template <int W, bool Vec, int P>
 struct CkptPart {
     static constexpr int N = Vec ? kCpt / P : kCpt;
@@ -438,14 +514,9 @@ struct CkptPart {
     __device__ __forceinline__ void load(const uint8_t* q, const float* scale, uint32_t t, uint32_t H) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const uint32_t c = Vec ? (t + 32 * W * i) * P : t + 32 * W * i;
+            const uint32_t c = t + 32 * W * i;
             if (c >= H) continue;
-            if constexpr (!Vec) code[i] = q[c];
-            else if constexpr (P == 8) {
-                const uint2 v = __ldcs(reinterpret_cast<const uint2*>(q + c));
-                code[2 * i] = v.x;
-                code[2 * i + 1] = v.y;
-            } else code[i] = __ldcs(reinterpret_cast<const uint32_t*>(q + c));
+            code[i] = q[c];
             s[i] = __ldg(scale + c / kFp8Block);
         }
     }
@@ -463,12 +534,13 @@ struct CkptPart {
 // dx of every row, and this CTA's sums over its rows of dy xh and dy: 16 columns per thread in
 // registers over all its rows, joined over the CTA's row groups at the end.
 template <typename T, int W, bool Vec, bool Ckpt>
-__global__ void __launch_bounds__(group_threads(W), W <= 8 ? 2 : 1) ln_bwd_row_kernel(const BwdArgs a) {
+__global__ void __launch_bounds__(group_threads(W), bwd_ctas(W)) ln_bwd_row_kernel(const BwdArgs a) {
     using Row = RowPart<T, W, Vec>;
     using Part = typename std::conditional<Ckpt, CkptPart<W, Vec, Row::P>, Row>::type;
-    constexpr int G = row_groups(W);
+    using Ring = BwdRing<T, W, Ckpt>;
+    constexpr int G = row_groups(W), Threads = group_threads(W), P = Row::P;
+    extern __shared__ __align__(16) uint8_t dyn[];  // the ring, and after it the sums of the row groups
     __shared__ float2 sh[G][2][W];
-    __shared__ float2 joined[G > 1 ? G * 2 * 32 * W * kPairs : 1];
     const uint32_t group = threadIdx.x / (32 * W), t = threadIdx.x % (32 * W), wir = t / 32;
     const uint32_t stride = gridDim.x * G;
     const float inv_h = 1.0f / static_cast<float>(a.H);
@@ -481,24 +553,92 @@ __global__ void __launch_bounds__(group_threads(W), W <= 8 ? 2 : 1) ln_bwd_row_k
     Part x_next;
     dy_next.clear();
     x_next.clear();
-    float mean_next = 0.f, rstd_next = 0.f;
-    auto fetch = [&](uint64_t r) {
-        dy_next.load(static_cast<const T*>(a.dy) + r * a.H, t, a.H);
-        if constexpr (Ckpt) {
-            x_next.load(a.q + r * a.H, a.scale + r * a.row_blocks, t, a.H);
-        } else {
-            x_next.load(static_cast<const T*>(a.x) + r * a.H, t, a.H);
-            mean_next = __ldg(a.mean + r);
+    // the ring, stage by stage: dy packs [N][Threads], then x packs [N][Threads], or codes [N][Threads] of P
+    // bytes and scales [N][Threads]
+    auto dy_slot = [&](uint32_t s, int i) { return reinterpret_cast<uint4*>(dyn + s * Ring::kStage) + i * Threads + threadIdx.x; };
+    auto x_slot = [&](uint32_t s, int i) {
+        return dyn + s * Ring::kStage + Ring::kFirst + (i * Threads + threadIdx.x) * (Ckpt ? P : 16);
+    };
+    auto s_slot = [&](uint32_t s, int i) {
+        return reinterpret_cast<float*>(dyn + s * Ring::kStage + Ring::kFirst + P * Row::N * Threads) + i * Threads + threadIdx.x;
+    };
+    auto smem_at = [](const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); };
+    // the row that is copied next, and where the thread's first column of it lies
+    uint64_t ahead = row, at = row * a.H + Row::first(t, 0), at_block = row * a.row_blocks;
+    const uint64_t step = static_cast<uint64_t>(stride) * a.H;
+    auto copy = [&](uint32_t s) {
+        if (ahead < a.rows) {
+#pragma unroll
+            for (int i = 0; i < Row::N; ++i) {
+                const uint32_t c = Row::first(t, i);
+                if (c >= a.H) continue;
+                cp_async16(smem_at(dy_slot(s, i)), static_cast<const T*>(a.dy) + at + Row::step(i));
+                if constexpr (Ckpt) {
+                    cp_async_small<P>(smem_at(x_slot(s, i)), a.q + at + Row::step(i));
+                    cp_async_small<4>(smem_at(s_slot(s, i)), a.scale + at_block + c / kFp8Block);
+                } else {
+                    cp_async16(smem_at(x_slot(s, i)), static_cast<const T*>(a.x) + at + Row::step(i));
+                }
+            }
         }
+        cp_async_commit();
+        ahead += stride;
+        at += step;
+        at_block += static_cast<uint64_t>(stride) * a.row_blocks;
+    };
+    float mean_next = 0.f, rstd_next = 0.f;
+    auto fetch = [&](uint64_t r) {  // statistics, and without a ring the row
+        if constexpr (!Vec) {
+            dy_next.load(static_cast<const T*>(a.dy) + r * a.H + Row::first(t, 0), t, a.H);
+            if constexpr (Ckpt) x_next.load(a.q + r * a.H, a.scale + r * a.row_blocks, t, a.H);
+            else x_next.load(static_cast<const T*>(a.x) + r * a.H + Row::first(t, 0), t, a.H);
+        }
+        if constexpr (!Ckpt) mean_next = __ldg(a.mean + r);
         rstd_next = __ldg(a.rstd + r);
     };
+    uint32_t stage = 0;
+    if constexpr (Vec) {
+        // columns behind the end: zeros that no copy overwrites (their codes and x stay zero in registers)
+        for (uint32_t s = 0; s < Ring::kStages; ++s)
+#pragma unroll
+            for (int i = 0; i < Row::N; ++i)
+                if (Row::first(t, i) >= a.H) *dy_slot(s, i) = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (uint32_t s = 0; s + 1 < Ring::kStages; ++s) copy(s);
+    }
     if (row < a.rows) fetch(row);
+    T* dx = static_cast<T*>(a.dx) + row * a.H + Row::first(t, 0);
     uint32_t flip = 0;
-    for (; row < a.rows; row += stride, flip ^= 1) {
+    for (; row < a.rows; row += stride, flip ^= 1, dx += step) {
         float2 g[kPairs], xh[kPairs];
+        if constexpr (Vec) {
+            cp_async_wait<Ring::kStages - 2>();
+#pragma unroll
+            for (int i = 0; i < Row::N; ++i) {
+                dy_next.r[i] = *dy_slot(stage, i);
+                if (Row::first(t, i) >= a.H) continue;
+                if constexpr (!Ckpt) {
+                    x_next.r[i] = *reinterpret_cast<const uint4*>(x_slot(stage, i));
+                } else {
+                    if constexpr (P == 8) {
+                        const uint2 v = *reinterpret_cast<const uint2*>(x_slot(stage, i));
+                        x_next.code[2 * i] = v.x;
+                        x_next.code[2 * i + 1] = v.y;
+                    } else {
+                        x_next.code[i] = *reinterpret_cast<const uint32_t*>(x_slot(stage, i));
+                    }
+                    x_next.s[i] = *s_slot(stage, i);
+                }
+            }
+        }
         dy_next.values(g);
         x_next.values(xh);
         const float mean = mean_next, rstd = rstd_next;
+        if constexpr (Vec) {
+            const uint32_t free = stage == 0 ? Ring::kStages - 1 : stage - 1;  // the row before, read by now
+            copy(free);
+            stage = stage + 1 == Ring::kStages ? 0 : stage + 1;
+        }
         if (row + stride < a.rows) fetch(row + stride);
         float2 s1 = f2(0.f), s2 = f2(0.f);
 #pragma unroll
@@ -515,10 +655,16 @@ __global__ void __launch_bounds__(group_threads(W), W <= 8 ? 2 : 1) ln_bwd_row_k
 #pragma unroll
         for (int i = 0; i < kPairs; ++i)
             g[i] = __fmul2_rn(__ffma2_rn(xh[i], c2, __fadd2_rn(g[i], c1)), f2(rstd));
-        Row::store(static_cast<T*>(a.dx) + row * a.H, g, t, a.H);
+        Row::store(dx, g, t, a.H);
     }
+    cudaTriggerProgrammaticLaunchCompletion();  // the join may be set up now; it waits for the sums
     float* part = a.parts + static_cast<uint64_t>(blockIdx.x) * 2 * a.H;
     if constexpr (G > 1) {  // [group][dgamma, dbeta][pair][t]
+        if constexpr (Vec) {
+            cp_async_wait<0>();
+            __syncthreads();  // the sums overwrite the ring
+        }
+        float2* joined = reinterpret_cast<float2*>(dyn);
         float2* mine = joined + group * 2 * 32 * W * kPairs;
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
@@ -599,7 +745,12 @@ int launch_bwd_rows(BwdArgs& a, cudaStream_t s) {
         constexpr int W = decltype(w)::value;
         const uint32_t groups = (a.rows + row_groups(W) - 1) / row_groups(W);
         a.parts_n = parts_of(groups);  // one per CTA
-        ln_bwd_row_kernel<T, W, Vec, Ckpt><<<a.parts_n, group_threads(W), 0, s>>>(a);
+        // the ring, or the joined sums of the row groups: 2 x 16 columns of each thread
+        constexpr size_t sums = row_groups(W) > 1 ? size_t(group_threads(W)) * 2 * kCpt * 4 : 0;
+        constexpr size_t ring = Vec ? BwdRing<T, W, Ckpt>::kBytes : 0, smem = ring > sums ? ring : sums;
+        auto* k = ln_bwd_row_kernel<T, W, Vec, Ckpt>;
+        if (int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(k), smem, "ln_bwd_row_kernel")) return rc;
+        k<<<a.parts_n, group_threads(W), smem, s>>>(a);
         return check_launch("layer_norm_bwd");
     });
 }
@@ -619,7 +770,16 @@ int launch_bwd(BwdArgs a, float* dgamma, float* dbeta, cudaStream_t s) {
         ln_bwd_cols_any_kernel<T, Ckpt><<<dim3((a.H + 31) / 32, a.parts_n), kThreads, 0, s>>>(a);
         if (int rc = check_launch("layer_norm_bwd")) return rc;
     }
-    ln_bwd_join_kernel<<<dim3((a.H + 31) / 32, 2), kThreads, 0, s>>>(a.parts, a.parts_n, a.H, dgamma, dbeta);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((a.H + 31) / 32, 2);
+    cfg.blockDim = dim3(32 * kJoinWarps);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, ln_bwd_join_kernel, const_cast<const float*>(a.parts), a.parts_n, a.H, dgamma, dbeta);
     return check_launch("layer_norm_bwd");
 }
 
