@@ -353,18 +353,26 @@ __device__ __forceinline__ float2 row_sum2(float2 v, float2* sh, uint32_t group,
     if (W == 1) return v;
     if ((threadIdx.x & 31) == 0) sh[warp_in_row] = v;
     asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * W) : "memory");
-    float2 s = sh[0];
+    v = sh[threadIdx.x % W];  // every run of W lanes adds up all warps
 #pragma unroll
-    for (int w = 1; w < W; ++w) {
-        s.x += sh[w].x;
-        s.y += sh[w].y;
+    for (int o = W / 2; o > 0; o >>= 1) {
+        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+        v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
     }
-    return s;
+    return v;
 }
 
 constexpr int bwd_ctas(int W) { return W <= 8 ? 2 : 1; }
 template <typename T, int W, bool Ckpt>
 using BwdRing = RingShape<T, group_threads(W), bwd_ctas(W), Ckpt>;
+
+// Sum over each run of W lanes.
+template <int W>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
 
 // Statistics: each warp takes the mean of its own columns (over deviations from its first one) and its
 // sum of squares around that, with shuffles alone; the row's follow from the W pairs behind one
@@ -382,7 +390,7 @@ __global__ void __launch_bounds__(group_threads(W), W <= 8 ? 3 : 1) ln_fwd_row_k
     float2 gamma[kPairs], beta[kPairs];
     Row::params(a.gamma, gamma, t, a.H);
     Row::params(a.beta, beta, t, a.H);
-    // columns of each warp of the row, and of this one
+    // columns of warp w of the row
     auto columns_of = [&](uint32_t w) {
         uint32_t n = 0;
 #pragma unroll
@@ -394,6 +402,7 @@ __global__ void __launch_bounds__(group_threads(W), W <= 8 ? 3 : 1) ln_fwd_row_k
     };
     const uint32_t n_mine = columns_of(wir);
     const float inv_mine = n_mine ? 1.0f / static_cast<float>(n_mine) : 0.f;
+    const float n_lane = static_cast<float>(columns_of(t % W));
     uint64_t row = static_cast<uint64_t>(blockIdx.x) * G + group;
     const T* x = static_cast<const T*>(a.x) + row * a.H + Row::first(t, 0);
     T* y = static_cast<T*>(a.y) + row * a.H + Row::first(t, 0);
@@ -420,20 +429,12 @@ __global__ void __launch_bounds__(group_threads(W), W <= 8 ? 3 : 1) ln_fwd_row_k
         if constexpr (W > 1) {
             if (t % 32 == 0) sh[group][flip][wir] = make_float2(mean, m2);
             asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * W) : "memory");
-            float2 w[W];
-#pragma unroll
-            for (int i = 0; i < W; ++i) w[i] = sh[group][flip][i];
-            const float own = mean;
-            float d = 0.f;
-#pragma unroll
-            for (int i = 1; i < W; ++i) d = fmaf(static_cast<float>(columns_of(i)), w[i].x - w[0].x, d);
-            mean = fmaf(d, inv_h, w[0].x);
-            m2 = 0.f;
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-                const float e = w[i].x - mean;
-                m2 += fmaf(static_cast<float>(columns_of(i)) * e, e, w[i].y);
-            }
+            // every run of W lanes joins all warps, one each
+            const float2 w = sh[group][flip][t % W];
+            const float own = mean, base = __shfl_sync(0xffffffffu, w.x, 0);
+            mean = fmaf(lanes_sum<W>(n_lane * (w.x - base)), inv_h, base);
+            const float e = w.x - mean;
+            m2 = lanes_sum<W>(fmaf(n_lane * e, e, w.y));
             off = own - mean;
         }
         const float rstd = rsqrtf(fmaf(m2, inv_h, a.eps));
@@ -555,29 +556,26 @@ __global__ void __launch_bounds__(group_threads(W), bwd_ctas(W)) ln_bwd_row_kern
     x_next.clear();
     // the ring, stage by stage: dy packs [N][Threads], then x packs [N][Threads], or codes [N][Threads] of P
     // bytes and scales [N][Threads]
-    auto dy_slot = [&](uint32_t s, int i) { return reinterpret_cast<uint4*>(dyn + s * Ring::kStage) + i * Threads + threadIdx.x; };
-    auto x_slot = [&](uint32_t s, int i) {
-        return dyn + s * Ring::kStage + Ring::kFirst + (i * Threads + threadIdx.x) * (Ckpt ? P : 16);
-    };
-    auto s_slot = [&](uint32_t s, int i) {
-        return reinterpret_cast<float*>(dyn + s * Ring::kStage + Ring::kFirst + P * Row::N * Threads) + i * Threads + threadIdx.x;
-    };
+    uint8_t* const dy_base = dyn + threadIdx.x * 16;
+    uint8_t* const x_base = dyn + Ring::kFirst + threadIdx.x * (Ckpt ? P : 16);
+    uint8_t* const s_base = dyn + Ring::kFirst + P * Row::N * Threads + threadIdx.x * 4;
+    constexpr int kXStep = Threads * (Ckpt ? P : 16);
     auto smem_at = [](const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); };
     // the row that is copied next, and where the thread's first column of it lies
     uint64_t ahead = row, at = row * a.H + Row::first(t, 0), at_block = row * a.row_blocks;
     const uint64_t step = static_cast<uint64_t>(stride) * a.H;
-    auto copy = [&](uint32_t s) {
+    auto copy = [&](uint32_t at_stage) {  // byte offset of a stage
         if (ahead < a.rows) {
 #pragma unroll
             for (int i = 0; i < Row::N; ++i) {
                 const uint32_t c = Row::first(t, i);
                 if (c >= a.H) continue;
-                cp_async16(smem_at(dy_slot(s, i)), static_cast<const T*>(a.dy) + at + Row::step(i));
+                cp_async16(smem_at(dy_base + at_stage + i * Threads * 16), static_cast<const T*>(a.dy) + at + Row::step(i));
                 if constexpr (Ckpt) {
-                    cp_async_small<P>(smem_at(x_slot(s, i)), a.q + at + Row::step(i));
-                    cp_async_small<4>(smem_at(s_slot(s, i)), a.scale + at_block + c / kFp8Block);
+                    cp_async_small<P>(smem_at(x_base + at_stage + i * kXStep), a.q + at + Row::step(i));
+                    cp_async_small<4>(smem_at(s_base + at_stage + i * Threads * 4), a.scale + at_block + c / kFp8Block);
                 } else {
-                    cp_async16(smem_at(x_slot(s, i)), static_cast<const T*>(a.x) + at + Row::step(i));
+                    cp_async16(smem_at(x_base + at_stage + i * kXStep), static_cast<const T*>(a.x) + at + Row::step(i));
                 }
             }
         }
@@ -596,15 +594,16 @@ __global__ void __launch_bounds__(group_threads(W), bwd_ctas(W)) ln_bwd_row_kern
         if constexpr (!Ckpt) mean_next = __ldg(a.mean + r);
         rstd_next = __ldg(a.rstd + r);
     };
-    uint32_t stage = 0;
+    uint32_t stage = 0;  // byte offset of the current row's stage
     if constexpr (Vec) {
         // columns behind the end: zeros that no copy overwrites (their codes and x stay zero in registers)
         for (uint32_t s = 0; s < Ring::kStages; ++s)
 #pragma unroll
             for (int i = 0; i < Row::N; ++i)
-                if (Row::first(t, i) >= a.H) *dy_slot(s, i) = make_uint4(0, 0, 0, 0);
+                if (Row::first(t, i) >= a.H)
+                    *reinterpret_cast<uint4*>(dy_base + s * Ring::kStage + i * Threads * 16) = make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (uint32_t s = 0; s + 1 < Ring::kStages; ++s) copy(s);
+        for (uint32_t s = 0; s + 1 < Ring::kStages; ++s) copy(s * Ring::kStage);
     }
     if (row < a.rows) fetch(row);
     T* dx = static_cast<T*>(a.dx) + row * a.H + Row::first(t, 0);
@@ -615,19 +614,19 @@ __global__ void __launch_bounds__(group_threads(W), bwd_ctas(W)) ln_bwd_row_kern
             cp_async_wait<Ring::kStages - 2>();
 #pragma unroll
             for (int i = 0; i < Row::N; ++i) {
-                dy_next.r[i] = *dy_slot(stage, i);
+                dy_next.r[i] = *reinterpret_cast<const uint4*>(dy_base + stage + i * Threads * 16);
                 if (Row::first(t, i) >= a.H) continue;
                 if constexpr (!Ckpt) {
-                    x_next.r[i] = *reinterpret_cast<const uint4*>(x_slot(stage, i));
+                    x_next.r[i] = *reinterpret_cast<const uint4*>(x_base + stage + i * kXStep);
                 } else {
                     if constexpr (P == 8) {
-                        const uint2 v = *reinterpret_cast<const uint2*>(x_slot(stage, i));
+                        const uint2 v = *reinterpret_cast<const uint2*>(x_base + stage + i * kXStep);
                         x_next.code[2 * i] = v.x;
                         x_next.code[2 * i + 1] = v.y;
                     } else {
-                        x_next.code[i] = *reinterpret_cast<const uint32_t*>(x_slot(stage, i));
+                        x_next.code[i] = *reinterpret_cast<const uint32_t*>(x_base + stage + i * kXStep);
                     }
-                    x_next.s[i] = *s_slot(stage, i);
+                    x_next.s[i] = *reinterpret_cast<const float*>(s_base + stage + i * Threads * 4);
                 }
             }
         }
@@ -635,9 +634,9 @@ __global__ void __launch_bounds__(group_threads(W), bwd_ctas(W)) ln_bwd_row_kern
         x_next.values(xh);
         const float mean = mean_next, rstd = rstd_next;
         if constexpr (Vec) {
-            const uint32_t free = stage == 0 ? Ring::kStages - 1 : stage - 1;  // the row before, read by now
-            copy(free);
-            stage = stage + 1 == Ring::kStages ? 0 : stage + 1;
+            constexpr uint32_t kLast = Ring::kBytes - Ring::kStage;
+            copy(stage == 0 ? kLast : stage - Ring::kStage);  // over the row before, read by now
+            stage = stage == kLast ? 0 : stage + Ring::kStage;
         }
         if (row + stride < a.rows) fetch(row + stride);
         float2 s1 = f2(0.f), s2 = f2(0.f);
