@@ -35,6 +35,8 @@
 // Function), since a Python formula would cost more host time than the kernels take on small rows.
 // Load with torch.ops.load_library("ascend-npu-harness_b200/lib/libhc_torch.so").
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -315,6 +317,12 @@ std::vector<int64_t> fp8_scale_shape(at::IntArrayRef x, int64_t block_rows) {
     return s;
 }
 
+// A dense CUDA output next to `x`, without the trip through the dispatcher: a layer norm's seven outputs
+// and buffers cost more host time that way than its kernels take on a few rows.
+at::Tensor cuda_empty(at::IntArrayRef shape, at::ScalarType type, const at::Tensor& x) {
+    return at::detail::empty_cuda(shape, type, x.device(), std::nullopt);
+}
+
 std::pair<at::Tensor, at::Tensor> fp8_outputs(const at::Tensor& x, int64_t block_rows) {
     return {at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn)),
             at::empty(fp8_scale_shape(x.sizes(), block_rows), x.options().dtype(at::kFloat))};
@@ -326,7 +334,8 @@ uint32_t cols_of(const at::Tensor& x) { return u32(x.size(-1), "cols"); }
 std::tuple<at::Tensor, at::Tensor> quantize_fp8_block_cuda(const at::Tensor& x, int64_t block_rows) {
     check_input(x, "x");
     c10::cuda::CUDAGuard guard(x.device());
-    auto [q, scale] = fp8_outputs(x, block_rows);
+    at::Tensor q = cuda_empty(x.sizes(), at::kFloat8_e4m3fn, x);
+    at::Tensor scale = cuda_empty(fp8_scale_shape(x.sizes(), block_rows), at::kFloat, x);
     fp8_block_tiling_data t{rows_of(x), cols_of(x), u32(block_rows, "block_rows")};
     ok_or_throw(hc_quantize_fp8_block_launch(x.data_ptr(), q.data_ptr(), scale.data_ptr<float>(), &t, dtype_code(x),
                                              stream_of(x)),
@@ -339,7 +348,7 @@ at::Tensor dequantize_fp8_block_cuda(const at::Tensor& q, const at::Tensor& scal
     check_arg(q, "q", at::kFloat8_e4m3fn, q.sizes(), q);
     check_arg(scale, "scale", at::kFloat, fp8_scale_shape(q.sizes(), block_rows), q);
     c10::cuda::CUDAGuard guard(q.device());
-    at::Tensor x = at::empty(q.sizes(), q.options().dtype(dtype));
+    at::Tensor x = cuda_empty(q.sizes(), dtype, q);
     fp8_block_tiling_data t{rows_of(q), cols_of(q), u32(block_rows, "block_rows")};
     ok_or_throw(hc_dequantize_fp8_block_launch(q.data_ptr(), scale.data_ptr<float>(), x.data_ptr(), &t, dtype_code(x),
                                                stream_of(q)),
@@ -356,7 +365,7 @@ at::Tensor matmul_fp8_block_cuda(const at::Tensor& a, const at::Tensor& a_scale,
     check_arg(b_scale, "b_scale", at::kFloat, fp8_scale_shape(b.sizes(), kFp8BlockSize), a);
     if (bias) check_arg(*bias, "bias", dtype, {b.size(0)}, a);
     c10::cuda::CUDAGuard guard(a.device());
-    at::Tensor c = at::empty({a.size(0), b.size(0)}, a.options().dtype(dtype));
+    at::Tensor c = cuda_empty({a.size(0), b.size(0)}, dtype, a);
     matmul_fp8_block_tiling_data t{u32(a.size(0), "M"), u32(a.size(1), "K"), u32(b.size(0), "N")};
     ok_or_throw(hc_matmul_fp8_block_launch(a.data_ptr(), a_scale.data_ptr<float>(), b.data_ptr(), b_scale.data_ptr<float>(),
                                            bias ? bias->data_ptr() : nullptr, c.data_ptr(), &t, dtype_code(c), stream_of(a)),
@@ -367,8 +376,9 @@ at::Tensor matmul_fp8_block_cuda(const at::Tensor& a, const at::Tensor& a_scale,
 std::tuple<at::Tensor, at::Tensor, at::Tensor> activation_gelu_silu_ckpt_cuda(const at::Tensor& x, int64_t act) {
     check_input(x, "x");
     c10::cuda::CUDAGuard guard(x.device());
-    auto [q, scale] = fp8_outputs(x, 1);
-    at::Tensor y = at::empty_like(x);
+    at::Tensor q = cuda_empty(x.sizes(), at::kFloat8_e4m3fn, x);
+    at::Tensor scale = cuda_empty(fp8_scale_shape(x.sizes(), 1), at::kFloat, x);
+    at::Tensor y = cuda_empty(x.sizes(), x.scalar_type(), x);
     activation_gelu_silu_ckpt_tiling_data t{rows_of(x), cols_of(x), u32(act, "act")};
     ok_or_throw(hc_activation_gelu_silu_ckpt_launch(x.data_ptr(), y.data_ptr(), q.data_ptr(), scale.data_ptr<float>(), &t,
                                                     dtype_code(x), stream_of(x)),
@@ -382,7 +392,7 @@ at::Tensor activation_gelu_silu_ckpt_bwd_cuda(const at::Tensor& dy, const at::Te
     check_arg(q, "q", at::kFloat8_e4m3fn, dy.sizes(), dy);
     check_arg(scale, "scale", at::kFloat, fp8_scale_shape(dy.sizes(), 1), dy);
     c10::cuda::CUDAGuard guard(dy.device());
-    at::Tensor dx = at::empty_like(dy);
+    at::Tensor dx = cuda_empty(dy.sizes(), dy.scalar_type(), dy);
     activation_gelu_silu_ckpt_tiling_data t{rows_of(dy), cols_of(dy), u32(act, "act")};
     ok_or_throw(hc_activation_gelu_silu_ckpt_bwd_launch(dy.data_ptr(), q.data_ptr(), scale.data_ptr<float>(), dx.data_ptr(),
                                                         &t, dtype_code(dy), stream_of(dy)),
@@ -405,9 +415,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_fwd_train_cuda(const a
     check_ln(x, gamma, "gamma");
     check_ln(x, beta, "beta");
     c10::cuda::CUDAGuard guard(x.device());
-    at::Tensor y = at::empty_like(x);
-    at::Tensor mean = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
-    at::Tensor rstd = at::empty_like(mean);
+    at::Tensor y = cuda_empty(x.sizes(), x.scalar_type(), x);
+    at::Tensor mean = cuda_empty(x.sizes().slice(0, x.dim() - 1), at::kFloat, x);
+    at::Tensor rstd = cuda_empty(mean.sizes(), at::kFloat, x);
     const layer_norm_tiling_data t = ln_tiling(x, eps);
     ok_or_throw(hc_layer_norm_fwd_train_launch(x.data_ptr(), gamma.data_ptr<float>(), beta.data_ptr<float>(), y.data_ptr(),
                                                mean.data_ptr<float>(), rstd.data_ptr<float>(), nullptr, nullptr, &t,
@@ -422,9 +432,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> layer_norm_ckpt_cuda(
     check_ln(x, gamma, "gamma");
     check_ln(x, beta, "beta");
     c10::cuda::CUDAGuard guard(x.device());
-    auto [q, scale] = fp8_outputs(x, 1);
-    at::Tensor y = at::empty_like(x);
-    at::Tensor rstd = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+    at::Tensor q = cuda_empty(x.sizes(), at::kFloat8_e4m3fn, x);
+    at::Tensor scale = cuda_empty(fp8_scale_shape(x.sizes(), 1), at::kFloat, x);
+    at::Tensor y = cuda_empty(x.sizes(), x.scalar_type(), x);
+    at::Tensor rstd = cuda_empty(x.sizes().slice(0, x.dim() - 1), at::kFloat, x);
     const layer_norm_tiling_data t = ln_tiling(x, eps);
     ok_or_throw(hc_layer_norm_fwd_train_launch(x.data_ptr(), gamma.data_ptr<float>(), beta.data_ptr<float>(), y.data_ptr(),
                                                nullptr, rstd.data_ptr<float>(), q.data_ptr(), scale.data_ptr<float>(), &t,
@@ -435,15 +446,16 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> layer_norm_ckpt_cuda(
 
 // Outputs and workspace of a layer norm backward, allocated on the current stream.
 struct LnGrads {
-    at::Tensor dx, dgamma, dbeta, work;
+    at::Tensor dx, dgamma, dbeta;
+    c10::DataPtr work;
+    size_t bytes = 0;
     layer_norm_tiling_data t;
     LnGrads(const at::Tensor& dy, const at::Tensor& gamma) : t(ln_tiling(dy, 0.0)) {
-        size_t bytes = 0;
         ok_or_throw(hc_layer_norm_bwd_workspace_size(&t, dtype_code(dy), &bytes), "layer_norm_bwd");
-        dx = at::empty_like(dy);
-        dgamma = at::empty_like(gamma);
-        dbeta = at::empty_like(gamma);
-        work = at::empty({static_cast<int64_t>(bytes)}, dy.options().dtype(at::kByte));
+        dx = cuda_empty(dy.sizes(), dy.scalar_type(), dy);
+        dgamma = cuda_empty(gamma.sizes(), at::kFloat, dy);
+        dbeta = cuda_empty(gamma.sizes(), at::kFloat, dy);
+        work = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);  // of the current device and stream
     }
 };
 
@@ -459,7 +471,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_bwd_cuda(const at::Ten
     LnGrads g(dy, gamma);
     ok_or_throw(hc_layer_norm_bwd_launch(dy.data_ptr(), x.data_ptr(), gamma.data_ptr<float>(), mean.data_ptr<float>(),
                                          rstd.data_ptr<float>(), g.dx.data_ptr(), g.dgamma.data_ptr<float>(),
-                                         g.dbeta.data_ptr<float>(), g.work.data_ptr(), g.work.numel(), &g.t,
+                                         g.dbeta.data_ptr<float>(), g.work.get(), g.bytes, &g.t,
                                          dtype_code(dy), stream_of(dy)),
                 "layer_norm_bwd");
     return {g.dx, g.dgamma, g.dbeta};
@@ -477,7 +489,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_ckpt_bwd_cuda(const at
     LnGrads g(dy, gamma);
     ok_or_throw(hc_layer_norm_ckpt_bwd_launch(dy.data_ptr(), q.data_ptr(), scale.data_ptr<float>(), gamma.data_ptr<float>(),
                                               rstd.data_ptr<float>(), g.dx.data_ptr(), g.dgamma.data_ptr<float>(),
-                                              g.dbeta.data_ptr<float>(), g.work.data_ptr(), g.work.numel(), &g.t,
+                                              g.dbeta.data_ptr<float>(), g.work.get(), g.bytes, &g.t,
                                               dtype_code(dy), stream_of(dy)),
                 "layer_norm_ckpt_bwd");
     return {g.dx, g.dgamma, g.dbeta};
@@ -498,18 +510,29 @@ c10::TypedOperatorHandle<F> op_handle(const char* name) {
     return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").template typed<F>();
 }
 
-// The ops below their autograd layer.
+// A CUDA tensor that no mode, functional transform or subclass wants to see dispatched.
+bool plain_cuda(TensorRef x) {
+    constexpr c10::DispatchKeySet usual({c10::DispatchKey::CUDA, c10::DispatchKey::AutogradCUDA,
+                                         c10::DispatchKey::ADInplaceOrView, c10::DispatchKey::AutocastCUDA});
+    const c10::impl::LocalDispatchKeySet local = c10::impl::tls_local_dispatch_key_set();
+    return (((x.key_set() | local.included_) - local.excluded_) - usual).empty() && x.is_cuda();
+}
+
+// The ops below their autograd layer (CUDA tensors: straight to the kernel's wrapper).
 Tensors3 ln_fwd_train_below(TensorRef x, TensorRef gamma, TensorRef beta, double eps) {
+    if (plain_cuda(x)) return layer_norm_fwd_train_cuda(x, gamma, beta, eps);
     static const auto op = op_handle<Tensors3(TensorRef, TensorRef, TensorRef, double)>("hc::layer_norm_fwd_train");
     at::AutoDispatchBelowADInplaceOrView guard;
     return op.call(x, gamma, beta, eps);
 }
 Tensors4 ln_ckpt_below(TensorRef x, TensorRef gamma, TensorRef beta, double eps) {
+    if (plain_cuda(x)) return layer_norm_ckpt_cuda(x, gamma, beta, eps);
     static const auto op = op_handle<Tensors4(TensorRef, TensorRef, TensorRef, double)>("hc::layer_norm_ckpt");
     at::AutoDispatchBelowADInplaceOrView guard;
     return op.call(x, gamma, beta, eps);
 }
 Tensors3 act_ckpt_below(TensorRef x, int64_t act) {
+    if (plain_cuda(x)) return activation_gelu_silu_ckpt_cuda(x, act);
     static const auto op = op_handle<Tensors3(TensorRef, int64_t)>("hc::activation_gelu_silu_ckpt");
     at::AutoDispatchBelowADInplaceOrView guard;
     return op.call(x, act);
