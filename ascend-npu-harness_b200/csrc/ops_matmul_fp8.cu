@@ -54,7 +54,8 @@ struct Params {
     uint32_t M, N, K, kb;  // kb = ceil(K / 128)
     uint32_t nb;           // ceil(N / 128)
     uint32_t tiles_m, tiles_n, num_tiles;
-    uint32_t vec_store;    // rows of C start on 16-byte boundaries
+    uint32_t vec_store;    // rows of C are whole 16-byte packs on 16-byte boundaries
+    uint32_t vec_bias;     // bias starts on a 16-byte boundary
 };
 
 // K blocks are 128 e4m3 bytes deep: one swizzle row, one scale.
@@ -69,8 +70,8 @@ constexpr uint32_t kPanel = 128 * kBK;  // 16 KB: 128 rows of either operand
 //               two TMEM accumulators of 256 columns.  Two N=128 halves with accumulators of their
 //               own would hand over sooner but read A twice: with the TMA writes 80 KB of shared
 //               memory per block instead of 64, and 128 B/cycle make that 640 cycles instead of 512
-//   warps 2-3   products of the scales for four K blocks at a time, row by row into shared memory: read
-//               by the promoting threads themselves (32 rows, 32 lines each) they cost a third of the time
+//   warps 2-3   products of the scales for eight K blocks at a time into shared memory: read by the
+//               promoting threads themselves (32 rows, 32 lines each) they cost a third of the time
 //   warps 4-11  promotion: warp w reads TMEM lanes 32 (w % 4) .. + 31 (thread = row) and 128 columns, one
 //               128-block of N: 128 running sums per thread, one multiply-add each (as f32x2 pairs)
 //               with one product of scales per block, the next 32 columns on their way meanwhile.
@@ -87,15 +88,17 @@ constexpr uint32_t kPairEpiWarps = 8;
 constexpr uint32_t kPairThreads = 128 + 32 * kPairEpiWarps;
 constexpr uint32_t kPairStageBytes = 2 * kPanel;
 constexpr uint32_t kPairOffTurn = kPairStages * kPairStageBytes;             // turning tiles of the promoting warps
-constexpr uint32_t kPairOffScale = kPairOffTurn + kPairEpiWarps * 32 * 16 * 4;  // [2 groups][4 blocks][2 panels][128]
-constexpr uint32_t kPairOffBar = kPairOffScale + 2 * 4 * 256 * 4;
+constexpr uint32_t kScaleGroup = 8;                                            // K blocks
+constexpr uint32_t kScaleRow = 2 * 128 + 4;  // products of one block, [2 panels][128], padded against bank conflicts
+constexpr uint32_t kPairOffScale = kPairOffTurn + kPairEpiWarps * 32 * 16 * 4;  // [2 groups][kScaleGroup][kScaleRow]
+constexpr uint32_t kPairOffBar = kPairOffScale + 2 * kScaleGroup * kScaleRow * 4;
 constexpr uint32_t kPairSmem = kPairOffBar + 256 + 1024;
 constexpr uint32_t kPairGroupM = 8;  // pair-tile rows per rasterisation group (A and B panels shared in L2)
 
 struct PairBars {
     uint64_t full[kPairStages], empty[kPairStages];
     uint64_t acc_full[2], acc_empty[2];  // [block & 1]
-    uint64_t sc_full[2], sc_empty[2];    // [group of four blocks & 1]
+    uint64_t sc_full[2], sc_empty[2];    // [group of blocks & 1]
     uint64_t mma_done;
 };
 
@@ -117,7 +120,7 @@ __device__ __forceinline__ void scale_add32(float2* acc, const uint32_t (&d)[32]
         acc[i] = __ffma2_rn(make_float2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), s2, acc[i]);
 }
 
-// 128 sums of one row to C (vec_store): packs of 16 bytes, the last columns one by one.
+// 128 sums of one row to C (vec_store) in packs of 16 bytes.
 template <typename T>
 __device__ __forceinline__ void store_row(const Params& p, const float2* acc, uint64_t row, uint32_t n0) {
     constexpr uint32_t P = elem<T>::kPack;
@@ -125,20 +128,22 @@ __device__ __forceinline__ void store_row(const Params& p, const float2* acc, ui
     T* crow = static_cast<T*>(p.c) + row * p.N;
 #pragma unroll
     for (uint32_t j = 0; j < 128; j += P) {
+        if (n0 + j >= p.N) break;  // N is a multiple of P here
         float v[P];
 #pragma unroll
-        for (uint32_t e = 0; e < P; ++e) {
-            const float2 pr = acc[(j + e) / 2];
-            v[e] = (e & 1) ? pr.y : pr.x;
-            if (bias && n0 + j + e < p.N) v[e] += elem<T>::to_f(bias[n0 + j + e]);
-        }
-        if (n0 + j + P <= p.N) {
-            *reinterpret_cast<pack<T>*>(crow + n0 + j) = pack_from_f<T>(v);
-        } else {
+        for (uint32_t e = 0; e < P; ++e) v[e] = (e & 1) ? acc[(j + e) / 2].y : acc[(j + e) / 2].x;
+        if (bias) {
+            pack<T> b;
+            if (p.vec_bias) {
+                b = ld_cached(reinterpret_cast<const pack<T>*>(bias + n0 + j));
+            } else {
 #pragma unroll
-            for (uint32_t e = 0; e < P; ++e)
-                if (n0 + j + e < p.N) crow[n0 + j + e] = elem<T>::from_f(v[e]);
+                for (uint32_t e = 0; e < P; ++e) b.v[e] = bias[n0 + j + e];
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < P; ++e) v[e] += elem<T>::to_f(b.v[e]);
         }
+        *reinterpret_cast<pack<T>*>(crow + n0 + j) = pack_from_f<T>(v);
     }
 }
 
@@ -294,43 +299,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             }
         } else if (warp < 4) {
             // ============================= products of the scales =============================
-            // two rows per thread; the loads of the next four blocks are under way while the last are read
-            const uint32_t r = (warp - 2) * 32 + lane;
-            float* ring = reinterpret_cast<float*>(smem + kPairOffScale);
+            // a load instruction takes four rows of eight blocks; the loads of the next group are under way
+            // while the last is read
+            const uint32_t k = lane % kScaleGroup, r0 = (warp - 2) * 64 + lane / kScaleGroup;
+            float* ring = reinterpret_cast<float*>(smem + kPairOffScale) + k * kScaleRow + r0;
             uint32_t sg = 0;
             bool ok = true;
             for (uint32_t t = cluster; t < p.num_tiles && ok; t += clusters) {
                 uint32_t tm, tn;
                 pair_tile(p, t, tm, tn);
-                // rows and columns behind the end: any valid scale, nothing of them is stored
-                const uint32_t row = tm * 256 + rank * 128 + r;
-                const float* sa[2] = {p.a_scale + static_cast<uint64_t>(min(row, p.M - 1)) * p.kb,
-                                      p.a_scale + static_cast<uint64_t>(min(row + 64, p.M - 1)) * p.kb};
-                const float* sb[2] = {p.b_scale + static_cast<uint64_t>(min(tn * 2, p.nb - 1)) * p.kb,
-                                      p.b_scale + static_cast<uint64_t>(min(tn * 2 + 1, p.nb - 1)) * p.kb};
-                for (uint32_t kb = 0; kb < p.kb; kb += 4, ++sg) {
-                    float va[2][4], vb[2][4];
-    #pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i) {
-                        const uint32_t k = min(kb + i, p.kb - 1);
-    #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            va[j][i] = __ldg(sa[j] + k);
-                            vb[j][i] = __ldg(sb[j] + k);
-                        }
-                    }
+                // rows, columns and blocks behind the end: any valid scale, nothing of them is used
+                const uint32_t row = tm * 256 + rank * 128 + r0;
+                const float* sb0 = p.b_scale + static_cast<uint64_t>(min(tn * 2, p.nb - 1)) * p.kb;
+                const float* sb1 = p.b_scale + static_cast<uint64_t>(min(tn * 2 + 1, p.nb - 1)) * p.kb;
+                for (uint32_t kb = 0; kb < p.kb; kb += kScaleGroup, ++sg) {
+                    const uint32_t kk = min(kb + k, p.kb - 1);
+                    constexpr uint32_t kRows = 32 / kScaleGroup, kLoads = 64 / kRows;
+                    float va[kLoads];
+#pragma unroll
+                    for (uint32_t i = 0; i < kLoads; ++i)
+                        va[i] = __ldg(p.a_scale + static_cast<uint64_t>(min(row + kRows * i, p.M - 1)) * p.kb + kk);
+                    const float b0 = __ldg(sb0 + kk), b1 = __ldg(sb1 + kk);
                     ok = mbar_wait_bounded(&bars->sc_empty[sg & 1], ((sg >> 1) & 1) ^ 1, abort_flag, &g_mm8_error_word,
                                            kErrScale);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    float* out = ring + (sg & 1) * 1024 + r;
-    #pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i)
-    #pragma unroll
-                        for (int pn = 0; pn < 2; ++pn) {
-                            out[i * 256 + pn * 128] = va[0][i] * vb[pn][i];
-                            out[i * 256 + pn * 128 + 64] = va[1][i] * vb[pn][i];
-                        }
+                    float* out = ring + (sg & 1) * kScaleGroup * kScaleRow;
+#pragma unroll
+                    for (uint32_t i = 0; i < kLoads; ++i) {
+                        out[kRows * i] = va[i] * b0;
+                        out[kRows * i + 128] = va[i] * b1;
+                    }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bars->sc_full[sg & 1]);
                 }
@@ -351,9 +350,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         float s;
         // scale and the first 32 columns of the next block (kb of its tile)
         auto fetch = [&](uint32_t kb) {
-            if (kb % 4 == 0)
+            if (kb % kScaleGroup == 0)
                 mbar_wait_bounded(&bars->sc_full[sg & 1], (sg >> 1) & 1, abort_flag, &g_mm8_error_word, kErrScale);
-            s = ring[(sg & 1) * 1024 + (kb % 4) * 256];
+            s = ring[((sg & 1) * kScaleGroup + kb % kScaleGroup) * kScaleRow];
             mbar_wait_bounded(&bars->acc_full[g & 1], (g >> 1) & 1, abort_flag, &g_mm8_error_word, kErrEpi);
             __syncwarp();
             tc_fence_after();
@@ -378,7 +377,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 tmem_wait_ld32(d1);
                 tc_fence_before();
                 __syncwarp();
-                const bool group_end = kb % 4 == 3 || kb + 1 == p.kb;
+                const bool group_end = kb % kScaleGroup == kScaleGroup - 1 || kb + 1 == p.kb;
                 if (lane == 0) {
                     mbar_arrive_peer(empty_even + (g & 1) * 8);
                     if (group_end) mbar_arrive(&bars->sc_empty[sg & 1]);
@@ -850,6 +849,7 @@ int launch(Params p, cudaStream_t s) {
     p.tiles_m = (p.M + 255) / 256;
     p.tiles_n = (p.N + 255) / 256;
     const uint64_t tiles = static_cast<uint64_t>(p.tiles_m) * p.tiles_n;
+    p.vec_bias = aligned16(p.bias);
     p.vec_store = aligned16(p.c) && (static_cast<uint64_t>(p.N) * sizeof(T)) % 16 == 0;
     const int pairs = pair_clusters();
     // grid limits of the few-token kernel: 65535 weight tiles and token tiles
@@ -889,7 +889,7 @@ extern "C" int hc_matmul_fp8_block_launch(const void* a, const float* a_scale, c
     if (!a || !a_scale || !b || !b_scale || !c) return fail(HC_ERR_INVALID, "matmul_fp8_block: null pointer");
     if (fault_hit("launch")) return fail(HC_ERR_INJECTED, "matmul_fp8_block: injected launch failure");
     mm8::Params p{static_cast<const uint8_t*>(a), a_scale, static_cast<const uint8_t*>(b), b_scale, bias, c,
-                  t->M, t->N, t->K, (t->K + kFp8Block - 1) / kFp8Block, (t->N + kFp8Block - 1) / kFp8Block, 0, 0, 0, 0};
+                  t->M, t->N, t->K, (t->K + kFp8Block - 1) / kFp8Block, (t->N + kFp8Block - 1) / kFp8Block, 0, 0, 0, 0, 0};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (dtype) {
         case HC_DTYPE_F32: return mm8::launch<float>(p, s);
