@@ -21,6 +21,7 @@
 #include <cuda_runtime.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "fp8_block.cuh"
 #include "hc_device.cuh"
@@ -55,7 +56,7 @@ struct Params {
     uint32_t nb;           // ceil(N / 128)
     uint32_t tiles_m, tiles_n, num_tiles;
     uint32_t vec_store;    // rows of C are whole 16-byte packs on 16-byte boundaries
-    uint32_t vec_bias;     // bias starts on a 16-byte boundary
+    uint32_t word_store;   // ... whole 4-byte words on 4-byte boundaries
 };
 
 // K blocks are 128 e4m3 bytes deep: one swizzle row, one scale.
@@ -120,54 +121,72 @@ __device__ __forceinline__ void scale_add32(float2* acc, const uint32_t (&d)[32]
         acc[i] = __ffma2_rn(make_float2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), s2, acc[i]);
 }
 
+// Adds the bias of columns [n0, n0 + 128) to a thread's 128 sums: lane l fetches columns 4 l .. 4 l + 3, one
+// load latency for all, and the warp passes them round (one load per column from every thread
+// cost 6 us a tile).
+template <typename T>
+__device__ __forceinline__ void add_bias(const Params& p, float2* acc, uint32_t n0, uint32_t lane) {
+    const T* bias = static_cast<const T*>(p.bias);
+    float b[4];
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) b[e] = n0 + lane * 4 + e < p.N ? elem<T>::to_f(bias[n0 + lane * 4 + e]) : 0.f;
+#pragma unroll
+    for (uint32_t j = 0; j < 64; ++j) {
+        acc[j].x += __shfl_sync(0xffffffffu, b[j % 2 * 2], j / 2);
+        acc[j].y += __shfl_sync(0xffffffffu, b[j % 2 * 2 + 1], j / 2);
+    }
+}
+
 // 128 sums of one row to C (vec_store) in packs of 16 bytes.
 template <typename T>
 __device__ __forceinline__ void store_row(const Params& p, const float2* acc, uint64_t row, uint32_t n0) {
     constexpr uint32_t P = elem<T>::kPack;
-    const T* bias = static_cast<const T*>(p.bias);
     T* crow = static_cast<T*>(p.c) + row * p.N;
 #pragma unroll
-    for (uint32_t j = 0; j < 128; j += P) {
-        if (n0 + j >= p.N) break;  // N is a multiple of P here
-        float v[P];
-#pragma unroll
-        for (uint32_t e = 0; e < P; ++e) v[e] = (e & 1) ? acc[(j + e) / 2].y : acc[(j + e) / 2].x;
-        if (bias) {
-            pack<T> b;
-            if (p.vec_bias) {
-                b = ld_cached(reinterpret_cast<const pack<T>*>(bias + n0 + j));
-            } else {
-#pragma unroll
-                for (uint32_t e = 0; e < P; ++e) b.v[e] = bias[n0 + j + e];
-            }
-#pragma unroll
-            for (uint32_t e = 0; e < P; ++e) v[e] += elem<T>::to_f(b.v[e]);
-        }
-        *reinterpret_cast<pack<T>*>(crow + n0 + j) = pack_from_f<T>(v);
-    }
+    for (uint32_t j = 0; j < 128; j += P)
+        if (n0 + j < p.N)  // N is a multiple of P here
+            *reinterpret_cast<pack<T>*>(crow + n0 + j) = pack_from_f<T>(&acc[j / 2].x);
 }
 
-// A warp's 32 rows x 128 sums to C for any row alignment: 32 x 16 tiles are turned in shared memory so
-// that a store instruction writes 16 neighbouring columns of two rows; row r is rotated by r / 2
-// columns, which spreads both the writes and the reads over all banks.
+// A warp's 32 rows x 128 sums to C for any row alignment: tiles of 32 rows x 16 words (two 16-bit
+// columns, or one fp32) are turned in shared memory so that a store instruction writes neighbouring
+// columns of one or two rows; row r is rotated by r / 2 words, which spreads both the writes and
+// the reads over all banks.
 template <typename T>
-__device__ __forceinline__ void store_turned(const Params& p, const float2* acc, float* tile, uint32_t row0, uint32_t n0,
-                                             uint32_t lane) {
-    const T* bias = static_cast<const T*>(p.bias);
+__device__ __forceinline__ void store_turned(const Params& p, const float2* acc, uint32_t* tile, uint32_t row0,
+                                             uint32_t n0, uint32_t lane) {
+    constexpr uint32_t kPerWord = 4 / sizeof(T), kCols = 16 * kPerWord;
 #pragma unroll
-    for (uint32_t c = 0; c < 8; ++c) {
+    for (uint32_t c = 0; c < 128 / kCols; ++c) {
 #pragma unroll
-        for (uint32_t j = 0; j < 16; ++j)
-            tile[lane * 16 + (j + lane / 2) % 16] = (j & 1) ? acc[c * 8 + j / 2].y : acc[c * 8 + j / 2].x;
-        __syncwarp();
-        const uint32_t n = n0 + c * 16 + lane % 16;
-        const float b = bias && n < p.N ? elem<T>::to_f(bias[n]) : 0.f;
-#pragma unroll 4
-        for (uint32_t r = lane / 16; r < 32; r += 2)
-            if (row0 + r < p.M && n < p.N) {
-                const float v = tile[r * 16 + (lane + r / 2) % 16];
-                static_cast<T*>(p.c)[static_cast<uint64_t>(row0 + r) * p.N + n] = elem<T>::from_f(bias ? v + b : v);
+        for (uint32_t j = 0; j < 16; ++j) {
+            uint32_t w;
+            if constexpr (sizeof(T) == 4) w = __float_as_uint(j & 1 ? acc[c * 8 + j / 2].y : acc[c * 8 + j / 2].x);
+            else if constexpr (std::is_same<T, bf16_t>::value) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(acc[c * 16 + j].x, acc[c * 16 + j].y);
+                w = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                const __half2 h = __floats2half2_rn(acc[c * 16 + j].x, acc[c * 16 + j].y);
+                w = *reinterpret_cast<const uint32_t*>(&h);
             }
+            tile[lane * 16 + (j + lane / 2) % 16] = w;
+        }
+        __syncwarp();
+        if (p.word_store) {
+            const uint32_t n = n0 + c * kCols + lane % 16 * kPerWord;
+            uint8_t* dst = static_cast<uint8_t*>(p.c) + (static_cast<uint64_t>(row0 + lane / 16) * p.N + n) * sizeof(T);
+            const uint64_t step = 2ull * p.N * sizeof(T);
+#pragma unroll 8
+            for (uint32_t r = lane / 16; r < 32; r += 2, dst += step)
+                if (row0 + r < p.M && n < p.N) *reinterpret_cast<uint32_t*>(dst) = tile[r * 16 + (lane + r / 2) % 16];
+        } else {  // 16-bit rows that start between words
+            const uint32_t n = n0 + c * kCols + lane;
+            uint16_t* dst = static_cast<uint16_t*>(p.c) + static_cast<uint64_t>(row0) * p.N + n;
+#pragma unroll 8
+            for (uint32_t r = 0; r < 32; ++r, dst += p.N)
+                if (row0 + r < p.M && n < p.N)
+                    *dst = static_cast<uint16_t>(tile[r * 16 + (lane / 2 + r / 2) % 16] >> (lane % 2 * 16));
+        }
         __syncwarp();
     }
 }
@@ -341,7 +360,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const uint32_t quarter = warp & 3, panel = (warp - 4) / 4;
         const uint32_t tmem_cols = tmem_base + panel * 128 + ((quarter * 32) << 16);
         const uint32_t empty_even = mapa_shared(smem_u32(&bars->acc_empty[0]), 0);
-        float* turn = reinterpret_cast<float*>(smem + kPairOffTurn) + (warp - 4) * 32 * 16;
+        uint32_t* turn = reinterpret_cast<uint32_t*>(smem + kPairOffTurn) + (warp - 4) * 32 * 16;
         const float* ring = reinterpret_cast<const float*>(smem + kPairOffScale) + panel * 128 + quarter * 32 + lane;
         // A wait that gave up has set the error word and the abort flag: the rest runs through, without
         // waiting again, on whatever the accumulators hold.
@@ -391,6 +410,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             uint32_t tm, tn;
             pair_tile(p, t, tm, tn);
             const uint32_t row0 = tm * 256 + rank * 128 + quarter * 32, n0 = tn * 256 + panel * 128;
+            if (p.bias) add_bias<T>(p, acc, n0, lane);
             if (p.vec_store) {
                 if (row0 + lane < p.M) store_row<T>(p, acc, row0 + lane, n0);
             } else {
@@ -849,7 +869,7 @@ int launch(Params p, cudaStream_t s) {
     p.tiles_m = (p.M + 255) / 256;
     p.tiles_n = (p.N + 255) / 256;
     const uint64_t tiles = static_cast<uint64_t>(p.tiles_m) * p.tiles_n;
-    p.vec_bias = aligned16(p.bias);
+    p.word_store = reinterpret_cast<uintptr_t>(p.c) % 4 == 0 && (static_cast<uint64_t>(p.N) * sizeof(T)) % 4 == 0;
     p.vec_store = aligned16(p.c) && (static_cast<uint64_t>(p.N) * sizeof(T)) % 16 == 0;
     const int pairs = pair_clusters();
     // grid limits of the few-token kernel: 65535 weight tiles and token tiles
