@@ -56,6 +56,13 @@ __device__ __forceinline__ float fp8_decode(uint8_t one) {
     return __half2float(*reinterpret_cast<const __half*>(&h));
 }
 
+// max(|a|, |b|, |c|), NaN if any of them is.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+    float m;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+    return m;
+}
+
 __device__ __forceinline__ uint32_t warp_umax(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 
 }  // namespace hc

@@ -13,6 +13,8 @@
 // the variance over deviations from the mean, as in the forward-only kernels.
 #include <cuda_runtime.h>
 
+#include <algorithm>
+
 #include "fp8_block.cuh"
 #include "hc_device.cuh"
 #include "hc_internal.h"
@@ -340,7 +342,7 @@ struct RingShape {
     static constexpr uint32_t kSecond = Ckpt ? (P + 4) * N * Threads : 16 * N * Threads;
     static constexpr uint32_t kStage = kFirst + kSecond;
     static constexpr uint32_t kFit = 192 * 1024 / CtasPerSm / kStage;
-    static constexpr uint32_t kStages = kFit > 6 ? 6 : kFit;
+    static constexpr uint32_t kStages = kFit > 4 ? 4 : kFit;
     static_assert(kStages >= 2, "a ring of one row would not run ahead");
     static constexpr uint32_t kBytes = kStages * kStage;
 };
@@ -445,25 +447,35 @@ __global__ void __launch_bounds__(group_threads(W), W <= 8 ? 3 : 1) ln_fwd_row_k
             a.rstd[row] = rstd;
         }
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) v[i] = __fmul2_rn(__fadd2_rn(v[i], f2(off)), f2(rstd));
+        for (int i = 0; i < kPairs; ++i) v[i] = __ffma2_rn(v[i], f2(rstd), f2(off * rstd));
         Row::clear_behind(v, t, a.H);
         if constexpr (Ckpt && Vec) {
+            // the two quotients of each of the group's N blocks, in one division: lane 2 i of a group of
+            // lanes takes 448 / amax of block i, lane 2 i + 1 its scale
+            uint32_t bits = 0;
 #pragma unroll
             for (int i = 0; i < Row::N; ++i) {
                 const float2* h = v + i * P / 2;
-                uint32_t m = 0;
+                float m = fabsf(h[0].x);
+                m = max3_abs(m, h[0].y, h[1].x);
+                m = max3_abs(m, h[1].y, h[1].y);
 #pragma unroll
-                for (int e = 0; e < P / 2; ++e) m = max(m, max(abs_bits(h[e].x), abs_bits(h[e].y)));
+                for (int e = 2; e < P / 2; ++e) m = max3_abs(m, h[e].x, h[e].y);
+                uint32_t u = abs_bits(m);
 #pragma unroll
-                for (uint32_t o = kFp8Block / P / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-                // one division for both quotients: even lanes 448 / amax, odd lanes the scale
-                const float amax = fp8_amax(m);
-                const float ratio = __fdiv_rn(t & 1 ? amax : kFp8Max, t & 1 ? kFp8Max : amax);
-                const float other = __shfl_xor_sync(0xffffffffu, ratio, 1);
-                const float inv = t & 1 ? other : ratio;
+                for (uint32_t o = kFp8Block / P / 2; o > 0; o >>= 1) u = max(u, __shfl_xor_sync(0xffffffffu, u, o));
+                if (t / 2 % Row::N == i) bits = u;
+            }
+            const float amax = fp8_amax(bits);
+            const float ratio = __fdiv_rn(t & 1 ? amax : kFp8Max, t & 1 ? kFp8Max : amax);
+#pragma unroll
+            for (int i = 0; i < Row::N; ++i) {
+                const float2* h = v + i * P / 2;
+                const float inv = __shfl_sync(0xffffffffu, ratio, 2 * i, kFp8Block / P);
+                const float scale = __shfl_sync(0xffffffffu, ratio, 2 * i + 1, kFp8Block / P);
                 const uint32_t c = Row::first(t, i);
                 if (c >= a.H) continue;
-                if (c % kFp8Block == 0) a.scale[row * a.row_blocks + c / kFp8Block] = other;
+                if (c % kFp8Block == 0) a.scale[row * a.row_blocks + c / kFp8Block] = scale;
                 uint32_t w[P / 4];
 #pragma unroll
                 for (int e = 0; e < P / 2; e += 2) {
@@ -748,7 +760,9 @@ int launch_bwd_rows(BwdArgs& a, float* dgamma, float* dbeta, cudaStream_t s) {
         const uint32_t groups = (a.rows + row_groups(W) - 1) / row_groups(W);
         // A few rows: one CTA goes through them (up to four times, about 1 us each) and writes the sums
         // itself, which saves the join's launch (2 us of host time, 3 us on the GPU).
-        a.parts_n = groups <= 4 ? 1 : parts_of(groups);  // one per CTA
+        // Otherwise one CTA per place on the GPU: a second wave would fill its ring with nothing to hide it.
+        const uint32_t places = static_cast<uint32_t>(sm_count()) * bwd_ctas(W);
+        a.parts_n = groups <= 4 ? 1 : std::min(parts_of(groups), places);
         a.sum_gamma = a.parts_n == 1 ? dgamma : a.parts;
         a.sum_beta = a.parts_n == 1 ? dbeta : a.parts + a.H;
         // the ring, or the joined sums of the row groups: 2 x 16 columns of each thread
