@@ -85,13 +85,14 @@ constexpr uint32_t kPanel = 128 * kBK;  // 16 KB: 128 rows of either operand
 // A block costs the tensor core 512 cycles (256 x 256 x 128 products at 2 x 8192 per cycle).
 // ======================================================================================
 constexpr uint32_t kPairStages = 6;
-constexpr uint32_t kPairEpiWarps = 8;
+constexpr uint32_t kPairEpiWarps = 16;
+constexpr uint32_t kPairCols = 256 * 4 / kPairEpiWarps;                        // columns of a promoting warp
 constexpr uint32_t kPairThreads = 128 + 32 * kPairEpiWarps;
 constexpr uint32_t kPairStageBytes = 2 * kPanel;
 constexpr uint32_t kPairOffTurn = kPairStages * kPairStageBytes;             // turning tiles of the promoting warps
 constexpr uint32_t kScaleGroup = 8;                                            // K blocks
 constexpr uint32_t kScaleRow = 2 * 128 + 4;  // products of one block, [2 panels][128], padded against bank conflicts
-constexpr uint32_t kPairOffScale = kPairOffTurn + kPairEpiWarps * 32 * 16 * 4;  // [2 groups][kScaleGroup][kScaleRow]
+constexpr uint32_t kPairOffScale = kPairOffTurn + kPairEpiWarps * 32 * 8 * 4;  // [2 groups][kScaleGroup][kScaleRow]
 constexpr uint32_t kPairOffBar = kPairOffScale + 2 * kScaleGroup * kScaleRow * 4;
 constexpr uint32_t kPairSmem = kPairOffBar + 256 + 1024;
 constexpr uint32_t kPairGroupM = 8;  // pair-tile rows per rasterisation group (A and B panels shared in L2)
@@ -121,61 +122,60 @@ __device__ __forceinline__ void scale_add32(float2* acc, const uint32_t (&d)[32]
         acc[i] = __ffma2_rn(make_float2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), s2, acc[i]);
 }
 
-// Adds the bias of columns [n0, n0 + 128) to a thread's 128 sums: lane l fetches columns 4 l .. 4 l + 3, one
+// Adds the bias of columns [n0, n0 + 64) to a thread's sums: lane l fetches columns 2 l and 2 l + 1, one
 // load latency for all, and the warp passes them round (one load per column from every thread
 // cost 6 us a tile).
 template <typename T>
 __device__ __forceinline__ void add_bias(const Params& p, float2* acc, uint32_t n0, uint32_t lane) {
     const T* bias = static_cast<const T*>(p.bias);
-    float b[4];
+    const uint32_t n = n0 + lane * 2;
+    const float b0 = n < p.N ? elem<T>::to_f(bias[n]) : 0.f, b1 = n + 1 < p.N ? elem<T>::to_f(bias[n + 1]) : 0.f;
 #pragma unroll
-    for (uint32_t e = 0; e < 4; ++e) b[e] = n0 + lane * 4 + e < p.N ? elem<T>::to_f(bias[n0 + lane * 4 + e]) : 0.f;
-#pragma unroll
-    for (uint32_t j = 0; j < 64; ++j) {
-        acc[j].x += __shfl_sync(0xffffffffu, b[j % 2 * 2], j / 2);
-        acc[j].y += __shfl_sync(0xffffffffu, b[j % 2 * 2 + 1], j / 2);
+    for (uint32_t j = 0; j < kPairCols / 2; ++j) {
+        acc[j].x += __shfl_sync(0xffffffffu, b0, j);
+        acc[j].y += __shfl_sync(0xffffffffu, b1, j);
     }
 }
 
-// A warp's 32 rows x 128 sums to C for any row alignment: tiles of 32 rows x 16 words (two 16-bit
+// A warp's 32 rows x 64 sums to C for any row alignment: tiles of 32 rows x 8 words (two 16-bit
 // columns, or one fp32) are turned in shared memory so that a store instruction writes neighbouring
-// columns of one or two rows; row r is rotated by r / 2 words, which spreads both the writes and
+// columns of four rows (two); row r is rotated by r / 4 words, which spreads both the writes and
 // the reads over all banks.  Rows of whole 16-byte packs take this way too: a lane writing its own
 // row in packs was slower (5327 x 5736 x 720: 54 us against 50).
 template <typename T>
 __device__ __forceinline__ void store_turned(const Params& p, const float2* acc, uint32_t* tile, uint32_t row0,
                                              uint32_t n0, uint32_t lane) {
-    constexpr uint32_t kPerWord = 4 / sizeof(T), kCols = 16 * kPerWord;
+    constexpr uint32_t kPerWord = 4 / sizeof(T), kCols = 8 * kPerWord;
 #pragma unroll
-    for (uint32_t c = 0; c < 128 / kCols; ++c) {
+    for (uint32_t c = 0; c < kPairCols / kCols; ++c) {
 #pragma unroll
-        for (uint32_t j = 0; j < 16; ++j) {
+        for (uint32_t j = 0; j < 8; ++j) {
             uint32_t w;
-            if constexpr (sizeof(T) == 4) w = __float_as_uint(j & 1 ? acc[c * 8 + j / 2].y : acc[c * 8 + j / 2].x);
+            if constexpr (sizeof(T) == 4) w = __float_as_uint(j & 1 ? acc[c * 4 + j / 2].y : acc[c * 4 + j / 2].x);
             else if constexpr (std::is_same<T, bf16_t>::value) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(acc[c * 16 + j].x, acc[c * 16 + j].y);
+                const __nv_bfloat162 h = __floats2bfloat162_rn(acc[c * 8 + j].x, acc[c * 8 + j].y);
                 w = *reinterpret_cast<const uint32_t*>(&h);
             } else {
-                const __half2 h = __floats2half2_rn(acc[c * 16 + j].x, acc[c * 16 + j].y);
+                const __half2 h = __floats2half2_rn(acc[c * 8 + j].x, acc[c * 8 + j].y);
                 w = *reinterpret_cast<const uint32_t*>(&h);
             }
-            tile[lane * 16 + (j + lane / 2) % 16] = w;
+            tile[lane * 8 + (j + lane / 4) % 8] = w;
         }
         __syncwarp();
         if (p.word_store) {
-            const uint32_t n = n0 + c * kCols + lane % 16 * kPerWord;
-            uint8_t* dst = static_cast<uint8_t*>(p.c) + (static_cast<uint64_t>(row0 + lane / 16) * p.N + n) * sizeof(T);
-            const uint64_t step = 2ull * p.N * sizeof(T);
+            const uint32_t n = n0 + c * kCols + lane % 8 * kPerWord;
+            uint8_t* dst = static_cast<uint8_t*>(p.c) + (static_cast<uint64_t>(row0 + lane / 8) * p.N + n) * sizeof(T);
+            const uint64_t step = 4ull * p.N * sizeof(T);
 #pragma unroll 8
-            for (uint32_t r = lane / 16; r < 32; r += 2, dst += step)
-                if (row0 + r < p.M && n < p.N) *reinterpret_cast<uint32_t*>(dst) = tile[r * 16 + (lane + r / 2) % 16];
+            for (uint32_t r = lane / 8; r < 32; r += 4, dst += step)
+                if (row0 + r < p.M && n < p.N) *reinterpret_cast<uint32_t*>(dst) = tile[r * 8 + (lane + r / 4) % 8];
         } else {  // 16-bit rows that start between words
-            const uint32_t n = n0 + c * kCols + lane;
-            uint16_t* dst = static_cast<uint16_t*>(p.c) + static_cast<uint64_t>(row0) * p.N + n;
+            const uint32_t n = n0 + c * kCols + lane % 16;
+            uint16_t* dst = static_cast<uint16_t*>(p.c) + static_cast<uint64_t>(row0 + lane / 16) * p.N + n;
 #pragma unroll 8
-            for (uint32_t r = 0; r < 32; ++r, dst += p.N)
+            for (uint32_t r = lane / 16; r < 32; r += 2, dst += 2ull * p.N)
                 if (row0 + r < p.M && n < p.N)
-                    *dst = static_cast<uint16_t>(tile[r * 16 + (lane / 2 + r / 2) % 16] >> (lane % 2 * 16));
+                    *dst = static_cast<uint16_t>(tile[r * 8 + (lane % 16 / 2 + r / 4) % 8] >> (lane % 2 * 16));
         }
         __syncwarp();
     }
@@ -223,7 +223,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const uint32_t s_base = smem_u32(smem);
 
     if (warp < 4) {
-        setmaxnreg_dec<72>();
+        setmaxnreg_dec<64>();
         if (warp == 0) {
             // ================================ TMA producers ================================
             if (lane == 0) {
@@ -346,44 +346,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         }
     } else {
         // ================================== promotion ==================================
-        setmaxnreg_inc<216>();
-        const uint32_t quarter = warp & 3, panel = (warp - 4) / 4;
-        const uint32_t tmem_cols = tmem_base + panel * 128 + ((quarter * 32) << 16);
+        setmaxnreg_inc<104>();
+        const uint32_t quarter = warp & 3, part = (warp - 4) / 4;
+        const uint32_t tmem_cols = tmem_base + part * kPairCols + ((quarter * 32) << 16);
         const uint32_t empty_even = mapa_shared(smem_u32(&bars->acc_empty[0]), 0);
-        uint32_t* turn = reinterpret_cast<uint32_t*>(smem + kPairOffTurn) + (warp - 4) * 32 * 16;
-        const float* ring = reinterpret_cast<const float*>(smem + kPairOffScale) + panel * 128 + quarter * 32 + lane;
+        uint32_t* turn = reinterpret_cast<uint32_t*>(smem + kPairOffTurn) + (warp - 4) * 32 * 8;
+        const float* ring = reinterpret_cast<const float*>(smem + kPairOffScale) + part * kPairCols / 128 * 128 + quarter * 32 + lane;
         // A wait that gave up has set the error word and the abort flag: the rest runs through, without
         // waiting again, on whatever the accumulators hold.
         uint32_t g = 0, sg = 0;
-        uint32_t d0[32], d1[32];
-        float s;
-        // scale and the first 32 columns of the next block (kb of its tile)
-        auto fetch = [&](uint32_t kb) {
-            if (kb % kScaleGroup == 0)
-                mbar_wait_bounded(&bars->sc_full[sg & 1], (sg >> 1) & 1, abort_flag, &g_mm8_error_word, kErrScale);
-            s = ring[((sg & 1) * kScaleGroup + kb % kScaleGroup) * kScaleRow];
-            mbar_wait_bounded(&bars->acc_full[g & 1], (g >> 1) & 1, abort_flag, &g_mm8_error_word, kErrEpi);
-            __syncwarp();
-            tc_fence_after();
-            tmem_ld32(tmem_cols + (g & 1) * 256, d0);
-        };
         for (uint32_t t = cluster; t < p.num_tiles; t += clusters) {
-            float2 acc[64];
+            float2 acc[kPairCols / 2];
 #pragma unroll
-            for (int i = 0; i < 64; ++i) acc[i] = make_float2(0.f, 0.f);
-            fetch(0);
-            for (uint32_t kb = 0; kb < p.kb; ++kb) {
+            for (int i = 0; i < kPairCols / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+            for (uint32_t kb = 0; kb < p.kb; ++kb, ++g) {
+                if (kb % kScaleGroup == 0)
+                    mbar_wait_bounded(&bars->sc_full[sg & 1], (sg >> 1) & 1, abort_flag, &g_mm8_error_word, kErrScale);
+                const float s = ring[((sg & 1) * kScaleGroup + kb % kScaleGroup) * kScaleRow];
+                mbar_wait_bounded(&bars->acc_full[g & 1], (g >> 1) & 1, abort_flag, &g_mm8_error_word, kErrEpi);
+                __syncwarp();
+                tc_fence_after();
                 const uint32_t base = tmem_cols + (g & 1) * 256;
-                tmem_wait_ld32(d0);
-                tmem_ld32(base + 32, d1);
-                scale_add32(acc, d0, s);
-                tmem_wait_ld32(d1);
-                tmem_ld32(base + 64, d0);
-                scale_add32(acc + 16, d1, s);
-                tmem_wait_ld32(d0);
-                tmem_ld32(base + 96, d1);
-                scale_add32(acc + 32, d0, s);
-                tmem_wait_ld32(d1);
+                uint32_t d[32];
+                tmem_ld32(base, d);
+                tmem_wait_ld32(d);
+                scale_add32(acc, d, s);
+                tmem_ld32(base + 32, d);
+                tmem_wait_ld32(d);
                 tc_fence_before();
                 __syncwarp();
                 const bool group_end = kb % kScaleGroup == kScaleGroup - 1 || kb + 1 == p.kb;
@@ -392,14 +381,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     if (group_end) mbar_arrive(&bars->sc_empty[sg & 1]);
                 }
                 if (group_end) ++sg;
-                ++g;
-                const float s_last = s;
-                if (kb + 1 < p.kb) fetch(kb + 1);  // under way while the last 32 columns are added
-                scale_add32(acc + 48, d1, s_last);
+                scale_add32(acc + 16, d, s);
             }
             uint32_t tm, tn;
             pair_tile(p, t, tm, tn);
-            const uint32_t row0 = tm * 256 + rank * 128 + quarter * 32, n0 = tn * 256 + panel * 128;
+            const uint32_t row0 = tm * 256 + rank * 128 + quarter * 32, n0 = tn * 256 + part * kPairCols;
             if (p.bias) add_bias<T>(p, acc, n0, lane);
             store_turned<T>(p, acc, turn, row0, n0, lane);
         }
