@@ -578,7 +578,9 @@ def load_torch_ops():
     hc::flash_attention_fwd_fused gets an autograd formula: hc::flash_attention_bwd (q, k, v get
     gradients; the lse output is not differentiable).  hc::layer_norm_fwd_train, hc::layer_norm_ckpt and
     hc::activation_gelu_silu_ckpt are differentiable in their first output through their _bwd ops, the latter two
-    from the 8-bit blocks they return, without keeping their input."""
+    from the 8-bit blocks they return, without keeping their input.  Capturing such a backward into a CUDA
+    graph follows torch's rule: no eager graph of the same leaves may live meanwhile (torch raises); the _bwd
+    ops themselves can be captured at any time."""
     global _torch_ops_loaded
     torch = _torch()
     if not _torch_ops_loaded:

@@ -198,6 +198,37 @@ def test_matmul(cuda, M, N, K, kind):
     hc.check_device_error()
 
 
+# (M, N, K, path): pairs with rows of C that are whole packs, whole words, and neither; several tiles per
+# pair; one K block and fewer blocks than a group of scales; then the few-token kernel with its
+# clusters of 1 to 8 CTAs and each of its token tiles
+PATHS = [(2500, 2304, 400, 3), (2311, 2310, 1040, 3), (2305, 2561, 2064, 3), (4100, 4099, 128, 3), (5000, 2055, 1168, 3),
+         (9000, 4000, 272, 3), (1, 6272, 2048, 1), (2, 3712, 2560, 1), (7, 3000, 3056, 1), (1, 2688, 3584, 1),
+         (20, 384, 8192, 1), (48, 20000, 512, 1), (90, 777, 4096, 1), (96, 1030, 144, 1), (100, 4001, 1024, 1),
+         (200, 257, 16384, 1)]
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("M,N,K,path", PATHS)
+def test_matmul_paths(cuda, M, N, K, path, kind):
+    ops4 = operands(M, N, K, 12)
+    bias = rnd((N,), 13, kind).cuda()
+    c = hc.matmul_fp8_block(*ops4, bias, R.DTYPES[kind])
+    assert hc.load().hc_matmul_fp8_block_last_path() == path
+    check_product(c, *ops4, bias)
+    hc.check_device_error()
+
+
+def test_matmul_output_past_32_bits(cuda):
+    """More than 2^32 elements of C: the last rows are those of the same product on its own."""
+    M, N, K = 66000, 65600, 128
+    a_q, a_s, w_q, w_s = operands(300, N, K, 28)
+    big = a_q.view(torch.uint8).repeat(M // 300 + 1, 1)[:M].contiguous().view(F8)
+    c = hc.matmul_fp8_block(big, a_s.repeat(M // 300 + 1, 1)[:M].contiguous(), w_q, w_s)
+    first = M // 300 * 300
+    assert torch.equal(c[first:], c[:M - first]) and torch.equal(c[first - 300:first], c[:300])
+    check_product(c[M - 3:], big[M - 3:], a_s.repeat(M // 300 + 1, 1)[M - 3:M].contiguous(), w_q, w_s, None)
+
+
 @pytest.mark.parametrize("M,N,K", [(5, 9, 33), (40, 130, 200), (300, 260, 1001), (1, 64, 8)])
 def test_matmul_rows_of_any_length(cuda, M, N, K):
     """K that is no multiple of 16 runs on the SIMT kernel."""
@@ -269,6 +300,23 @@ def test_matmul_rows_do_not_depend_on_the_batch(cuda):
                                                       torch.cuda.current_stream().cuda_stream))
         check_product(buf[:m], a_q[:m], a_s[:m], w_q, w_s, None)
         assert bool((buf[m:] == 7.0).all())
+
+
+@pytest.mark.parametrize("cols", [128, 520])
+def test_more_than_32_bits_of_elements(ops, cols):
+    """Over 2^32 elements: the last rows of a tensor of repeated rows equal the first."""
+    part = rnd((512, cols), 29, "bf16").cuda()
+    n = (1 << 32) // (512 * cols) + 2
+    x = part.repeat(n, 1)
+    assert x.numel() > 1 << 32
+    y, q, scale = ops.activation_gelu_silu_ckpt(x, 1)
+    y0, q0, s0 = ops.activation_gelu_silu_ckpt(part, 1)
+    for at in (0, n // 2, n - 1):
+        rows = slice(512 * at, 512 * (at + 1))
+        assert torch.equal(y[rows], y0) and torch.equal(scale[rows], s0)
+        assert torch.equal(q[rows].view(torch.uint8), q0.view(torch.uint8))
+    dx = ops.activation_gelu_silu_ckpt_bwd(x, q, scale, 1)
+    assert torch.equal(dx[-512:], ops.activation_gelu_silu_ckpt_bwd(part, q0, s0, 1))
 
 
 # ------------------------------------------------------------------------------ streams, graphs, together

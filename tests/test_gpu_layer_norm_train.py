@@ -14,7 +14,7 @@ EPS = 1e-5
 KINDS = ["f32", "f16", "bf16"]
 SHAPES = [(1, 1), (3, 2), (5, 7), (2, 8), (4, 64), (9, 127), (1, 128), (37, 129), (2, 3, 136), (33, 768), (8, 1024), (65, 1000),
           (130, 1001), (700, 256), (40, 2048), (301, 520), (16, 4096), (3, 5120), (5, 8192), (3, 8200), (2, 16384), (2, 20000),
-          (2, 20001), (2000, 72)]
+          (2, 20001), (2000, 72), (5000, 8), (600, 1536), (1300, 4096), (700, 6000), (450, 7001)]
 
 
 @pytest.fixture(scope="module")
@@ -235,3 +235,59 @@ def test_training_step_in_a_graph(ops):
         graph.replay()
         for a, want in zip(out, step()):
             assert torch.equal(a, want)
+
+
+def test_explicit_backward_in_a_graph_beside_an_eager_graph(ops):
+    """torch refuses to capture an autograd backward while an eager graph of the same leaves lives; the _bwd
+    ops can be captured then, and the eager graph still gives its gradients afterwards."""
+    x, gamma, beta, dy = inputs((70, 520), "bf16")
+    leaf = x.clone().requires_grad_(True)
+    alive = ops.layer_norm_fwd_train(leaf, gamma, beta, EPS)[0]
+
+    def step():
+        with torch.no_grad():
+            y, q, scale, rstd = ops.layer_norm_ckpt(leaf, gamma, beta, EPS)
+            return (y, *ops.layer_norm_ckpt_bwd(dy, q, scale, gamma, rstd))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    graph.replay()
+    for a, want in zip(out, step()):
+        assert torch.equal(a, want)
+    alive.backward(dy)
+    _, mean, rstd = ops.layer_norm_fwd_train(x, gamma, beta, EPS)
+    assert torch.equal(leaf.grad, ops.layer_norm_bwd(dy, x, gamma, mean, rstd)[0])
+
+
+@pytest.mark.parametrize("H", [264, 4104])
+def test_more_than_32_bits_of_elements(ops, H):
+    """Over 2^32 elements: the last rows of a tensor of repeated rows equal the first, and the weights'
+    gradients are those of one copy times the number of copies, within the additions' error."""
+    part, gamma, beta, dpart = inputs((256, H), "bf16")
+    n = (1 << 32) // (256 * H) + 2
+    x, dy = part.repeat(n, 1), dpart.repeat(n, 1)
+    assert x.numel() > 1 << 32
+    y0, q0, s0, r0 = ops.layer_norm_ckpt(part, gamma, beta, EPS)
+    y, q, scale, rstd = ops.layer_norm_ckpt(x, gamma, beta, EPS)
+    assert torch.equal(y[-256:], y0) and torch.equal(scale[-256:], s0) and torch.equal(rstd[-256:], r0)
+    assert torch.equal(q[-256:].view(torch.uint8), q0.view(torch.uint8))
+    dx0, _, _ = ops.layer_norm_ckpt_bwd(dpart, q0, s0, gamma, r0)
+    dx, dgamma, dbeta = ops.layer_norm_ckpt_bwd(dy, q, scale, gamma, rstd)
+    assert torch.equal(dx[-256:], dx0)
+    xh = R.values(q0, s0)
+    bound = R.layer_norm_grad_bounds(dpart, xh, R.U * xh.abs(), r0.double()[:, None], gamma)
+    _, dg, db = R.layer_norm_grads(dpart, xh, r0.double()[:, None], gamma)
+    rows = x.shape[0] + 16  # additions, instead of the 256 + 16 of one copy
+    R.assert_within(dgamma, n * dg, n * bound[1] * rows / (256 + 16), "dgamma")
+    R.assert_within(dbeta, n * db, n * bound[2] * rows / (256 + 16), "dbeta")
+    del y, q, dx
+    y, mean, rstd = ops.layer_norm_fwd_train(x, gamma, beta, EPS)
+    assert torch.equal(y[-256:], y0) and torch.equal(rstd[-256:], r0)
+    dx, _, _ = ops.layer_norm_bwd(dy, x, gamma, mean, rstd)
+    assert torch.equal(dx[-256:], dx[:256])
