@@ -75,7 +75,7 @@ template <typename T, bool HasAct>
 __global__ void __launch_bounds__(kThreads) block_bwd_kernel(const T* __restrict__ dy, const uint8_t* __restrict__ q,
                                                              const float* __restrict__ scale, T* __restrict__ out,
                                                              uint32_t rows, uint32_t cols, uint32_t row_blocks,
-                                                             ActSlope<sizeof(T) == 4> slope) {
+                                                             ActSlope slope) {
     const uint32_t lane = threadIdx.x & 31;
     const uint64_t total = static_cast<uint64_t>(rows) * row_blocks;
     const uint64_t stride = static_cast<uint64_t>(gridDim.x) * (kThreads / 32);
@@ -194,7 +194,8 @@ __global__ void __launch_bounds__(kThreads) block_fwd_vec_kernel(const T* __rest
         uint32_t n = 0;
         at[u] = b < blocks ? map.start(b, n) + c : 0;
         have[u] = c < n;  // rows are whole packs, so a pack is in or out
-        if (have[u]) in[u] = ld_stream(reinterpret_cast<const pack<T>*>(x + at[u]));
+        // without a branch around it, so that all loads are issued before the first is used
+        in[u] = ld_stream(reinterpret_cast<const pack<T>*>(x + (have[u] ? at[u] : 0)));
     }
     // The two divisions of each of the group's blocks, all at once: lane 2 u of the group takes
     // 448 / amax of block u, lane 2 u + 1 amax / 448 (eight lanes; every lane computing its own two
@@ -233,7 +234,7 @@ template <typename T, bool HasAct>
 __global__ void __launch_bounds__(kThreads) block_bwd_vec_kernel(const T* __restrict__ dy, const uint8_t* __restrict__ q,
                                                                  const float* __restrict__ scale, T* __restrict__ out,
                                                                  uint32_t blocks, const BlockMap map,
-                                                                 ActSlope<sizeof(T) == 4> slope) {
+                                                                 ActSlope slope) {
     using V = Vec<T>;
     const uint32_t c = threadIdx.x % V::G * V::P;
     const uint32_t b0 = blockIdx.x * V::kPerCta + threadIdx.x / V::G;
@@ -248,28 +249,27 @@ __global__ void __launch_bounds__(kThreads) block_bwd_vec_kernel(const T* __rest
         uint32_t n = 0;
         at[u] = b < blocks ? map.start(b, n) + c : 0;
         have[u] = c < n;
-        if (!have[u]) continue;
-        if (HasAct) in[u] = ld_stream(reinterpret_cast<const pack<T>*>(dy + at[u]));
+        const uint64_t from = have[u] ? at[u] : 0;  // without a branch around them, as in the forward
+        if (HasAct) in[u] = ld_stream(reinterpret_cast<const pack<T>*>(dy + from));
         if (V::P == 8)
-            codes[u] = __ldcs(reinterpret_cast<const uint2*>(q + at[u]));
+            codes[u] = __ldcs(reinterpret_cast<const uint2*>(q + from));
         else
-            codes[u].x = __ldcs(reinterpret_cast<const uint32_t*>(q + at[u]));
-        s[u] = __ldg(scale + b);
+            codes[u].x = __ldcs(reinterpret_cast<const uint32_t*>(q + from));
+        s[u] = __ldg(scale + min(b, blocks - 1));
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
         if (!have[u]) continue;
-        float v[V::P], g[V::P];
+        float v[V::P];
 #pragma unroll
         for (uint32_t e = 0; e < V::P; e += 2) {
-            const float2 f = fp8_decode2((e < 4 ? codes[u].x : codes[u].y) >> (e % 4 * 8));
-            v[e] = __fmul_rn(f.x, s[u]);
-            v[e + 1] = __fmul_rn(f.y, s[u]);
-        }
-        if (HasAct) {
-            unpack<T>(in[u], g);
-#pragma unroll
-            for (uint32_t e = 0; e < V::P; ++e) v[e] = __fmul_rn(g[e], slope(v[e]));
+            float2 f = __fmul2_rn(fp8_decode2((e < 4 ? codes[u].x : codes[u].y) >> (e % 4 * 8)), make_float2(s[u], s[u]));
+            if (HasAct) {
+                const float2 g = make_float2(elem<T>::to_f(in[u].v[e]), elem<T>::to_f(in[u].v[e + 1]));
+                f = __fmul2_rn(g, slope.apply2(f));
+            }
+            v[e] = f.x;
+            v[e + 1] = f.y;
         }
         st_stream(reinterpret_cast<pack<T>*>(out + at[u]), pack_from_f<T>(v));
     }
@@ -375,7 +375,7 @@ template <typename T, bool HasAct>
 int launch_bwd(const void* dy, const void* q, const float* scale, void* out, uint32_t rows, uint32_t cols, uint32_t act,
                cudaStream_t s, const char* name) {
     const uint32_t nb = (cols + kFp8Block - 1) / kFp8Block;
-    const auto slope = ActSlope<sizeof(T) == 4>::make(act);
+    const auto slope = ActSlope::make(act);
     const uint64_t blocks = static_cast<uint64_t>(rows) * nb;
     if (vec_ok<T>(out, HasAct ? dy : out, q, rows, cols, nb)) {
         const unsigned grid = static_cast<unsigned>((blocks + Vec<T>::kPerCta - 1) / Vec<T>::kPerCta);
