@@ -758,11 +758,12 @@ int launch_bwd_rows(BwdArgs& a, float* dgamma, float* dbeta, cudaStream_t s) {
     return by_warps(a.H, [&](auto w) {
         constexpr int W = decltype(w)::value;
         const uint32_t groups = (a.rows + row_groups(W) - 1) / row_groups(W);
-        // A few rows: one CTA goes through them (up to four times, about 1 us each) and writes the sums
-        // itself, which saves the join's launch (2 us of host time, 3 us on the GPU).
+        // A few rows: one CTA goes through them (up to four times, about 1 us each; 5 us where a row's
+        // elements are loaded one by one) and writes the sums itself, which saves the join's launch (2 us
+        // of host time, 3 us on the GPU).
         // Otherwise one CTA per place on the GPU: a second wave would fill its ring with nothing to hide it.
         const uint32_t places = static_cast<uint32_t>(sm_count()) * bwd_ctas(W);
-        a.parts_n = groups <= 4 ? 1 : std::min(parts_of(groups), places);
+        a.parts_n = groups <= (Vec ? 4 : 1) ? 1 : std::min(parts_of(groups), places);
         a.sum_gamma = a.parts_n == 1 ? dgamma : a.parts;
         a.sum_beta = a.parts_n == 1 ? dbeta : a.parts + a.H;
         // the ring, or the joined sums of the row groups: 2 x 16 columns of each thread

@@ -789,18 +789,62 @@ int launch_pair(Params p, int pairs, cudaStream_t s) {
     return check_launch("mm8_pair_kernel");
 }
 
-// Splits of K for the few-token kernel: the least work of the busiest SM, in K blocks and a join that
-// costs about as much as two; at most as many CTAs as are resident at once, unless one split is more.
+// Clusters of `c` CTAs of the few-token kernel that the current device holds at once (cached per device):
+// fewer than its SMs give by number, since a cluster lies in one group of SMs (of seven CTAs with an
+// SM each, a B200 holds some 18).
+template <typename T, uint32_t TN>
+uint32_t few_clusters(uint32_t c) {
+    static std::mutex mu;
+    static uint32_t cache[64][9] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+        cudaGetLastError();
+        return 1;
+    }
+    std::lock_guard<std::mutex> lock(mu);
+    uint32_t& n = cache[dev][c];
+    if (n == 0) {
+        auto* k = mm8_few_kernel<T, TN>;
+        n = static_cast<uint32_t>(sm_count()) * Few<TN>::kPerSm / c;
+        if (set_max_dynamic_smem(reinterpret_cast<const void*>(k), Few<TN>::kSmem, "mm8_few_kernel") == HC_OK) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(c);
+            cfg.blockDim = dim3(Few<TN>::kThreads);
+            cfg.dynamicSmemBytes = Few<TN>::kSmem;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = c;
+            attr[0].val.clusterDim.y = 1;
+            attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            int active = 0;
+            if (cudaOccupancyMaxActiveClusters(&active, k, &cfg) == cudaSuccess && active > 0)
+                n = static_cast<uint32_t>(active);
+            else
+                cudaGetLastError();
+        }
+        if (n == 0) n = 1;
+    }
+    return n;
+}
+
+// Splits of K: the least time in K blocks (about 0.4 us each) of the busiest SM, with what a wave of
+// clusters costs besides: some three blocks to start, and to join the sums two more, five with over
+// 64 tokens.
 struct FewPlan {
     uint32_t splits;
-    uint64_t cost;  // K blocks of the busiest SM
+    uint64_t cost;
 };
-FewPlan few_plan(uint64_t tiles, uint32_t kb, uint32_t per_sm) {
-    const uint64_t sms = sm_count();
+template <typename T, uint32_t TN>
+FewPlan few_plan(const Params& p) {
+    const uint64_t tiles = static_cast<uint64_t>(p.nb) * ((p.M + TN - 1) / TN), sms = sm_count();
     FewPlan best{1, ~0ull};
-    for (uint32_t c = 1; c <= 8 && c <= kb; ++c) {
-        if (c > 1 && tiles * c > sms * per_sm) break;
-        const uint64_t cost = (tiles * c + sms - 1) / sms * ((kb + c - 1) / c) + (c > 1 ? 2 : 0);
+    for (uint32_t c = 1; c <= 8 && c <= p.kb; ++c) {
+        const uint64_t room = few_clusters<T, TN>(c), waves = (tiles + room - 1) / room;
+        if (c > 1 && waves > 1) break;
+        const uint64_t at_once = tiles < room ? tiles : room, per_sm = (at_once * c + sms - 1) / sms;
+        const uint64_t cost = waves * (per_sm * ((p.kb + c - 1) / c) + 3 + (c > 1 ? (TN > 64 ? 5 : 2) : 0));
         if (cost < best.cost) best = FewPlan{c, cost};
     }
     return best;
@@ -813,10 +857,9 @@ int launch_few(const Params& p, cudaStream_t s) {
     if (int rc = operand_map(&tmb, p.b, p.N, p.K, 128)) return rc;
     auto* k = mm8_few_kernel<T, TN>;
     if (int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(k), Few<TN>::kSmem, "mm8_few_kernel")) return rc;
-    const uint32_t token_tiles = (p.M + TN - 1) / TN;
-    const uint32_t splits = few_plan(static_cast<uint64_t>(p.nb) * token_tiles, p.kb, Few<TN>::kPerSm).splits;
+    const uint32_t splits = few_plan<T, TN>(p).splits;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(splits, p.nb, token_tiles);
+    cfg.gridDim = dim3(splits, p.nb, (p.M + TN - 1) / TN);
     cfg.blockDim = dim3(Few<TN>::kThreads);
     cfg.dynamicSmemBytes = Few<TN>::kSmem;
     cfg.stream = s;
@@ -848,13 +891,10 @@ int launch(Params p, cudaStream_t s) {
     const bool few_fits = p.nb <= 65535 && (p.M + 127) / 128 <= 65535;
     if (tiles > 0x7FFFFFFFull) return launch_simt<T>(p, s);
     p.num_tiles = static_cast<uint32_t>(tiles);
-    // Pairs where a busy SM has no more K blocks to go through than with 128-token tiles: a block costs
-    // both about the same time, 0.65 us (4096 x 4096 weight: M = 256 15.7 us against 24 in pairs, M = 512
-    // 24 either way, M = 1024 49 against 25).
-    const uint64_t pair_cost = pairs > 0 ? (tiles + pairs - 1) / pairs * p.kb : ~0ull;
-    if (pairs > 0 && (!few_fits || (p.M > 128 && pair_cost <= few_plan(static_cast<uint64_t>(p.nb) * ((p.M + 127) / 128),
-                                                                       p.kb, Few<128>::kPerSm).cost)))
-        return launch_pair<T>(p, pairs, s);
+    // Pairs where that takes no longer than 128-token tiles: a block costs both about the same time (4096 x
+    // 4096 weight: M = 256 15.7 us against 24 in pairs, M = 512 24 either way, M = 1024 49 against 25).
+    const uint64_t pair_cost = pairs > 0 ? (tiles + pairs - 1) / pairs * p.kb + 3 : ~0ull;
+    if (pairs > 0 && (!few_fits || (p.M > 128 && pair_cost <= few_plan<T, 128>(p).cost))) return launch_pair<T>(p, pairs, s);
     if (!few_fits) return launch_simt<T>(p, s);
     if (p.M <= 16) return launch_few<T, 16>(p, s);
     if (p.M <= 32) return launch_few<T, 32>(p, s);
