@@ -891,9 +891,10 @@ int launch(Params p, cudaStream_t s) {
     const bool few_fits = p.nb <= 65535 && (p.M + 127) / 128 <= 65535;
     if (tiles > 0x7FFFFFFFull) return launch_simt<T>(p, s);
     p.num_tiles = static_cast<uint32_t>(tiles);
-    // Pairs where that takes no longer than 128-token tiles: a block costs both about the same time (4096 x
-    // 4096 weight: M = 256 15.7 us against 24 in pairs, M = 512 24 either way, M = 1024 49 against 25).
-    const uint64_t pair_cost = pairs > 0 ? (tiles + pairs - 1) / pairs * p.kb + 3 : ~0ull;
+    // Pairs where that takes no longer than 128-token tiles: a block costs both about the same time, starting
+    // and draining a 256 x 256 tile some eight (4096 x 4096 weight: M = 256 15.7 us against 24 in
+    // pairs, M = 512 24 either way, M = 1024 49 against 25; 1467 x 793 x 1328 11.9 against 15.3).
+    const uint64_t pair_cost = pairs > 0 ? (tiles + pairs - 1) / pairs * p.kb + 8 : ~0ull;
     if (pairs > 0 && (!few_fits || (p.M > 128 && pair_cost <= few_plan<T, 128>(p).cost))) return launch_pair<T>(p, pairs, s);
     if (!few_fits) return launch_simt<T>(p, s);
     if (p.M <= 16) return launch_few<T, 16>(p, s);
