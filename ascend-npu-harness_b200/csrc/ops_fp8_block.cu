@@ -15,6 +15,7 @@
 #include "fp8_block.cuh"
 #include "hc_device.cuh"
 #include "hc_internal.h"
+#include "overlap.cuh"
 
 namespace hc {
 namespace {
@@ -79,6 +80,7 @@ __global__ void __launch_bounds__(kThreads) block_fwd_kernel(const T* __restrict
                                                              uint8_t* __restrict__ q, float* __restrict__ scale,
                                                              uint32_t blocks, const BlockMap map,
                                                              typename ActOf<T>::Op op) {
+    overlap_begin();
     constexpr int kAnyUnroll = kAnyFwd;
     const uint32_t lane = threadIdx.x & 31;
     const uint32_t b0 = (blockIdx.x * kAnyWarps + threadIdx.x / 32) * kAnyUnroll;
@@ -122,6 +124,7 @@ template <typename T, bool HasAct>
 __global__ void __launch_bounds__(kThreads) block_bwd_kernel(const T* __restrict__ dy, const uint8_t* __restrict__ q,
                                                              const float* __restrict__ scale, T* __restrict__ out,
                                                              uint32_t blocks, const BlockMap map, ActSlope slope) {
+    overlap_begin();
     constexpr int kAnyUnroll = kAnyBwd;
     const uint32_t lane = threadIdx.x & 31;
     const uint32_t b0 = (blockIdx.x * kAnyWarps + threadIdx.x / 32) * kAnyUnroll;
@@ -208,6 +211,7 @@ __global__ void __launch_bounds__(kThreads) block_fwd_vec_kernel(const T* __rest
                                                                  uint8_t* __restrict__ q, float* __restrict__ scale,
                                                                  uint32_t blocks, const BlockMap map,
                                                                  typename ActOf<T>::Op op) {
+    overlap_begin();
     using V = Vec<T>;
     const uint32_t gl = threadIdx.x % V::G, c = gl * V::P;
     const uint32_t b0 = blockIdx.x * V::kPerCta + threadIdx.x / V::G;
@@ -261,6 +265,7 @@ __global__ void __launch_bounds__(kThreads) block_bwd_vec_kernel(const T* __rest
                                                                  const float* __restrict__ scale, T* __restrict__ out,
                                                                  uint32_t blocks, const BlockMap map,
                                                                  ActSlope slope) {
+    overlap_begin();
     using V = Vec<T>;
     const uint32_t c = threadIdx.x % V::G * V::P;
     const uint32_t b0 = blockIdx.x * V::kPerCta + threadIdx.x / V::G;
@@ -309,6 +314,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) tile_quant_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
                                                               float* __restrict__ scale, uint32_t rows, uint32_t cols,
                                                               uint32_t col_tiles, uint64_t tiles) {
+    overlap_begin();
     __shared__ uint32_t part[kThreads / 32];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     for (uint64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
@@ -340,6 +346,7 @@ __global__ void __launch_bounds__(kThreads) tile_dequant_kernel(const uint8_t* _
                                                                 const float* __restrict__ scale, T* __restrict__ x,
                                                                 uint32_t rows, uint32_t cols, uint32_t col_tiles,
                                                                 uint64_t tiles) {
+    overlap_begin();
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     for (uint64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
         const uint32_t r0 = static_cast<uint32_t>(t / col_tiles) * kFp8Block;
@@ -388,13 +395,13 @@ int launch_fwd(const void* x, void* y, void* q, float* scale, uint32_t rows, uin
     if (blocks > kMaxBlocks) return fail(HC_ERR_UNSUPPORTED, "%s: too many blocks", name);
     if (vec_ok<T>(x, HasAct ? y : x, q, cols)) {
         const unsigned grid = static_cast<unsigned>((blocks + Vec<T>::kPerCta - 1) / Vec<T>::kPerCta);
-        block_fwd_vec_kernel<T, HasAct><<<grid, kThreads, 0, s>>>(static_cast<const T*>(x), static_cast<T*>(y),
+        launch_overlapped(block_fwd_vec_kernel<T, HasAct>, grid, kThreads, 0, 0, s, static_cast<const T*>(x), static_cast<T*>(y),
                                                                   static_cast<uint8_t*>(q), scale,
                                                                   static_cast<uint32_t>(blocks), block_map(cols, nb), op);
         return check_launch(name);
     }
     const unsigned grid = static_cast<unsigned>((blocks + kAnyWarps * kAnyFwd - 1) / (kAnyWarps * kAnyFwd));
-    block_fwd_kernel<T, HasAct><<<grid, kThreads, 0, s>>>(static_cast<const T*>(x), static_cast<T*>(y),
+    launch_overlapped(block_fwd_kernel<T, HasAct>, grid, kThreads, 0, 0, s, static_cast<const T*>(x), static_cast<T*>(y),
                                                           static_cast<uint8_t*>(q), scale, static_cast<uint32_t>(blocks),
                                                           block_map(cols, nb), op);
     return check_launch(name);
@@ -409,13 +416,13 @@ int launch_bwd(const void* dy, const void* q, const float* scale, void* out, uin
     if (blocks > kMaxBlocks) return fail(HC_ERR_UNSUPPORTED, "%s: too many blocks", name);
     if (vec_ok<T>(out, HasAct ? dy : out, q, cols)) {
         const unsigned grid = static_cast<unsigned>((blocks + Vec<T>::kPerCta - 1) / Vec<T>::kPerCta);
-        block_bwd_vec_kernel<T, HasAct><<<grid, kThreads, 0, s>>>(static_cast<const T*>(dy), static_cast<const uint8_t*>(q),
+        launch_overlapped(block_bwd_vec_kernel<T, HasAct>, grid, kThreads, 0, 0, s, static_cast<const T*>(dy), static_cast<const uint8_t*>(q),
                                                                   scale, static_cast<T*>(out),
                                                                   static_cast<uint32_t>(blocks), block_map(cols, nb), slope);
         return check_launch(name);
     }
     const unsigned grid = static_cast<unsigned>((blocks + kAnyWarps * kAnyBwd - 1) / (kAnyWarps * kAnyBwd));
-    block_bwd_kernel<T, HasAct><<<grid, kThreads, 0, s>>>(static_cast<const T*>(dy), static_cast<const uint8_t*>(q), scale,
+    launch_overlapped(block_bwd_kernel<T, HasAct>, grid, kThreads, 0, 0, s, static_cast<const T*>(dy), static_cast<const uint8_t*>(q), scale,
                                                           static_cast<T*>(out), static_cast<uint32_t>(blocks),
                                                           block_map(cols, nb), slope);
     return check_launch(name);
@@ -428,7 +435,7 @@ int launch_quant(const void* x, void* q, float* scale, const fp8_block_tiling_da
     const uint32_t ct = (t->cols + kFp8Block - 1) / kFp8Block;
     const uint64_t tiles = static_cast<uint64_t>((t->rows + kFp8Block - 1) / kFp8Block) * ct;
     auto* k = tile_quant_kernel<T>;
-    k<<<grid_of(k, tiles, 1), kThreads, 0, s>>>(static_cast<const T*>(x), static_cast<uint8_t*>(q), scale, t->rows,
+    launch_overlapped(k, grid_of(k, tiles, 1), kThreads, 0, 0, s, static_cast<const T*>(x), static_cast<uint8_t*>(q), scale, t->rows,
                                                 t->cols, ct, tiles);
     return check_launch("quantize_fp8_block");
 }
@@ -440,7 +447,7 @@ int launch_dequant(const void* q, const float* scale, void* x, const fp8_block_t
     const uint32_t ct = (t->cols + kFp8Block - 1) / kFp8Block;
     const uint64_t tiles = static_cast<uint64_t>((t->rows + kFp8Block - 1) / kFp8Block) * ct;
     auto* k = tile_dequant_kernel<T>;
-    k<<<grid_of(k, tiles, 1), kThreads, 0, s>>>(static_cast<const uint8_t*>(q), scale, static_cast<T*>(x), t->rows,
+    launch_overlapped(k, grid_of(k, tiles, 1), kThreads, 0, 0, s, static_cast<const uint8_t*>(q), scale, static_cast<T*>(x), t->rows,
                                                 t->cols, ct, tiles);
     return check_launch("dequantize_fp8_block");
 }

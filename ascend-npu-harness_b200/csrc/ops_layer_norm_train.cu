@@ -18,6 +18,7 @@
 #include "fp8_block.cuh"
 #include "hc_device.cuh"
 #include "hc_internal.h"
+#include "overlap.cuh"
 
 namespace hc {
 namespace {
@@ -71,6 +72,7 @@ __device__ __forceinline__ float cta_sum(float v, float* sh) {
 // ---------------------------------------------------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(kThreads) ln_fwd_any_kernel(const FwdArgs a) {
+    overlap_begin();
     __shared__ float sh[kWarps];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     const float H = static_cast<float>(a.H);
@@ -124,6 +126,7 @@ __device__ __forceinline__ float xhat_at(const BwdArgs& a, uint64_t row, uint32_
 
 template <typename T, bool Ckpt>
 __global__ void __launch_bounds__(kThreads) ln_bwd_dx_any_kernel(const BwdArgs a) {
+    overlap_begin();
     __shared__ float sh[kWarps];
     const float H = static_cast<float>(a.H);
     for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -147,6 +150,7 @@ __global__ void __launch_bounds__(kThreads) ln_bwd_dx_any_kernel(const BwdArgs a
 // Partial dgamma and dbeta: a CTA takes 32 columns and one part's rows, a warp every 8th of them.
 template <typename T, bool Ckpt>
 __global__ void __launch_bounds__(kThreads) ln_bwd_cols_any_kernel(const BwdArgs a) {
+    overlap_begin();
     __shared__ float sg[kWarps][32], sb[kWarps][32];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     const uint32_t c = blockIdx.x * 32 + lane, part = blockIdx.y;
@@ -173,7 +177,7 @@ __global__ void __launch_bounds__(kThreads) ln_bwd_cols_any_kernel(const BwdArgs
 }
 
 // dgamma and dbeta from the partial rows, always added in the same order: a warp per 32nd partial row, its
-// loads all under way at once.  Launched to start while the kernel before drains.
+// loads all under way at once.
 constexpr int kJoinWarps = 32;
 __global__ void __launch_bounds__(32 * kJoinWarps) ln_bwd_join_kernel(const float* __restrict__ parts, uint32_t parts_n,
                                                                       uint32_t H, float* __restrict__ dgamma,
@@ -181,7 +185,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) ln_bwd_join_kernel(const floa
     __shared__ float sh[kJoinWarps][33];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     const uint32_t c = blockIdx.x * 32 + lane;
-    cudaGridDependencySynchronize();
+    overlap_begin();
     float v[(kMaxParts + kJoinWarps - 1) / kJoinWarps];
     constexpr int N = sizeof(v) / sizeof(v[0]);
 #pragma unroll
@@ -383,6 +387,7 @@ __device__ __forceinline__ float lanes_sum(float v) {
 // barrier, M2 = sum_w M2_w + n_w (mean_w - mean)^2, which is as exact as two passes over the row.
 template <typename T, int W, bool Vec, bool Ckpt>
 __global__ void __launch_bounds__(group_threads(W), W <= 8 ? 3 : 1) ln_fwd_row_kernel(const FwdArgs a) {
+    overlap_begin();
     using Row = RowPart<T, W, Vec>;
     constexpr int G = row_groups(W), P = Row::P;
     __shared__ float2 sh[G][2][W];
@@ -550,6 +555,7 @@ struct CkptPart {
 // registers over all its rows, joined over the CTA's row groups at the end.
 template <typename T, int W, bool Vec, bool Ckpt>
 __global__ void __launch_bounds__(group_threads(W), bwd_ctas(W)) ln_bwd_row_kernel(const BwdArgs a) {
+    overlap_begin();
     using Row = RowPart<T, W, Vec>;
     using Part = typename std::conditional<Ckpt, CkptPart<W, Vec, Row::P>, Row>::type;
     using Ring = BwdRing<T, W, Ckpt>;
@@ -670,7 +676,6 @@ __global__ void __launch_bounds__(group_threads(W), bwd_ctas(W)) ln_bwd_row_kern
             g[i] = __fmul2_rn(__ffma2_rn(xh[i], c2, __fadd2_rn(g[i], c1)), f2(rstd));
         Row::store(dx, g, t, a.H);
     }
-    cudaTriggerProgrammaticLaunchCompletion();  // the join may be set up now; it waits for the sums
     float* to_gamma = a.sum_gamma + static_cast<uint64_t>(blockIdx.x) * 2 * a.H;
     float* to_beta = a.sum_beta + static_cast<uint64_t>(blockIdx.x) * 2 * a.H;
     if constexpr (G > 1) {  // [group][dgamma, dbeta][pair][t]
@@ -734,7 +739,7 @@ int launch_fwd_rows(const FwdArgs& a, cudaStream_t s) {
         auto* k = ln_fwd_row_kernel<T, W, Vec, Ckpt>;
         const uint64_t groups = (static_cast<uint64_t>(a.rows) + row_groups(W) - 1) / row_groups(W);
         const uint64_t cap = static_cast<uint64_t>(resident_blocks(reinterpret_cast<const void*>(k), group_threads(W), 0));
-        k<<<static_cast<unsigned>(groups < cap ? groups : (cap ? cap : 1)), group_threads(W), 0, s>>>(a);
+        launch_overlapped(k, static_cast<unsigned>(groups < cap ? groups : (cap ? cap : 1)), group_threads(W), 0, 0, s, a);
         return check_launch("layer_norm_fwd_train");
     });
 }
@@ -747,7 +752,7 @@ int launch_fwd(const FwdArgs& a, cudaStream_t s) {
         return a.q ? launch_fwd_rows<T, false, true>(a, s) : launch_fwd_rows<T, false, false>(a, s);
     }
     auto* k = ln_fwd_any_kernel<T>;
-    k<<<row_grid(reinterpret_cast<const void*>(k), a.rows), kThreads, 0, s>>>(a);
+    launch_overlapped(k, row_grid(reinterpret_cast<const void*>(k), a.rows), kThreads, 0, 0, s, a);
     return check_launch("layer_norm_fwd_train");
 }
 
@@ -771,7 +776,7 @@ int launch_bwd_rows(BwdArgs& a, float* dgamma, float* dbeta, cudaStream_t s) {
         constexpr size_t ring = Vec ? BwdRing<T, W, Ckpt>::kBytes : 0, smem = ring > sums ? ring : sums;
         auto* k = ln_bwd_row_kernel<T, W, Vec, Ckpt>;
         if (int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(k), smem, "ln_bwd_row_kernel")) return rc;
-        k<<<a.parts_n, group_threads(W), smem, s>>>(a);
+        launch_overlapped(k, a.parts_n, group_threads(W), smem, 0, s, a);
         return check_launch("layer_norm_bwd");
     });
 }
@@ -789,21 +794,13 @@ int launch_bwd(BwdArgs a, float* dgamma, float* dbeta, cudaStream_t s) {
         a.rows_per_part = (a.rows + parts_of(a.rows) - 1) / parts_of(a.rows);
         a.parts_n = (a.rows + a.rows_per_part - 1) / a.rows_per_part;
         auto* k = ln_bwd_dx_any_kernel<T, Ckpt>;
-        k<<<row_grid(reinterpret_cast<const void*>(k), a.rows), kThreads, 0, s>>>(a);
+        launch_overlapped(k, row_grid(reinterpret_cast<const void*>(k), a.rows), kThreads, 0, 0, s, a);
         if (int rc = check_launch("layer_norm_bwd")) return rc;
-        ln_bwd_cols_any_kernel<T, Ckpt><<<dim3((a.H + 31) / 32, a.parts_n), kThreads, 0, s>>>(a);
+        launch_overlapped(ln_bwd_cols_any_kernel<T, Ckpt>, dim3((a.H + 31) / 32, a.parts_n), kThreads, 0, 0, s, a);
         if (int rc = check_launch("layer_norm_bwd")) return rc;
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((a.H + 31) / 32, 2);
-    cfg.blockDim = dim3(32 * kJoinWarps);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, ln_bwd_join_kernel, const_cast<const float*>(a.parts), a.parts_n, a.H, dgamma, dbeta);
+    launch_overlapped(ln_bwd_join_kernel, dim3((a.H + 31) / 32, 2), 32 * kJoinWarps, 0, 0, s,
+                      const_cast<const float*>(a.parts), a.parts_n, a.H, dgamma, dbeta);
     return check_launch("layer_norm_bwd");
 }
 

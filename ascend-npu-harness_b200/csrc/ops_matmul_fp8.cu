@@ -26,6 +26,7 @@
 #include "fp8_block.cuh"
 #include "hc_device.cuh"
 #include "hc_internal.h"
+#include "overlap.cuh"
 #include "sm100.cuh"
 #include "tmap.h"
 
@@ -219,6 +220,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     tc_fence_before();
     cluster_sync_all();  // both CTAs' barriers are initialised before either signals the other
     tc_fence_after();
+    overlap_begin();
     const uint32_t tmem_base = *tmem_slot;
     const uint32_t s_base = smem_u32(smem);
 
@@ -478,6 +480,7 @@ __global__ void __launch_bounds__(Few<TN>::kThreads, Few<TN>::kPerSm)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    overlap_begin();
     const uint32_t tmem_base = *tmem_slot;
     const uint32_t s_base = smem_u32(smem);
 
@@ -671,6 +674,7 @@ __global__ void __launch_bounds__(Few<TN>::kThreads, Few<TN>::kPerSm)
 
 template <typename T>
 __global__ void __launch_bounds__(256) mm8_simt_kernel(const Params p) {
+    overlap_begin();
     __shared__ float As[16][64 + 1];
     __shared__ float Bs[16][64 + 1];
     const uint32_t tx = threadIdx.x % 16, ty = threadIdx.x / 16;
@@ -735,7 +739,7 @@ template <typename T>
 int launch_simt(const Params& p, cudaStream_t s) {
     const uint64_t mt = (static_cast<uint64_t>(p.M) + 63) / 64;
     const dim3 grid(static_cast<unsigned>((static_cast<uint64_t>(p.N) + 63) / 64), mt < 65535 ? static_cast<unsigned>(mt) : 65535);
-    mm8_simt_kernel<T><<<grid, 256, 0, s>>>(p);
+    launch_overlapped(mm8_simt_kernel<T>, grid, 256, 0, 0, s, p);
     t_last_path = 2;
     return check_launch("mm8_simt_kernel");
 }
@@ -784,7 +788,7 @@ int launch_pair(Params p, int pairs, cudaStream_t s) {
     auto* k = mm8_pair_kernel<T>;
     if (int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(k), kPairSmem, "mm8_pair_kernel")) return rc;
     const uint32_t clusters = static_cast<uint32_t>(pairs) < p.num_tiles ? static_cast<uint32_t>(pairs) : p.num_tiles;
-    k<<<2 * clusters, kPairThreads, kPairSmem, s>>>(tma, tmb, p);
+    launch_overlapped(k, 2 * clusters, kPairThreads, kPairSmem, 0, s, tma, tmb, p);
     t_last_path = 3;
     return check_launch("mm8_pair_kernel");
 }
@@ -858,19 +862,8 @@ int launch_few(const Params& p, cudaStream_t s) {
     auto* k = mm8_few_kernel<T, TN>;
     if (int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(k), Few<TN>::kSmem, "mm8_few_kernel")) return rc;
     const uint32_t splits = few_plan<T, TN>(p).splits;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(splits, p.nb, (p.M + TN - 1) / TN);
-    cfg.blockDim = dim3(Few<TN>::kThreads);
-    cfg.dynamicSmemBytes = Few<TN>::kSmem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = splits;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, k, tma, tmb, p, splits);
+    launch_overlapped(k, dim3(splits, p.nb, (p.M + TN - 1) / TN), Few<TN>::kThreads, Few<TN>::kSmem, splits, s, tma, tmb, p,
+                      splits);
     t_last_path = 1;
     return check_launch("mm8_few_kernel");
 }
