@@ -8,7 +8,10 @@
 //   ..._ckpt_bwd               (dy, q, scale) -> dx = dy * act'(q * scale)
 //
 // All are HBM streams: per element the forward moves 2 e + 1 + 1/32 bytes (e = element size) and
-// the backward the same, against ~10 flops and two special-function calls.
+// the backward the same, against ~10 flops and two special-function calls.  Measured on one B200, copy
+// rate 6.56 TB/s: [16384, 4096] bf16 (338 MB) forward 52 us, backward 53 us (6.4-6.5 TB/s, 98 %); fp32
+// (606 MB) 102 and 89 us; quantise 33 us (6.1 TB/s).  Rows that are not whole 16-byte packs run at about
+// half of that ([8192, 4001] bf16: 46 us either way), held back by one- and two-byte accesses.
 #include <cuda_runtime.h>
 
 #include "activation.cuh"

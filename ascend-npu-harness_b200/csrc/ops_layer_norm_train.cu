@@ -9,8 +9,17 @@
 // xh comes from x, mean and rstd, or from the checkpoint (q * scale), which needs rstd only: the
 // 8-bit form keeps xh and not x, whose offset would cost it precision.
 //
-// Statistics and sums are fp32.  The mean is taken over deviations from the row's first element and
-// the variance over deviations from the mean, as in the forward-only kernels.
+// Statistics and sums are fp32.  The mean is taken over deviations from an element of the row and the
+// variance over deviations from the mean, as in the forward-only kernels.
+//
+// Both directions are HBM streams: the forward moves 2 e bytes per element (e = element size) and 1 + 1/32 more
+// for the checkpoint, the backward 3 e, or 2 e + 1 + 1/32 from the checkpoint.  Measured on one B200, copy rate 6.56 TB/s:
+//   [16384, 4096] bf16   forward 53 us (5.1 TB/s, 77 %), gradients 80 us (5.0 TB/s; their kernel alone
+//                        75 us, 82 %, the join of the partial sums the rest)
+//   [8192, 4096] fp32    forward 44 us (6.1 TB/s), gradients 67 us (6.0 TB/s)
+//   [8192, 8192] bf16    with the checkpoint: forward 73 us, gradients 83 us (4.1 TB/s)
+// 16-bit rows are bound by issue slots and shared-memory traffic per element (issue 43-54 % active, 14-17
+// warp instructions per 32 elements), not by DRAM: fp32 rows, with half the elements per byte, run at 92 %.
 #include <cuda_runtime.h>
 
 #include <algorithm>

@@ -56,8 +56,8 @@ struct Params {
     uint32_t M, N, K, kb;  // kb = ceil(K / 128)
     uint32_t nb;           // ceil(N / 128)
     uint32_t tiles_m, tiles_n, num_tiles;
-    uint32_t vec_store;    // rows of C are whole 16-byte packs on 16-byte boundaries
-    uint32_t word_store;   // ... whole 4-byte words on 4-byte boundaries
+    uint32_t vec_store;    // rows of C are whole 16-byte packs on 16-byte boundaries (few-token kernel)
+    uint32_t word_store;   // ... whole 4-byte words on 4-byte boundaries (pairs)
 };
 
 // K blocks are 128 e4m3 bytes deep: one swizzle row, one scale.
@@ -74,16 +74,19 @@ constexpr uint32_t kPanel = 128 * kBK;  // 16 KB: 128 rows of either operand
 //               memory per block instead of 64, and 128 B/cycle make that 640 cycles instead of 512
 //   warps 2-3   products of the scales for eight K blocks at a time into shared memory: read by the
 //               promoting threads themselves (32 rows, 32 lines each) they cost a third of the time
-//   warps 4-11  promotion: warp w reads TMEM lanes 32 (w % 4) .. + 31 (thread = row) and 128 columns, one
-//               128-block of N: 128 running sums per thread, one multiply-add each (as f32x2 pairs)
-//               with one product of scales per block, the next 32 columns on their way meanwhile.
-//               Registers: 72 / 216 per thread of the two kinds of warps (4 x 32 x 72 + 8 x 32 x 216
-//               = 384 x 168, what the block is launched with).  Sixteen warps of 64 columns spent more
-//               on waits than on sums.
+//   warps 4-19  promotion: warp w reads TMEM lanes 32 (w % 4) .. + 31 (thread = row) and 64 columns, half of
+//               a 128-block of N: 64 running sums per thread, one multiply-add each (as f32x2 pairs)
+//               with one product of scales per block.  Registers: 64 / 104 per thread of the two kinds
+//               of warps (4 x 32 x 64 + 16 x 32 x 104 = 640 x 96, what the block is launched with).
+//               Eight warps of 128 columns, with the next 32 on their way meanwhile, are as fast on
+//               8192^3 and up to 10 % slower on smaller products, where waits count more than power.
 // "Accumulator read" goes straight to the even CTA's barrier with a release at CTA scope (no data in
 // memory hangs on it: the TMEM reads are complete and ordered by the tcgen05 fences); a release
 // at cluster scope takes about 1000 cycles here, several times the block itself.
-// A block costs the tensor core 512 cycles (256 x 256 x 128 products at 2 x 8192 per cycle).
+// A block costs the tensor core 512 cycles (256 x 256 x 128 products at 2 x 8192 per cycle) and takes about
+// 1050: tensor pipe 47 % active, issue slots 58 % (4096^3).  Reading and promoting 256 x 256 sums per
+// block is what a scale for each 128 costs.  8192^3 to bf16: 515 us (2.13 PFLOP/s) from a cool start, 600 us
+// sustained, where the power cap holds the clock at 1.52 GHz; 4096^3: 79 us.
 // ======================================================================================
 constexpr uint32_t kPairStages = 6;
 constexpr uint32_t kPairEpiWarps = 16;
@@ -408,6 +411,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 // as the N operand and every S-th run of K blocks; the S CTAs of a cluster then add their sums in
 // rank order through distributed shared memory.  Reading the weight is the work (N K bytes), so S is
 // chosen to give every SM a part of it, and the ring holds all that fits beside a second CTA.
+// 1 x 4096 x 4096: 6.2 us with the weight in hand after 3.6 (6.8 TB/s once loads run; 1.2 us to the first
+// block, 2 us for the join); 1 x 8192 x 8192: 17 us (67 MB, 4.0 TB/s); 77 x 10001 x 2064: 13 us.
 //   warp 0      TMA producer: 16 KB of weight and TN x 128 bytes of tokens per K block
 //   warp 1      issues M=128, N=TN, K=32 MMAs into one of kAcc accumulators of TN columns
 //   warps 2 on  promotion, kEpi = 4 or 8 warps: thread = weight row (TMEM lane), kCols of the tokens:

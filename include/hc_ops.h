@@ -317,7 +317,8 @@ struct matmul_fp8_block_tiling_data {
 /* C[M,N] = A . B^T + bias for a linear layer with 8-bit blocks: a [M,K] with a_scale
  * [M, ceil(K/128)] (blockRows 1), b [N,K] with b_scale [ceil(N/128), ceil(K/128)] (blockRows 128),
  * bias [N] of C's type or NULL, C of type `dtype` (F32, F16 or BF16), fp32 sums, one rounding.
- * K >= 1.  The gradient to A is the same call with the transposed weight and its transposed
+ * K >= 1.  K a multiple of 16 with 16-byte aligned a and b -> tcgen05 kernels; otherwise a SIMT
+ * kernel.  The gradient to A is the same call with the transposed weight and its transposed
  * scales. */
 int hc_matmul_fp8_block_launch(const void* a, const float* a_scale, const void* b, const float* b_scale,
                                const void* bias, void* c, const struct matmul_fp8_block_tiling_data* t, int dtype,
