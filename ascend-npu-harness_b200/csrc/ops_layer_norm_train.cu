@@ -248,6 +248,8 @@ struct RowPart {
     using Raw = typename std::conditional<Vec, uint4, T>::type;
     Raw r[N];
     __device__ __forceinline__ static uint32_t first(uint32_t t, int i) { return Vec ? (t + 32 * W * i) * P : t + 32 * W * i; }
+    // column of the thread's j-th element, or of the load that brings it (which is in or out as a whole)
+    __device__ __forceinline__ static uint32_t column(uint32_t t, int j) { return first(t, j / kRun); }
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < N; ++i) r[i] = Raw{};
@@ -671,7 +673,11 @@ __global__ void __launch_bounds__(group_threads(W), bwd_ctas(W)) ln_bwd_row_kern
         float2 s1 = f2(0.f), s2 = f2(0.f);
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
-            if constexpr (!Ckpt) xh[i] = __fmul2_rn(__fadd2_rn(xh[i], f2(-mean)), f2(rstd));  // meets g = 0 behind the end
+            if constexpr (!Ckpt) {
+                // zero behind the end: mean * rstd may overflow there, and infinity spoils even g = 0
+                const float2 r = make_float2(Row::column(t, 2 * i) < a.H ? rstd : 0.f, Row::column(t, 2 * i + 1) < a.H ? rstd : 0.f);
+                xh[i] = __fmul2_rn(__fadd2_rn(xh[i], f2(-mean)), r);
+            }
             dgamma[i] = __ffma2_rn(g[i], xh[i], dgamma[i]);
             dbeta[i] = __fadd2_rn(dbeta[i], g[i]);
             g[i] = __fmul2_rn(g[i], gamma[i]);

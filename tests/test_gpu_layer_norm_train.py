@@ -144,6 +144,23 @@ def test_constant_and_nonfinite_rows(cuda, H):
     assert bool(dx[:3].isfinite().all()) and bool(dx[3:].isnan().all())
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("H", [5, 37, 136, 1000, 1001, 2056, 6000])
+def test_constant_rows_of_large_values(cuda, H, kind):
+    """mean * rstd above the largest fp32: x - mean is zero, and so is xh.  Rows that leave some of their
+    threads' columns unused take no part of what those would compute."""
+    _, gamma, beta, dy = inputs((6, H), kind)
+    x = torch.full((6, H), 1e36, dtype=R.DTYPES[kind], device="cuda")
+    y, mean, rstd = hc.layer_norm_fwd_train(x, gamma, beta, 1e-12)
+    assert torch.equal(mean, x[:, 0].float()) and torch.equal(y, beta.to(y.dtype).expand_as(y))
+    assert bool((mean * rstd).isinf().all())
+    xh, r = torch.zeros(6, H, dtype=torch.float64, device="cuda"), rstd.double()[:, None]
+    ref = R.layer_norm_grads(dy, xh, r, gamma)
+    bounds = R.layer_norm_grad_bounds(dy, xh, xh, r, gamma)
+    for name, got, want, bound in zip(("dx", "dgamma", "dbeta"), hc.layer_norm_bwd(dy, x, gamma, mean, rstd), ref, bounds):
+        R.assert_within(got, want, bound, name)
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_unaligned_buffers(cuda, kind):
     """Contiguous views that start off a 16-byte boundary."""
