@@ -344,7 +344,8 @@ int hc_activation_gelu_silu_ckpt_bwd_launch(const void* dy, const void* q, const
                                             void* stream);
 
 /* ------------------------------------------------------------------------------------------
- * Layer norm for training (no counterpart in the reference, whose ladder is forward only).
+ * Layer norm for training (no counterpart in the reference, whose ladder is forward only).  Dense
+ * buffers; outputs must not overlap inputs or each other.
  * ---------------------------------------------------------------------------------------- */
 
 /* The layer norm of x [rows, lastDim] with the statistics its backward needs: y, mean [rows] (may
