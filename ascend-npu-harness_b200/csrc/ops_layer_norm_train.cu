@@ -18,6 +18,8 @@
 //                        75 us, 82 %, the join of the partial sums the rest)
 //   [8192, 4096] fp32    forward 44 us (6.1 TB/s), gradients 67 us (6.0 TB/s)
 //   [8192, 8192] bf16    with the checkpoint: forward 73 us, gradients 83 us (4.1 TB/s)
+//   [8192, 4001] bf16    (rows that are not whole packs) forward 43 us, gradients 72 us (2.7 TB/s); with the
+//                        checkpoint 63 and 70 us
 // 16-bit rows are bound by issue slots and shared-memory traffic per element (issue 43-54 % active, 14-17
 // warp instructions per 32 elements), not by DRAM: fp32 rows, with half the elements per byte, run at 92 %.
 #include <cuda_runtime.h>
@@ -221,7 +223,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) ln_bwd_join_kernel(const floa
 // neighbouring lanes hold a block of 128 and its maximum is a shuffle tree.  In the backward each thread
 // copies its own packs into a ring in shared memory with cp.async and waits for its own copies
 // alone: no barrier and no registers, which the weight gradients need.
-// Other rows: thread t holds elements t + 32 W i, the next row's in registers.
+// Other rows: thread t holds elements t + 32 W i; the next row's in registers where these suffice.
 // Columns behind the row's end hold zeros and are not stored.
 // ---------------------------------------------------------------------------------------
 constexpr int kCpt = 16;
@@ -381,9 +383,14 @@ __device__ __forceinline__ float2 row_sum2(float2 v, float2* sh, uint32_t group,
     return v;
 }
 
-constexpr int bwd_ctas(int W) { return W <= 8 ? 2 : 1; }
+// Rows loaded one element at a time: whether the next row is held in registers, which leaves room for
+// one CTA per SM without spills; otherwise two, which wait for each row.  x form, bf16: [16384, 2001] 76 us with, 109
+// without; [32768, 1001] 74 and 89; [8192, 4001] 100 and 72; [4096, 7777] 97 and 90.  Checkpoint: 77 and 120 at
+// [16384, 2001], 97 and 70 at [8192, 4001].
+constexpr bool bwd_ahead(int W) { return W <= 4; }
+constexpr int bwd_ctas(int W, bool vec) { return W > 8 || (!vec && bwd_ahead(W)) ? 1 : 2; }
 template <typename T, int W, bool Ckpt>
-using BwdRing = RingShape<T, group_threads(W), bwd_ctas(W), Ckpt>;
+using BwdRing = RingShape<T, group_threads(W), bwd_ctas(W, true), Ckpt>;
 
 // Sum over each run of W lanes.
 template <int W>
@@ -393,11 +400,15 @@ __device__ __forceinline__ float lanes_sum(float v) {
     return v;
 }
 
+// CTAs per SM that the registers are divided for.  Rows loaded one element at a time hold the next row in
+// 16 registers instead of 8 and spilled with three ([8192, 4001] bf16: 55 us with three, 43 with two).
+constexpr int fwd_ctas(int W, bool vec) { return W > 8 ? 1 : vec ? 3 : 2; }
+
 // Statistics: each warp takes the mean of its own columns (over deviations from its first one) and its
 // sum of squares around that, with shuffles alone; the row's follow from the W pairs behind one
 // barrier, M2 = sum_w M2_w + n_w (mean_w - mean)^2, which is as exact as two passes over the row.
 template <typename T, int W, bool Vec, bool Ckpt>
-__global__ void __launch_bounds__(group_threads(W), W <= 8 ? 3 : 1) ln_fwd_row_kernel(const FwdArgs a) {
+__global__ void __launch_bounds__(group_threads(W), fwd_ctas(W, Vec)) ln_fwd_row_kernel(const FwdArgs a) {
     overlap_begin();
     using Row = RowPart<T, W, Vec>;
     constexpr int G = row_groups(W), P = Row::P;
@@ -511,16 +522,22 @@ __global__ void __launch_bounds__(group_threads(W), W <= 8 ? 3 : 1) ln_fwd_row_k
             }
             if (W == 1) __syncwarp();
             else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * W) : "memory");
+            // the quotients of the warp's 16 columns in one division: lane 2 i takes 448 / amax of column i's
+            // block, lane 2 i + 1 its scale and stores it (every lane computing its own: 118 us at
+            // [8192, 4001] bf16; shuffling the scales, too, and encoding one column at a time: 85; now 63)
+            const uint4 m = *reinterpret_cast<const uint4*>(&quarter[group][(W * (t % 32 / 2) + wir) / 4 * 4]);
+            const float amax = fp8_amax(max(max(m.x, m.y), max(m.z, m.w)));
+            const float ratio = __fdiv_rn(t & 1 ? amax : kFp8Max, t & 1 ? kFp8Max : amax);
+            const uint32_t c0 = 32 * wir + 32 * W * (t % 32 / 2);  // the warp's first column of them
+            if ((t & 1) && c0 % kFp8Block == 0 && c0 < a.H) a.scale[row * a.row_blocks + c0 / kFp8Block] = ratio;
+            uint8_t* q = a.q + row * a.H;
 #pragma unroll
-            for (int i = 0; i < kCpt; ++i) {
-                const uint32_t b = (W * i + wir) / 4;
-                const uint4 m = *reinterpret_cast<const uint4*>(&quarter[group][b * 4]);
-                float inv, sc;
-                fp8_block_scale(max(max(m.x, m.y), max(m.z, m.w)), inv, sc);
-                const uint32_t c = Row::first(t, i);
-                if (c >= a.H) continue;
-                if (c % kFp8Block == 0) a.scale[row * a.row_blocks + b] = sc;
-                a.q[row * a.H + c] = fp8_encode(__fmul_rn(i & 1 ? v[i / 2].y : v[i / 2].x, inv));
+            for (int i = 0; i < kPairs; ++i) {
+                const float2 inv = make_float2(__shfl_sync(0xffffffffu, ratio, 4 * i), __shfl_sync(0xffffffffu, ratio, 4 * i + 2));
+                const float2 w = __fmul2_rn(v[i], inv);
+                const uint32_t codes = fp8_encode2(w.x, w.y), c = Row::first(t, 2 * i), c2 = Row::first(t, 2 * i + 1);
+                if (c < a.H) q[c] = static_cast<uint8_t>(codes);
+                if (c2 < a.H) q[c2] = static_cast<uint8_t>(codes >> 8);
             }
             if (W == 1) __syncwarp();  // with more warps, the next row's sums lie between this read and the next write
         }
@@ -535,20 +552,22 @@ template <int W, bool Vec, int P>
 struct CkptPart {
     static constexpr int N = Vec ? kCpt / P : kCpt;
     uint32_t code[Vec ? kCpt / 4 : kCpt];
-    float s[N];
+    float s[Vec ? N : 1];  // element by element: lane l holds the scale of the warp's columns l
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < (Vec ? kCpt / 4 : kCpt); ++i) code[i] = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) s[i] = 0.f;
+        for (int i = 0; i < (Vec ? N : 1); ++i) s[i] = 0.f;
     }
     __device__ __forceinline__ void load(const uint8_t* q, const float* scale, uint32_t t, uint32_t H) {
+        // a warp's 32 neighbouring columns lie in one block
+        const uint32_t c0 = t / 32 * 32 + 32 * W * (t % 32);
+        if (c0 < H && t % 32 < N) s[0] = __ldg(scale + c0 / kFp8Block);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const uint32_t c = t + 32 * W * i;
             if (c >= H) continue;
             code[i] = q[c];
-            s[i] = __ldg(scale + c / kFp8Block);
         }
     }
     __device__ __forceinline__ void values(float2 (&v)[kPairs]) const {
@@ -557,7 +576,8 @@ struct CkptPart {
             if constexpr (Vec)
                 v[i] = __fmul2_rn(fp8_decode2(code[i / 2] >> (i % 2 * 16)), f2(s[2 * i / P]));
             else
-                v[i] = __fmul2_rn(fp8_decode2(code[2 * i] | code[2 * i + 1] << 8), make_float2(s[2 * i], s[2 * i + 1]));
+                v[i] = __fmul2_rn(fp8_decode2(code[2 * i] | code[2 * i + 1] << 8),
+                                  make_float2(__shfl_sync(0xffffffffu, s[0], 2 * i), __shfl_sync(0xffffffffu, s[0], 2 * i + 1)));
         }
     }
 };
@@ -565,7 +585,7 @@ struct CkptPart {
 // dx of every row, and this CTA's sums over its rows of dy xh and dy: 16 columns per thread in
 // registers over all its rows, joined over the CTA's row groups at the end.
 template <typename T, int W, bool Vec, bool Ckpt>
-__global__ void __launch_bounds__(group_threads(W), bwd_ctas(W)) ln_bwd_row_kernel(const BwdArgs a) {
+__global__ void __launch_bounds__(group_threads(W), bwd_ctas(W, Vec)) ln_bwd_row_kernel(const BwdArgs a) {
     overlap_begin();
     using Row = RowPart<T, W, Vec>;
     using Part = typename std::conditional<Ckpt, CkptPart<W, Vec, Row::P>, Row>::type;
@@ -616,12 +636,14 @@ __global__ void __launch_bounds__(group_threads(W), bwd_ctas(W)) ln_bwd_row_kern
         at_block += static_cast<uint64_t>(stride) * a.row_blocks;
     };
     float mean_next = 0.f, rstd_next = 0.f;
-    auto fetch = [&](uint64_t r) {  // statistics, and without a ring the row
-        if constexpr (!Vec) {
-            dy_next.load(static_cast<const T*>(a.dy) + r * a.H + Row::first(t, 0), t, a.H);
-            if constexpr (Ckpt) x_next.load(a.q + r * a.H, a.scale + r * a.row_blocks, t, a.H);
-            else x_next.load(static_cast<const T*>(a.x) + r * a.H + Row::first(t, 0), t, a.H);
-        }
+    constexpr bool kAhead = !Vec && bwd_ahead(W);
+    auto fetch_row = [&](uint64_t r) {  // without a ring
+        dy_next.load(static_cast<const T*>(a.dy) + r * a.H + Row::first(t, 0), t, a.H);
+        if constexpr (Ckpt) x_next.load(a.q + r * a.H, a.scale + r * a.row_blocks, t, a.H);
+        else x_next.load(static_cast<const T*>(a.x) + r * a.H + Row::first(t, 0), t, a.H);
+    };
+    auto fetch = [&](uint64_t r) {  // what is held for the next row
+        if constexpr (kAhead) fetch_row(r);
         if constexpr (!Ckpt) mean_next = __ldg(a.mean + r);
         rstd_next = __ldg(a.rstd + r);
     };
@@ -661,6 +683,7 @@ __global__ void __launch_bounds__(group_threads(W), bwd_ctas(W)) ln_bwd_row_kern
                 }
             }
         }
+        if constexpr (!Vec && !kAhead) fetch_row(row);
         dy_next.values(g);
         x_next.values(xh);
         const float mean = mean_next, rstd = rstd_next;
@@ -782,7 +805,7 @@ int launch_bwd_rows(BwdArgs& a, float* dgamma, float* dbeta, cudaStream_t s) {
         // elements are loaded one by one) and writes the sums itself, which saves the join's launch (2 us
         // of host time, 3 us on the GPU).
         // Otherwise one CTA per place on the GPU: a second wave would fill its ring with nothing to hide it.
-        const uint32_t places = static_cast<uint32_t>(sm_count()) * bwd_ctas(W);
+        const uint32_t places = static_cast<uint32_t>(sm_count()) * bwd_ctas(W, Vec);
         a.parts_n = groups <= (Vec ? 4 : 1) ? 1 : std::min(parts_of(groups), places);
         a.sum_gamma = a.parts_n == 1 ? dgamma : a.parts;
         a.sum_beta = a.parts_n == 1 ? dbeta : a.parts + a.H;
