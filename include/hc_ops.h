@@ -319,7 +319,8 @@ struct matmul_fp8_block_tiling_data {
  * bias [N] of C's type or NULL, C of type `dtype` (F32, F16 or BF16), fp32 sums, one rounding.
  * K >= 1.  K a multiple of 16 with 16-byte aligned a and b -> tcgen05 kernels; otherwise a SIMT
  * kernel.  The gradient to A is the same call with the transposed weight and its transposed
- * scales. */
+ * scales.  The tcgen05 kernels form a_scale * b_scale in fp32: where the largest magnitudes of a block
+ * of A and a tile of B multiply to more than 2^145 it is infinite, and below 2^-108 it loses bits. */
 int hc_matmul_fp8_block_launch(const void* a, const float* a_scale, const void* b, const float* b_scale,
                                const void* bias, void* c, const struct matmul_fp8_block_tiling_data* t, int dtype,
                                void* stream);
