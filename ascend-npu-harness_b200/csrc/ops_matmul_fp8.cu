@@ -435,6 +435,9 @@ struct Few {
     static constexpr uint32_t kOffBar = kOffScale + 8 * TN * 4;
     static constexpr uint32_t kSmem = kOffBar + 512 + 1024;
     static_assert(TN * 128 * 4 <= kOffScale, "the joined sums reuse the ring");
+    // Clusters wait for CTAs on several SMs, so an allocation must not wait for another kernel's: whatever sizes
+    // two streams bring together, what fits the shared memory of an SM fits its 512 columns.
+    static_assert(kTmem <= 256 && 3 * kSmem > 227 * 1024, "three CTAs could share an SM");
 };
 
 template <uint32_t TN>

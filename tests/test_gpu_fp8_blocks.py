@@ -339,6 +339,61 @@ def test_other_stream_and_empty_tensors(ops):
     assert ops.matmul_fp8_block(a, torch.empty(0, 1, device="cuda"), w_q, w_s, None, torch.bfloat16).shape == (0, 64)
 
 
+def test_two_threads_on_two_streams(ops):
+    """Both kinds of tensor-core kernel, the layer norm's gradients and the activation, called by two threads at
+    once, each on its own stream: the bits of the calls alone."""
+    import threading
+
+    products = [operands(M, N, K, 30 + M) for M, N, K in ((16, 4096, 2048), (64, 2048, 4096), (100, 1024, 1024), (600, 1024, 1024))]
+    x, dy = (rnd((300, 1024), s, "bf16").cuda() for s in (40, 41))
+    gamma, beta = rnd((1024,), 42).cuda(), rnd((1024,), 43).cuda()
+
+    def calls():
+        out = [ops.matmul_fp8_block(*p, None, torch.bfloat16) for p in products]
+        y, mean, rstd = ops.layer_norm_fwd_train(x, gamma, beta, 1e-5)
+        out += [y, mean, rstd, *ops.layer_norm_bwd(dy, x, gamma, mean, rstd)]
+        y, q, scale = ops.activation_gelu_silu_ckpt(x, 0)
+        return out + [y, scale, ops.activation_gelu_silu_ckpt_bwd(dy, q, scale, 0)]
+
+    want = calls()
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got[i].append(calls())
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert [len(g) for g in got] == [10, 10]
+    for g in got:
+        for outs in g:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_tensors_on_another_device(ops):
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    x = rnd((200, 512), 44, "bf16")
+    gamma, beta = rnd((512,), 45), rnd((512,), 46)
+    w = operands(200, 256, 512, 47)
+    outs = []
+    for d in (0, 1):
+        on = [t.to(f"cuda:{d}") for t in (x, gamma, beta, *w)]
+        with torch.cuda.device(0):  # the current device stays the first
+            y, q, scale, rstd = ops.layer_norm_ckpt(*on[:3], 1e-5)
+            grads = ops.layer_norm_ckpt_bwd(on[0], q, scale, on[1], rstd)
+            outs.append([t.cpu() for t in (y, scale, rstd, *grads, ops.matmul_fp8_block(*on[3:], None, torch.float32),
+                                           hc.matmul_fp8_block(*on[3:]))])
+            assert torch.cuda.current_device() == 0
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
 def feed_forward(ops, x, gamma, beta, w1, w2, dout):
     """One training step of a feed-forward layer with 8-bit operands and checkpoints: out, and the
     gradients of x, gamma, beta and both weights (bf16 [N, K])."""
