@@ -20,6 +20,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <mutex>
 #include <type_traits>
 
@@ -847,19 +848,31 @@ uint32_t few_clusters(uint32_t c) {
 struct FewPlan {
     uint32_t splits;
     uint64_t cost;
+    uint64_t waves, per_sm, blocks;  // blocks: of one CTA
 };
 template <typename T, uint32_t TN>
 FewPlan few_plan(const Params& p) {
     const uint64_t tiles = static_cast<uint64_t>(p.nb) * ((p.M + TN - 1) / TN), sms = sm_count();
-    FewPlan best{1, ~0ull};
+    FewPlan best{1, ~0ull, 1, 1, p.kb};
     for (uint32_t c = 1; c <= 8 && c <= p.kb; ++c) {
         const uint64_t room = few_clusters<T, TN>(c), waves = (tiles + room - 1) / room;
         if (c > 1 && waves > 1) break;
         const uint64_t at_once = tiles < room ? tiles : room, per_sm = (at_once * c + sms - 1) / sms;
-        const uint64_t cost = waves * (per_sm * ((p.kb + c - 1) / c) + 3 + (c > 1 ? (TN > 64 ? 5 : 2) : 0));
-        if (cost < best.cost) best = FewPlan{c, cost};
+        const uint64_t blocks = (p.kb + c - 1) / c;
+        const uint64_t cost = waves * (per_sm * blocks + 3 + (c > 1 ? (TN > 64 ? 5 : 2) : 0));
+        if (cost < best.cost) best = FewPlan{c, cost, waves, per_sm, blocks};
     }
     return best;
+}
+
+// What that plan takes, in units of 10 ns: a block 0.53 us with 128 tokens, 0.46 with 96 and 0.42 with 64, or
+// 0.29 where two CTAs of 64 share the SM; starting and draining a wave 4.8, 4.1 and 3.2 us, the join 1.5 and 0.8.
+template <typename T, uint32_t TN>
+uint64_t few_time(const Params& p) {
+    const FewPlan f = few_plan<T, TN>(p);
+    const uint64_t block = TN > 96 ? 53 : TN > 64 ? 46 : f.per_sm > 1 ? 29 : 42;
+    const uint64_t join = f.splits > 1 ? (TN > 64 ? 150 : 80) : 0;
+    return f.waves * (f.per_sm * f.blocks * block + (TN > 96 ? 480 : TN > 64 ? 410 : 320) + join);
 }
 
 template <typename T, uint32_t TN>
@@ -876,6 +889,8 @@ int launch_few(const Params& p, cudaStream_t s) {
     return check_launch("mm8_few_kernel");
 }
 
+constexpr uint64_t kL2Weight = 64ull << 20;  // half of the L2
+
 template <typename T>
 int launch(Params p, cudaStream_t s) {
     const bool tc = p.K % 16 == 0 && aligned16(p.a) && aligned16(p.b);
@@ -889,19 +904,27 @@ int launch(Params p, cudaStream_t s) {
     p.vec_store = aligned16(p.c) && (static_cast<uint64_t>(p.N) * sizeof(T)) % 16 == 0;
     const int pairs = pair_clusters();
     // grid limits of the few-token kernel: 65535 weight tiles and token tiles
-    const bool few_fits = p.nb <= 65535 && (p.M + 127) / 128 <= 65535;
+    const bool few_fits = p.nb <= 65535 && (p.M + 63) / 64 <= 65535;
     if (tiles > 0x7FFFFFFFull) return launch_simt<T>(p, s);
     p.num_tiles = static_cast<uint32_t>(tiles);
-    // Pairs where that takes no longer than 128-token tiles: a block costs both about the same time, starting
-    // and draining a 256 x 256 tile some eight (4096 x 4096 weight: M = 256 15.7 us against 24 in
-    // pairs, M = 512 24 either way, M = 1024 49 against 25; 1467 x 793 x 1328 11.9 against 15.3).
-    const uint64_t pair_cost = pairs > 0 ? (tiles + pairs - 1) / pairs * p.kb + 8 : ~0ull;
-    if (pairs > 0 && (!few_fits || (p.M > 128 && pair_cost <= few_plan<T, 128>(p).cost))) return launch_pair<T>(p, pairs, s);
-    if (!few_fits) return launch_simt<T>(p, s);
+    if (!few_fits) return pairs > 0 ? launch_pair<T>(p, pairs, s) : launch_simt<T>(p, s);
     if (p.M <= 16) return launch_few<T, 16>(p, s);
     if (p.M <= 32) return launch_few<T, 32>(p, s);
     if (p.M <= 64) return launch_few<T, 64>(p, s);
-    if (p.M <= 96) return launch_few<T, 96>(p, s);
+    // More tokens: the least time of pairs (0.5 us a block, 4 us to start and drain a wave of tiles) and token tiles
+    // of 128, 96 or 64.  us measured with 64 / 96 / 128 / pairs: 133x1640x176 4.5 / 5.7 / 6.7 / 7.9,
+    // 420x2679x7136 26.4 / 29.5 / 33.4 / 33.6, 300x4096x4096 22.2 / 19.5 / 22.7 / 21.7, 1000x1000x4096
+    // 17.3 / 19.4 / 14.9 / 20.8, 700x4096x4096 39 / 38 / 44 / 22.9.  Token tiles that read a weight more than once
+    // count on the L2 holding it.
+    const uint64_t weight = static_cast<uint64_t>(p.N) * p.K;
+    const uint64_t pair = p.M > 128 && pairs > 0 ? (tiles + pairs - 1) / pairs * (p.kb * 50ull + 400) + 200 : ~0ull;
+    const uint64_t t128 = few_time<T, 128>(p);
+    const uint64_t t96 = p.M <= 96 || weight <= kL2Weight ? few_time<T, 96>(p) : ~0ull;
+    const uint64_t t64 = weight <= kL2Weight ? few_time<T, 64>(p) : ~0ull;
+    const uint64_t least = std::min(std::min(pair, t128), std::min(t96, t64));
+    if (least == pair) return launch_pair<T>(p, pairs, s);
+    if (least == t64) return launch_few<T, 64>(p, s);
+    if (least == t96) return launch_few<T, 96>(p, s);
     return launch_few<T, 128>(p, s);
 }
 
