@@ -14,14 +14,14 @@
 //
 // Both directions are HBM streams: the forward moves 2 e bytes per element (e = element size) and 1 + 1/32 more
 // for the checkpoint, the backward 3 e, or 2 e + 1 + 1/32 from the checkpoint.  Measured on one B200, copy rate 6.56 TB/s:
-//   [16384, 4096] bf16   forward 53 us (5.1 TB/s, 77 %), gradients 80 us (5.0 TB/s; their kernel alone
-//                        75 us, 82 %, the join of the partial sums the rest)
-//   [8192, 4096] fp32    forward 44 us (6.1 TB/s), gradients 67 us (6.0 TB/s)
-//   [8192, 8192] bf16    with the checkpoint: forward 73 us, gradients 83 us (4.1 TB/s)
+//   [16384, 4096] bf16   forward 51 us (5.3 TB/s, 80 %), gradients 72.5 us (5.6 TB/s, the join of the partial
+//                        sums included)
+//   [8192, 4096] fp32    forward 44 us (6.1 TB/s), gradients 65 us (6.2 TB/s)
+//   [8192, 8192] bf16    with the checkpoint: forward 72 us, gradients 76 us (4.5 TB/s)
 //   [8192, 4001] bf16    (rows that are not whole packs) forward 43 us, gradients 72 us (2.7 TB/s); with the
 //                        checkpoint 63 and 70 us
 // 16-bit rows are bound by issue slots and shared-memory traffic per element (issue 43-54 % active, 14-17
-// warp instructions per 32 elements), not by DRAM: fp32 rows, with half the elements per byte, run at 92 %.
+// warp instructions per 32 elements), not by DRAM: fp32 rows, with half the elements per byte, run at 94 %.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -297,13 +297,42 @@ struct RowPart {
     }
     // Parameters of the thread's columns (read once per thread; zeros behind the end).
     __device__ __forceinline__ static void params(const float* p, float2 (&v)[kPairs], uint32_t t, uint32_t H) {
-        float f[kCpt];
+        alignas(16) float f[kCpt];
+        if (Vec && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
+            for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int e = 0; e < kRun; ++e) f[i * kRun + e] = first(t, i) < H ? __ldg(p + first(t, i) + e) : 0.f;
+                for (int e = 0; e + 3 < kRun; e += 4)
+                    *reinterpret_cast<float4*>(f + i * kRun + e) = first(t, i) < H
+                        ? __ldg(reinterpret_cast<const float4*>(p + first(t, i) + e)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+                for (int e = 0; e < kRun; ++e) f[i * kRun + e] = first(t, i) < H ? __ldg(p + first(t, i) + e) : 0.f;
+        }
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) v[i] = make_float2(f[2 * i], f[2 * i + 1]);
+    }
+    // Sums of the thread's columns, four at a time where the row's start allows (one at a time 32 lanes write
+    // into as many sectors: 4 us more per CTA of 16 warps).
+    __device__ __forceinline__ static void store_sums(float* p, const float2 (&v)[kPairs], uint32_t t, uint32_t H) {
+        const bool wide = Vec && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t c = first(t, i);
+            if (c >= H) continue;
+            if (wide) {
+#pragma unroll
+                for (int e = 0; e + 3 < kRun; e += 4) {
+                    const float2 lo = v[(i * kRun + e) / 2], hi = v[(i * kRun + e) / 2 + 1];
+                    *reinterpret_cast<float4*>(p + c + e) = make_float4(lo.x, lo.y, hi.x, hi.y);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < kRun; ++e) p[c + e] = (i * kRun + e) & 1 ? v[(i * kRun + e) / 2].y : v[(i * kRun + e) / 2].x;
+            }
+        }
     }
     // Zeros in the columns behind the end.
     __device__ __forceinline__ static void clear_behind(float2 (&v)[kPairs], uint32_t t, uint32_t H) {
@@ -737,17 +766,8 @@ __global__ void __launch_bounds__(group_threads(W), bwd_ctas(W, Vec)) ln_bwd_row
                 dbeta[i] = __fadd2_rn(dbeta[i], joined[((o * 2 + 1) * kPairs + i) * 32 * W + t]);
             }
     }
-#pragma unroll
-    for (int i = 0; i < Row::N; ++i) {
-        const uint32_t c = Row::first(t, i);
-        if (c >= a.H) continue;
-#pragma unroll
-        for (int e = 0; e < Row::kRun; ++e) {
-            const int j = i * Row::kRun + e;
-            to_gamma[c + e] = j & 1 ? dgamma[j / 2].y : dgamma[j / 2].x;
-            to_beta[c + e] = j & 1 ? dbeta[j / 2].y : dbeta[j / 2].x;
-        }
-    }
+    Row::store_sums(to_gamma, dgamma, t, a.H);
+    Row::store_sums(to_beta, dbeta, t, a.H);
 }
 
 // Calls f with the number of warps that own a row of H <= kMaxFastH elements.

@@ -183,6 +183,29 @@ def test_unaligned_buffers(cuda, kind):
             R.assert_within(got, want, bound, f"moved {f}")
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,H", [(1, 768), (40, 768), (3, 6000), (20, 6000)])
+def test_parameters_at_any_address(cuda, rows, H, kind):
+    """gamma, beta, dgamma and dbeta 4 bytes behind a 16-byte boundary: the bits of the aligned call, and nothing
+    written beside them."""
+    x, gamma, beta, dy = inputs((rows, H), kind)
+    off = [torch.cat([v[:1], v])[1:] for v in (gamma, beta)]
+    assert all(v.data_ptr() % 16 == 4 for v in off)
+    want = hc.layer_norm_fwd_train(x, gamma, beta, EPS)
+    assert all(torch.equal(a, b) for a, b in zip(hc.layer_norm_fwd_train(x, *off, EPS), want))
+    mean, rstd = want[1:]
+    dx, dgamma, dbeta = hc.layer_norm_bwd(dy, x, gamma, mean, rstd)
+    out, dx2 = torch.full((2, H + 8), 7.0, device="cuda"), torch.empty_like(dx)
+    t = hc.LayerNormTiling(rows, H, 0, EPS)
+    work = torch.empty(rows * 2 * H, device="cuda")
+    hc.check(hc.load().hc_layer_norm_bwd_launch(
+        dy.data_ptr(), x.data_ptr(), off[0].data_ptr(), mean.data_ptr(), rstd.data_ptr(), dx2.data_ptr(),
+        out[0, 1:].data_ptr(), out[1, 1:].data_ptr(), work.data_ptr(), work.numel() * 4, t, hc.dtype_code(x),
+        torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(dx2, dx) and torch.equal(out[0, 1:H + 1], dgamma) and torch.equal(out[1, 1:H + 1], dbeta)
+    assert bool((out[:, 0] == 7.0).all()) and bool((out[:, H + 1:] == 7.0).all())
+
+
 def test_no_rows(ops):
     x, gamma = torch.empty(0, 64, device="cuda"), torch.ones(64, device="cuda")
     y, mean, rstd = ops.layer_norm_fwd_train(x, gamma, gamma, EPS)
