@@ -9,8 +9,10 @@
 // xh comes from x, mean and rstd, or from the checkpoint (q * scale), which needs rstd only: the
 // 8-bit form keeps xh and not x, whose offset would cost it precision.
 //
-// Statistics and sums are fp32.  The mean is taken over deviations from an element of the row and the
-// variance over deviations from the mean, as in the forward-only kernels.
+// Statistics and sums are fp32.  A first mean is taken over deviations from an element of the row.  The squares are
+// of deviations from that mean, whose own sum corrects both it and them: with d = x - m and r = sum d,
+//   mean = m + r / H,  sum (x - mean)^2 = sum d^2 - r^2 / H,  x - mean = d - r / H,
+// so neither the element (which may be far from all others) nor the rounding of m is left in the row.
 //
 // Both directions are HBM streams: the forward moves 2 e bytes per element (e = element size) and 1 + 1/32 more
 // for the checkpoint, the backward 3 e, or 2 e + 1 + 1/32 from the checkpoint.  Measured on one B200, copy rate 6.56 TB/s:
@@ -79,6 +81,24 @@ __device__ __forceinline__ float cta_sum(float v, float* sh) {
     return s;
 }
 
+// The same of two values.
+__device__ __forceinline__ float2 cta_sum2(float2 v, float2* sh) {
+    v = make_float2(warp_sum(v.x), warp_sum(v.y));
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x / 32] = v;
+    __syncthreads();
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) s = make_float2(s.x + sh[w].x, s.y + sh[w].y);
+    return s;
+}
+
+// A sum of deviations that corrects a mean or a sum of squares m2, left out where m2 is infinite (a finite row's rstd
+// is 0 then) or NaN.
+__device__ __forceinline__ float residual(float r, float m2) { return m2 < __int_as_float(0x7F800000) ? r : 0.f; }
+// A corrected sum of squares, which roundings may leave just below zero; NaN stays.
+__device__ __forceinline__ float not_below_zero(float m2) { return m2 < 0.f ? 0.f : m2; }
+
 // ---------------------------------------------------------------------------------------
 // Any row length and alignment: one CTA per row, the row re-read from cache for each pass.
 // ---------------------------------------------------------------------------------------
@@ -86,6 +106,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) ln_fwd_any_kernel(const FwdArgs a) {
     overlap_begin();
     __shared__ float sh[kWarps];
+    __shared__ float2 sh2[kWarps];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     const float H = static_cast<float>(a.H);
     for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -94,15 +115,18 @@ __global__ void __launch_bounds__(kThreads) ln_fwd_any_kernel(const FwdArgs a) {
         const float K = elem<T>::to_f(x[0]);
         float s = 0.f;
         for (uint32_t c = threadIdx.x; c < a.H; c += kThreads) s += elem<T>::to_f(x[c]) - K;
-        const float mean = K + __fdiv_rn(cta_sum(s, sh), H);
-        s = 0.f;
+        const float first = K + __fdiv_rn(cta_sum(s, sh), H);
+        float2 sums = make_float2(0.f, 0.f);
         for (uint32_t c = threadIdx.x; c < a.H; c += kThreads) {
-            const float d = elem<T>::to_f(x[c]) - mean;
-            s = fmaf(d, d, s);
+            const float d = elem<T>::to_f(x[c]) - first;
+            sums = make_float2(sums.x + d, fmaf(d, d, sums.y));
         }
-        const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(cta_sum(s, sh), H) + a.eps));
+        sums = cta_sum2(sums, sh2);
+        const float r = residual(sums.x, sums.y), shift = __fdiv_rn(r, H);
+        const float m2 = not_below_zero(fmaf(-shift, r, sums.y));
+        const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(m2, H) + a.eps)), off = -shift * rstd;
         if (threadIdx.x == 0) {
-            if (a.mean) a.mean[row] = mean;
+            if (a.mean) a.mean[row] = first + shift;
             a.rstd[row] = rstd;
         }
         for (uint32_t b = warp; b < a.row_blocks; b += kWarps) {
@@ -111,7 +135,7 @@ __global__ void __launch_bounds__(kThreads) ln_fwd_any_kernel(const FwdArgs a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t c = b * kFp8Block + lane + 32 * i;
-                xh[i] = c < a.H ? (elem<T>::to_f(x[c]) - mean) * rstd : 0.f;
+                xh[i] = c < a.H ? fmaf(elem<T>::to_f(x[c]) - first, rstd, off) : 0.f;
                 m = max(m, abs_bits(xh[i]));
                 if (c < a.H) y[c] = elem<T>::from_f(fmaf(xh[i], a.gamma[c], a.beta[c]));
             }
@@ -348,26 +372,29 @@ struct RowPart {
             for (int e = 0; e < kRun; ++e) ((i * kRun + e) & 1 ? v[(i * kRun + e) / 2].y : v[(i * kRun + e) / 2].x) = 0.f;
         }
     }
-    // The sum of what `f` makes of each pair, over the thread's columns of the row; f may change them.
-    template <typename F>
-    __device__ __forceinline__ static float sum_of(float2 (&v)[kPairs], uint32_t t, uint32_t H, F f) {
-        float2 s = f2(0.f);
+    // Two sums of what `f` adds to them for each pair, over the thread's columns of the row (of the first `Loads` loads);
+    // f may change the pair.
+    template <int Loads, typename F>
+    __device__ __forceinline__ static float2 sums_of(float2 (&v)[kPairs], uint32_t t, uint32_t H, F f) {
+        float2 s = f2(0.f), q = f2(0.f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
+        for (int i = 0; i < Loads; ++i) {
             if constexpr (Vec) {
                 if (first(t, i) >= H) continue;
 #pragma unroll
-                for (int e = 0; e < kRun / 2; ++e) s = f(v[i * kRun / 2 + e], s);
+                for (int e = 0; e < kRun / 2; ++e) f(v[i * kRun / 2 + e], s, q);
             } else if (i % 2 == 0) {  // a pair's two columns end separately
-                if (first(t, i + 1) < H) s = f(v[i / 2], s);
+                if (first(t, i + 1) < H) f(v[i / 2], s, q);
                 else if (first(t, i) < H) {
-                    float2 one = v[i / 2];
-                    s.x = f(one, s).x;
+                    float2 one = v[i / 2], s1 = s, q1 = q;
+                    f(one, s1, q1);
+                    s.x = s1.x;
+                    q.x = q1.x;
                     v[i / 2] = make_float2(one.x, 0.f);
                 }
             }
         }
-        return s.x + s.y;
+        return make_float2(s.x + s.y, q.x + q.y);
     }
 };
 
@@ -435,39 +462,51 @@ __device__ __forceinline__ float lanes_sum(float v) {
 }
 
 // CTAs per SM that the registers are divided for.  Rows loaded one element at a time hold the next row in
-// 16 registers instead of 8 and spilled with three ([8192, 4001] bf16: 55 us with three, 43 with two).
-constexpr int fwd_ctas(int W, bool vec) { return W > 8 ? 1 : vec ? 3 : 2; }
+// 16 registers instead of 8 and spilled with three ([8192, 4001] bf16: 55 us with three, 43 with two).  Packs of fp32 and
+// the checkpoint spill up to 156 bytes with three, and two are better up to four warps ([8192, 2048] bf16 with the
+// checkpoint 18.9 us, with three 19.4; fp32 27.2 and 33.2, without it 24.6 and 25.7), not with eight ([8192, 3584] 42.5
+// fp32 with two, 38.9 with three) or one ([16384, 512] bf16 10.6 and 10.5).
+constexpr int fwd_ctas(int W, bool vec, bool ckpt, size_t bytes) {
+    return W > 8 ? 1 : !vec || ((ckpt || bytes == 4) && (W == 2 || W == 4)) ? 2 : 3;
+}
 
-// Statistics: each warp takes the mean of its own columns (over deviations from its first one) and its
-// sum of squares around that, with shuffles alone; the row's follow from the W pairs behind one
-// barrier, M2 = sum_w M2_w + n_w (mean_w - mean)^2, which is as exact as two passes over the row.
+// Statistics: each warp takes the mean m_w of the first half of its n_w columns (over deviations from its first one), and
+// the sums r_w and M2_w of all its columns' deviations from that and of their squares, with shuffles alone.  Half of the
+// columns will do, since r_w makes up for the difference.  The row's follow from the W triples behind one barrier, relative to the first warp's m_0:
+//   d_w = m_w - m_0, delta = sum_w (n_w d_w + r_w) / H, mean = m_0 + delta, x - mean = (x - m_w) + (d_w - delta),
+//   M2 = sum_w (M2_w + d_w (n_w d_w + 2 r_w)) - H delta^2,
+// two sums that need not wait for one another.  What cancels in M2 is at most H / 256 of it (m_0 is the mean of 256
+// columns, whose distance from the row's mean is part of the row's own squares), and about 1 / 256 where columns are alike.
+// Every rounding is of a deviation, as in two passes around the exact mean: an element 1e4 times the others at a
+// warp's front, or an offset of 1e6, leaves xh exact to 1e-7 (without r_w, and with x - m_w formed from the
+// rounded x - first: 4e-6 and 2e-2).
 template <typename T, int W, bool Vec, bool Ckpt>
-__global__ void __launch_bounds__(group_threads(W), fwd_ctas(W, Vec)) ln_fwd_row_kernel(const FwdArgs a) {
+__global__ void __launch_bounds__(group_threads(W), fwd_ctas(W, Vec, Ckpt, sizeof(T))) ln_fwd_row_kernel(const FwdArgs a) {
     overlap_begin();
     using Row = RowPart<T, W, Vec>;
     constexpr int G = row_groups(W), P = Row::P;
-    __shared__ float2 sh[G][2][W];
+    __shared__ float4 sh[G][2][W];
     __shared__ alignas(16) uint32_t quarter[Ckpt && !Vec ? G : 1][Ckpt && !Vec ? W * kCpt : 4];
     const uint32_t group = threadIdx.x / (32 * W), t = threadIdx.x % (32 * W), wir = t / 32;
     const uint32_t stride = gridDim.x * G;
     const uint64_t step = static_cast<uint64_t>(stride) * a.H;
-    const float inv_h = 1.0f / static_cast<float>(a.H);
+    const float H = static_cast<float>(a.H), inv_h = 1.0f / H;
     float2 gamma[kPairs], beta[kPairs];
     Row::params(a.gamma, gamma, t, a.H);
     Row::params(a.beta, beta, t, a.H);
     // columns of warp w of the row
-    auto columns_of = [&](uint32_t w) {
+    auto columns_of = [&](uint32_t w, int loads) {
         uint32_t n = 0;
 #pragma unroll
-        for (int i = 0; i < Row::N; ++i) {
+        for (int i = 0; i < loads; ++i) {
             const uint32_t c = Row::first(32 * w, i), len = 32 * Row::kRun;
             n += c >= a.H ? 0 : min(len, a.H - c);
         }
         return n;
     };
-    const uint32_t n_mine = columns_of(wir);
-    const float inv_mine = n_mine ? 1.0f / static_cast<float>(n_mine) : 0.f;
-    const float n_lane = static_cast<float>(columns_of(t % W));
+    const uint32_t n_half = columns_of(wir, Row::N / 2);
+    const float inv_half = n_half ? 1.0f / static_cast<float>(n_half) : 0.f;
+    const float n_lane = static_cast<float>(columns_of(t % W, Row::N));
     uint64_t row = static_cast<uint64_t>(blockIdx.x) * G + group;
     const T* x = static_cast<const T*>(a.x) + row * a.H + Row::first(t, 0);
     T* y = static_cast<T*>(a.y) + row * a.H + Row::first(t, 0);
@@ -481,27 +520,36 @@ __global__ void __launch_bounds__(group_threads(W), fwd_ctas(W, Vec)) ln_fwd_row
         x += step;
         if (row + stride < a.rows) next.load(x, t, a.H);
         const float K = __shfl_sync(0xffffffffu, v[0].x, 0);  // lane 0 holds the warp's first column
-        float s = Row::sum_of(v, t, a.H, [&](float2& p, float2 s) {
-            p = __fadd2_rn(p, f2(-K));
-            return __fadd2_rn(s, p);
+        const float lanes = Row::template sums_of<Row::N / 2>(v, t, a.H, [&](float2& p, float2& s, float2&) {
+            s = __fadd2_rn(s, __fadd2_rn(p, f2(-K)));
+        }).x;
+        const float own = fmaf(warp_sum(lanes), inv_half, K);
+        const float2 sums = Row::template sums_of<Row::N>(v, t, a.H, [&](float2& p, float2& s, float2& q) {
+            p = __fadd2_rn(p, f2(-own));
+            s = __fadd2_rn(s, p);
+            q = __ffma2_rn(p, p, q);
         });
-        const float shift = warp_sum(s) * inv_mine;  // the warp's mean is K + shift
-        s = Row::sum_of(v, t, a.H, [&](float2& p, float2 s) {
-            p = __fadd2_rn(p, f2(-shift));
-            return __ffma2_rn(p, p, s);
-        });
-        float m2 = warp_sum(s), mean = K + shift, off = 0.f;  // v holds deviations from the warp's mean
+        float r = warp_sum(sums.x), m2 = warp_sum(sums.y);
+        float mean, off;  // off: from the warp's mean to the row's
         if constexpr (W > 1) {
-            if (t % 32 == 0) sh[group][flip][wir] = make_float2(mean, m2);
+            if (t % 32 == 0) sh[group][flip][wir] = make_float4(own, r, m2, 0.f);
             asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * W) : "memory");
             // every run of W lanes joins all warps, one each
-            const float2 w = sh[group][flip][t % W];
-            const float own = mean, base = __shfl_sync(0xffffffffu, w.x, 0);
-            mean = fmaf(lanes_sum<W>(n_lane * (w.x - base)), inv_h, base);
-            const float e = w.x - mean;
-            m2 = lanes_sum<W>(fmaf(n_lane * e, e, w.y));
-            off = own - mean;
+            const float4 w = sh[group][flip][t % W];
+            const float base = __shfl_sync(0xffffffffu, w.x, 0), dist = w.x - base;
+            r = residual(w.y, w.z);
+            const float moment = fmaf(n_lane, dist, r), delta = lanes_sum<W>(moment) * inv_h;
+            m2 = lanes_sum<W>(fmaf(dist, moment + r, w.z));
+            m2 = fmaf(-residual(H * delta, m2), delta, m2);
+            mean = base + delta;
+            off = own - base - delta;
+        } else {
+            r = residual(r, m2);
+            off = -r * inv_h;
+            m2 = fmaf(off, r, m2);
+            mean = own - off;
         }
+        m2 = not_below_zero(m2);
         const float rstd = rsqrtf(fmaf(m2, inv_h, a.eps));
         if (t == 0) {
             if (a.mean) a.mean[row] = mean;
