@@ -33,12 +33,15 @@
 // hc.load_torch_ops() also registers the attention backward as the autograd formula of the forward
 // op; the two layer norms and the checkpointed activation have theirs here (class names ending in
 // Function), since a Python formula would cost more host time than the kernels take on small rows.
+// The other ops without reference counterparts raise where a derivative of them is asked for, and all of
+// them where a forward-mode one is.
 // Load with torch.ops.load_library("ascend-npu-harness_b200/lib/libhc_torch.so").
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
@@ -598,17 +601,26 @@ bool wants_grad(const T&... t) {
     return at::GradMode::is_enabled() && (t.requires_grad() || ...);
 }
 
+// A forward-mode tangent does not need requires_grad; without a formula it would be lost, i.e. count as zero.
+template <typename... T>
+void no_tangents(const char* op, const T&... t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!(t._fw_grad(/*level=*/0).defined() || ...), "hc::", op, " has no forward-mode derivative");
+}
+
 Tensors3 layer_norm_fwd_train_autograd(TensorRef x, TensorRef gamma, TensorRef beta, double eps) {
+    no_tangents("layer_norm_fwd_train", x, gamma, beta);
     if (!wants_grad(x, gamma, beta)) return ln_fwd_train_below(x, gamma, beta, eps);
     const variable_list o = LayerNormFunction::apply(x, gamma, beta, eps);
     return {o[0], o[1], o[2]};
 }
 Tensors4 layer_norm_ckpt_autograd(TensorRef x, TensorRef gamma, TensorRef beta, double eps) {
+    no_tangents("layer_norm_ckpt", x, gamma, beta);
     if (!wants_grad(x, gamma, beta)) return ln_ckpt_below(x, gamma, beta, eps);
     const variable_list o = LayerNormCkptFunction::apply(x, gamma, beta, eps);
     return {o[0], o[1], o[2], o[3]};
 }
 Tensors3 activation_gelu_silu_ckpt_autograd(TensorRef x, int64_t act) {
+    no_tangents("activation_gelu_silu_ckpt", x);
     if (!wants_grad(x)) return act_ckpt_below(x, act);
     const variable_list o = ActivationCkptFunction::apply(x, act);
     return {o[0], o[1], o[2]};
@@ -770,4 +782,8 @@ TORCH_LIBRARY_IMPL(hc, Autograd, m) {
     m.impl("activation_gelu_silu_ckpt", &activation_gelu_silu_ckpt_autograd);
     m.impl("layer_norm_fwd_train", &layer_norm_fwd_train_autograd);
     m.impl("layer_norm_ckpt", &layer_norm_ckpt_autograd);
+    // no derivative of their own: an error where one is asked for, instead of a gradient or tangent lost
+    for (const char* op : {"quantize_fp8_block", "dequantize_fp8_block", "matmul_fp8_block", "activation_gelu_silu_ckpt_bwd",
+                           "layer_norm_bwd", "layer_norm_ckpt_bwd"})
+        m.impl(op, torch::autograd::autogradNotImplementedFallback());
 }

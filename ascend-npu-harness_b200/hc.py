@@ -578,7 +578,8 @@ def load_torch_ops():
     hc::flash_attention_fwd_fused gets an autograd formula: hc::flash_attention_bwd (q, k, v get
     gradients; the lse output is not differentiable).  hc::layer_norm_fwd_train, hc::layer_norm_ckpt and
     hc::activation_gelu_silu_ckpt are differentiable in their first output through their _bwd ops, the latter two
-    from the 8-bit blocks they return, without keeping their input.  Capturing such a backward into a CUDA
+    from the 8-bit blocks they return, without keeping their input.  Forward-mode derivatives of these raise, and
+    so does any derivative of the other ops of this kind (quantise, dequantise, matmul_fp8_block, the _bwd ops).  Capturing such a backward into a CUDA
     graph follows torch's rule: no eager graph of the same leaves may live meanwhile (torch raises); the _bwd
     ops themselves can be captured at any time."""
     global _torch_ops_loaded
