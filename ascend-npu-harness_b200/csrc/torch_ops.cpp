@@ -543,6 +543,22 @@ Tensors3 act_ckpt_below(TensorRef x, int64_t act) {
     return op.call(x, act);
 }
 
+// The gradients as ops, so that every layer of the dispatcher (Meta, fake and traced tensors, modes, tangents) sees them.
+Tensors3 ln_bwd_op(TensorRef dy, TensorRef x, TensorRef gamma, TensorRef mean, TensorRef rstd) {
+    static const auto op = op_handle<Tensors3(TensorRef, TensorRef, TensorRef, TensorRef, TensorRef)>("hc::layer_norm_bwd");
+    return op.call(dy, x, gamma, mean, rstd);
+}
+Tensors3 ln_ckpt_bwd_op(TensorRef dy, TensorRef q, TensorRef scale, TensorRef gamma, TensorRef rstd) {
+    static const auto op =
+        op_handle<Tensors3(TensorRef, TensorRef, TensorRef, TensorRef, TensorRef)>("hc::layer_norm_ckpt_bwd");
+    return op.call(dy, q, scale, gamma, rstd);
+}
+at::Tensor act_ckpt_bwd_op(TensorRef dy, TensorRef q, TensorRef scale, int64_t act) {
+    static const auto op =
+        op_handle<at::Tensor(TensorRef, TensorRef, TensorRef, int64_t)>("hc::activation_gelu_silu_ckpt_bwd");
+    return op.call(dy, q, scale, act);
+}
+
 void no_double_backward(const char* op) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "hc::", op, " has no second derivative (create_graph=True)");
 }
@@ -558,7 +574,7 @@ struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
         no_double_backward("layer_norm_fwd_train");
         if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
         const auto s = ctx->get_saved_variables();
-        auto [dx, dgamma, dbeta] = layer_norm_bwd_cuda(grads[0].contiguous(), s[0], s[1], s[2], s[3]);
+        auto [dx, dgamma, dbeta] = ln_bwd_op(grads[0].contiguous(), s[0], s[1], s[2], s[3]);
         return {dx, dgamma, dbeta, at::Tensor()};
     }
 };
@@ -574,7 +590,7 @@ struct LayerNormCkptFunction : torch::autograd::Function<LayerNormCkptFunction> 
         no_double_backward("layer_norm_ckpt");
         if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
         const auto s = ctx->get_saved_variables();
-        auto [dx, dgamma, dbeta] = layer_norm_ckpt_bwd_cuda(grads[0].contiguous(), s[0], s[1], s[2], s[3]);
+        auto [dx, dgamma, dbeta] = ln_ckpt_bwd_op(grads[0].contiguous(), s[0], s[1], s[2], s[3]);
         return {dx, dgamma, dbeta, at::Tensor()};
     }
 };
@@ -591,8 +607,7 @@ struct ActivationCkptFunction : torch::autograd::Function<ActivationCkptFunction
         no_double_backward("activation_gelu_silu_ckpt");
         if (!grads[0].defined()) return {at::Tensor(), at::Tensor()};
         const auto s = ctx->get_saved_variables();
-        return {activation_gelu_silu_ckpt_bwd_cuda(grads[0].contiguous(), s[0], s[1], ctx->saved_data["act"].toInt()),
-                at::Tensor()};
+        return {act_ckpt_bwd_op(grads[0].contiguous(), s[0], s[1], ctx->saved_data["act"].toInt()), at::Tensor()};
     }
 };
 
