@@ -513,31 +513,18 @@ c10::TypedOperatorHandle<F> op_handle(const char* name) {
     return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").template typed<F>();
 }
 
-// CUDA tensors that no mode, functional transform or subclass wants to see dispatched.
-template <typename... T>
-bool plain_cuda(TensorRef x, const T&... others) {
-    constexpr c10::DispatchKeySet usual({c10::DispatchKey::CUDA, c10::DispatchKey::AutogradCUDA,
-                                         c10::DispatchKey::ADInplaceOrView, c10::DispatchKey::AutocastCUDA});
-    const c10::impl::LocalDispatchKeySet local = c10::impl::tls_local_dispatch_key_set();
-    const c10::DispatchKeySet keys = (x.key_set() | ... | others.key_set());
-    return (((keys | local.included_) - local.excluded_) - usual).empty() && x.is_cuda();
-}
-
-// The ops below their autograd layer (CUDA tensors: straight to the kernel's wrapper).
+// The ops below their autograd layer.
 Tensors3 ln_fwd_train_below(TensorRef x, TensorRef gamma, TensorRef beta, double eps) {
-    if (plain_cuda(x, gamma, beta)) return layer_norm_fwd_train_cuda(x, gamma, beta, eps);
     static const auto op = op_handle<Tensors3(TensorRef, TensorRef, TensorRef, double)>("hc::layer_norm_fwd_train");
     at::AutoDispatchBelowADInplaceOrView guard;
     return op.call(x, gamma, beta, eps);
 }
 Tensors4 ln_ckpt_below(TensorRef x, TensorRef gamma, TensorRef beta, double eps) {
-    if (plain_cuda(x, gamma, beta)) return layer_norm_ckpt_cuda(x, gamma, beta, eps);
     static const auto op = op_handle<Tensors4(TensorRef, TensorRef, TensorRef, double)>("hc::layer_norm_ckpt");
     at::AutoDispatchBelowADInplaceOrView guard;
     return op.call(x, gamma, beta, eps);
 }
 Tensors3 act_ckpt_below(TensorRef x, int64_t act) {
-    if (plain_cuda(x)) return activation_gelu_silu_ckpt_cuda(x, act);
     static const auto op = op_handle<Tensors3(TensorRef, int64_t)>("hc::activation_gelu_silu_ckpt");
     at::AutoDispatchBelowADInplaceOrView guard;
     return op.call(x, act);
