@@ -530,24 +530,27 @@ def layer_norm_ckpt(x, gamma, beta, eps: float, stream=None):
     return y, q, scale, rstd
 
 
-def _ln_bwd_outputs(dy, gamma):
+def _ln_bwd_outputs(dy, gamma, stream):
     torch = _torch()
     rows, last = _rows_cols(dy)
     t = LayerNormTiling(rows, last, 0, 0.0)
     size = _sz()
     check(load().hc_layer_norm_bwd_workspace_size(C.byref(t), dtype_code(dy), C.byref(size)))
     work = torch.empty(max(size.value, 1), dtype=torch.uint8, device=dy.device)
+    if stream is not None:  # freed when the call returns, while the kernels on that stream may be yet to run
+        work.record_stream(torch.cuda.ExternalStream(stream, device=dy.device))
     grads = (torch.empty_like(dy), torch.empty_like(gamma), torch.empty_like(gamma))
     return t, work, size, grads
 
 
 def layer_norm_bwd(dy, x, gamma, mean, rstd, stream=None):
-    """(dx, dgamma, dbeta) of the layer norm of x, from layer_norm_fwd_train's statistics."""
+    """(dx, dgamma, dbeta) of the layer norm of x, from layer_norm_fwd_train's statistics.  The outputs belong to the
+    current stream: order it and `stream` around the call, as for the inputs.  The workspace is kept for `stream`."""
     torch = _torch()
     xp = _expect(x, "x", dy.shape, dy.dtype, dy)
     gp = _expect(gamma, "gamma", dy.shape[-1:], torch.float32, dy)
     mp, rp = (_expect(v, n, dy.shape[:-1], torch.float32, dy) for v, n in ((mean, "mean"), (rstd, "rstd")))
-    t, work, size, (dx, dg, db) = _ln_bwd_outputs(dy, gamma)
+    t, work, size, (dx, dg, db) = _ln_bwd_outputs(dy, gamma, stream)
     with _on(dy):
         check(load().hc_layer_norm_bwd_launch(_ptr(dy), xp, gp, mp, rp, _ptr(dx), _ptr(dg), _ptr(db), _ptr(work),
                                               size.value, C.byref(t), dtype_code(dy), _stream(stream)))
@@ -561,7 +564,7 @@ def layer_norm_ckpt_bwd(dy, q, scale, gamma, rstd, stream=None):
     sp = _expect(scale, "scale", _fp8_scale_shape(dy.shape, 1), torch.float32, dy)
     gp = _expect(gamma, "gamma", dy.shape[-1:], torch.float32, dy)
     rp = _expect(rstd, "rstd", dy.shape[:-1], torch.float32, dy)
-    t, work, size, (dx, dg, db) = _ln_bwd_outputs(dy, gamma)
+    t, work, size, (dx, dg, db) = _ln_bwd_outputs(dy, gamma, stream)
     with _on(dy):
         check(load().hc_layer_norm_ckpt_bwd_launch(_ptr(dy), qp, sp, gp, rp, _ptr(dx), _ptr(dg), _ptr(db),
                                                    _ptr(work), size.value, C.byref(t), dtype_code(dy),
