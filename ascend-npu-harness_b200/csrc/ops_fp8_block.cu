@@ -79,7 +79,7 @@ constexpr uint32_t kAnyWarps = kThreads / 32;
 constexpr int kAnyFwd = 2, kAnyBwd = 1;
 
 template <typename T, bool HasAct>
-__global__ void __launch_bounds__(kThreads) block_fwd_kernel(const T* __restrict__ x, T* __restrict__ y,
+__global__ void __launch_bounds__(kThreads) block_fwd_kernel(const T* x, T* __restrict__ y,
                                                              uint8_t* __restrict__ q, float* __restrict__ scale,
                                                              uint32_t blocks, const BlockMap map,
                                                              typename ActOf<T>::Op op) {
@@ -124,8 +124,8 @@ __global__ void __launch_bounds__(kThreads) block_fwd_kernel(const T* __restrict
 
 // Act: the gradient dy * slope(q * scale); otherwise q * scale.
 template <typename T, bool HasAct>
-__global__ void __launch_bounds__(kThreads) block_bwd_kernel(const T* __restrict__ dy, const uint8_t* __restrict__ q,
-                                                             const float* __restrict__ scale, T* __restrict__ out,
+__global__ void __launch_bounds__(kThreads) block_bwd_kernel(const T* dy, const uint8_t* q,
+                                                             const float* scale, T* __restrict__ out,
                                                              uint32_t blocks, const BlockMap map, ActSlope slope) {
     overlap_begin();
     constexpr int kAnyUnroll = kAnyBwd;
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(kThreads) block_bwd_kernel(const T* __restrict
     for (int u = 0; u < kAnyUnroll; ++u) {
         n[u] = 0;
         at[u] = b0 + u < blocks ? map.start(b0 + u, n[u]) + lane : 0;
-        s[u] = __ldg(scale + min(b0 + u, blocks - 1));
+        s[u] = scale[min(b0 + u, blocks - 1)];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const bool in = lane + 32 * i < n[u];
@@ -210,7 +210,7 @@ struct AbsMax {
 };
 
 template <typename T, bool HasAct>
-__global__ void __launch_bounds__(kThreads) block_fwd_vec_kernel(const T* __restrict__ x, T* __restrict__ y,
+__global__ void __launch_bounds__(kThreads) block_fwd_vec_kernel(const T* x, T* __restrict__ y,
                                                                  uint8_t* __restrict__ q, float* __restrict__ scale,
                                                                  uint32_t blocks, const BlockMap map,
                                                                  typename ActOf<T>::Op op) {
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(kThreads) block_fwd_vec_kernel(const T* __rest
         at[u] = b < blocks ? map.start(b, n) + c : 0;
         have[u] = c < n;  // rows are whole packs, so a pack is in or out
         // without a branch around it, so that all loads are issued before the first is used
-        in[u] = ld_stream(reinterpret_cast<const pack<T>*>(x + (have[u] ? at[u] : 0)));
+        in[u] = ld_input_once(reinterpret_cast<const pack<T>*>(x + (have[u] ? at[u] : 0)));
     }
     // The two divisions of each of the group's blocks, all at once: lane 2 u of the group takes
     // 448 / amax of block u, lane 2 u + 1 amax / 448 (eight lanes; every lane computing its own two
@@ -264,8 +264,8 @@ __global__ void __launch_bounds__(kThreads) block_fwd_vec_kernel(const T* __rest
 }
 
 template <typename T, bool HasAct>
-__global__ void __launch_bounds__(kThreads) block_bwd_vec_kernel(const T* __restrict__ dy, const uint8_t* __restrict__ q,
-                                                                 const float* __restrict__ scale, T* __restrict__ out,
+__global__ void __launch_bounds__(kThreads) block_bwd_vec_kernel(const T* dy, const uint8_t* q,
+                                                                 const float* scale, T* __restrict__ out,
                                                                  uint32_t blocks, const BlockMap map,
                                                                  ActSlope slope) {
     overlap_begin();
@@ -284,12 +284,12 @@ __global__ void __launch_bounds__(kThreads) block_bwd_vec_kernel(const T* __rest
         at[u] = b < blocks ? map.start(b, n) + c : 0;
         have[u] = c < n;
         const uint64_t from = have[u] ? at[u] : 0;  // without a branch around them, as in the forward
-        if (HasAct) in[u] = ld_stream(reinterpret_cast<const pack<T>*>(dy + from));
+        if (HasAct) in[u] = ld_input_once(reinterpret_cast<const pack<T>*>(dy + from));
         if (V::P == 8)
-            codes[u] = __ldcs(reinterpret_cast<const uint2*>(q + from));
+            codes[u] = ld_input_once(reinterpret_cast<const uint2*>(q + from));
         else
-            codes[u].x = __ldcs(reinterpret_cast<const uint32_t*>(q + from));
-        s[u] = __ldg(scale + min(b, blocks - 1));
+            codes[u].x = ld_input_once(reinterpret_cast<const uint32_t*>(q + from));
+        s[u] = ld_input(scale + min(b, blocks - 1));
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(kThreads) block_bwd_vec_kernel(const T* __rest
 // from cache.
 // ---------------------------------------------------------------------------------------
 template <typename T>
-__global__ void __launch_bounds__(kThreads) tile_quant_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
+__global__ void __launch_bounds__(kThreads) tile_quant_kernel(const T* x, uint8_t* __restrict__ q,
                                                               float* __restrict__ scale, uint32_t rows, uint32_t cols,
                                                               uint32_t col_tiles, uint64_t tiles) {
     overlap_begin();
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(kThreads) tile_quant_kernel(const T* __restric
         uint32_t m = 0;
         for (uint32_t r = warp; r < nr; r += kThreads / 32)
             for (uint32_t c = lane; c < nc; c += 32)
-                m = max(m, abs_bits(elem<T>::to_f(x[static_cast<uint64_t>(r0 + r) * cols + c0 + c])));
+                m = max(m, abs_bits(elem<T>::to_f(ld_input(x + static_cast<uint64_t>(r0 + r) * cols + c0 + c))));
         m = warp_umax(m);
         if (lane == 0) part[warp] = m;
         __syncthreads();
@@ -338,15 +338,15 @@ __global__ void __launch_bounds__(kThreads) tile_quant_kernel(const T* __restric
         for (uint32_t r = warp; r < nr; r += kThreads / 32)
             for (uint32_t c = lane; c < nc; c += 32) {
                 const uint64_t i = static_cast<uint64_t>(r0 + r) * cols + c0 + c;
-                q[i] = fp8_encode(__fmul_rn(elem<T>::to_f(x[i]), inv));
+                q[i] = fp8_encode(__fmul_rn(elem<T>::to_f(ld_input(x + i)), inv));
             }
         __syncthreads();  // part is rewritten by the next tile
     }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) tile_dequant_kernel(const uint8_t* __restrict__ q,
-                                                                const float* __restrict__ scale, T* __restrict__ x,
+__global__ void __launch_bounds__(kThreads) tile_dequant_kernel(const uint8_t* q,
+                                                                const float* scale, T* __restrict__ x,
                                                                 uint32_t rows, uint32_t cols, uint32_t col_tiles,
                                                                 uint64_t tiles) {
     overlap_begin();
@@ -355,11 +355,11 @@ __global__ void __launch_bounds__(kThreads) tile_dequant_kernel(const uint8_t* _
         const uint32_t r0 = static_cast<uint32_t>(t / col_tiles) * kFp8Block;
         const uint32_t c0 = static_cast<uint32_t>(t % col_tiles) * kFp8Block;
         const uint32_t nr = min(kFp8Block, rows - r0), nc = min(kFp8Block, cols - c0);
-        const float s = scale[t];
+        const float s = ld_input(scale + t);
         for (uint32_t r = warp; r < nr; r += kThreads / 32)
             for (uint32_t c = lane; c < nc; c += 32) {
                 const uint64_t i = static_cast<uint64_t>(r0 + r) * cols + c0 + c;
-                x[i] = elem<T>::from_f(__fmul_rn(fp8_decode(q[i]), s));
+                x[i] = elem<T>::from_f(__fmul_rn(fp8_decode(ld_input(q + i)), s));
             }
     }
 }

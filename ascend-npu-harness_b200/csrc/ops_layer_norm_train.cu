@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kThreads) ln_bwd_cols_any_kernel(const BwdArgs
 // Few partial rows take a quarter of the warps, so that all CTAs run at once (14 x 6976 gradients 6.2 us, with
 // all 32 warps 7.7).
 template <int Warps, uint32_t Parts>
-__global__ void __launch_bounds__(32 * Warps) ln_bwd_join_kernel(const float* __restrict__ parts, uint32_t parts_n, uint32_t H,
+__global__ void __launch_bounds__(32 * Warps) ln_bwd_join_kernel(const float* parts, uint32_t parts_n, uint32_t H,
                                                                  float* __restrict__ dgamma, float* __restrict__ dbeta) {
     __shared__ float sh[Warps][33];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(32 * Warps) ln_bwd_join_kernel(const float* __
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const uint32_t p = warp + i * Warps;
-        v[i] = c < H && p < parts_n ? __ldcg(parts + (static_cast<uint64_t>(p) * 2 + blockIdx.y) * H + c) : 0.f;
+        v[i] = c < H && p < parts_n ? ld_input(parts + (static_cast<uint64_t>(p) * 2 + blockIdx.y) * H + c) : 0.f;
     }
     float s = 0.f;
 #pragma unroll
@@ -291,7 +291,7 @@ struct RowPart {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             if (first(t, i) >= H) continue;
-            if constexpr (Vec) r[i] = __ldcs(reinterpret_cast<const uint4*>(mine + step(i)));
+            if constexpr (Vec) r[i] = ld_input_once(reinterpret_cast<const uint4*>(mine + step(i)));
             else r[i] = mine[step(i)];
         }
     }
@@ -333,12 +333,12 @@ struct RowPart {
 #pragma unroll
                 for (int e = 0; e + 3 < kRun; e += 4)
                     *reinterpret_cast<float4*>(f + i * kRun + e) = first(t, i) < H
-                        ? __ldg(reinterpret_cast<const float4*>(p + first(t, i) + e)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        ? ld_input(reinterpret_cast<const float4*>(p + first(t, i) + e)) : make_float4(0.f, 0.f, 0.f, 0.f);
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i)
 #pragma unroll
-                for (int e = 0; e < kRun; ++e) f[i * kRun + e] = first(t, i) < H ? __ldg(p + first(t, i) + e) : 0.f;
+                for (int e = 0; e < kRun; ++e) f[i * kRun + e] = first(t, i) < H ? ld_input(p + first(t, i) + e) : 0.f;
         }
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) v[i] = make_float2(f[2 * i], f[2 * i + 1]);
@@ -644,7 +644,7 @@ struct CkptPart {
     __device__ __forceinline__ void load(const uint8_t* q, const float* scale, uint32_t t, uint32_t H) {
         // a warp's 32 neighbouring columns lie in one block
         const uint32_t c0 = t / 32 * 32 + 32 * W * (t % 32);
-        if (c0 < H && t % 32 < N) s[0] = __ldg(scale + c0 / kFp8Block);
+        if (c0 < H && t % 32 < N) s[0] = ld_input(scale + c0 / kFp8Block);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const uint32_t c = t + 32 * W * i;
@@ -726,8 +726,8 @@ __global__ void __launch_bounds__(group_threads(W), bwd_ctas(W, Vec)) ln_bwd_row
     };
     auto fetch = [&](uint64_t r) {  // what is held for the next row
         if constexpr (kAhead) fetch_row(r);
-        if constexpr (!Ckpt) mean_next = __ldg(a.mean + r);
-        rstd_next = __ldg(a.rstd + r);
+        if constexpr (!Ckpt) mean_next = ld_input(a.mean + r);
+        rstd_next = ld_input(a.rstd + r);
     };
     uint32_t stage = 0;  // byte offset of the current row's stage
     if constexpr (Vec) {

@@ -333,8 +333,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     float va[kLoads];
 #pragma unroll
                     for (uint32_t i = 0; i < kLoads; ++i)
-                        va[i] = __ldg(p.a_scale + static_cast<uint64_t>(min(row + kRows * i, p.M - 1)) * p.kb + kk);
-                    const float b0 = __ldg(sb0 + kk), b1 = __ldg(sb1 + kk);
+                        va[i] = ld_input(p.a_scale + static_cast<uint64_t>(min(row + kRows * i, p.M - 1)) * p.kb + kk);
+                    const float b0 = ld_input(sb0 + kk), b1 = ld_input(sb1 + kk);
                     ok = mbar_wait_bounded(&bars->sc_empty[sg & 1], ((sg >> 1) & 1) ^ 1, abort_flag, &g_mm8_error_word,
                                            kErrScale);
                     ok = __all_sync(0xffffffffu, ok);
@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(Few<TN>::kThreads, Few<TN>::kPerSm)
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
             const uint32_t k = min(kb0 + i, kb1 - 1);
-            next[i] = tid < TN ? __ldg(sa + k) * __ldg(sb + k) : 0.f;
+            next[i] = tid < TN ? ld_input(sa + k) * ld_input(sb + k) : 0.f;
         }
         uint32_t g = 0;
         for (uint32_t kb = kb0; kb < kb1; ++kb, ++g) {
@@ -579,7 +579,7 @@ __global__ void __launch_bounds__(Few<TN>::kThreads, Few<TN>::kPerSm)
                     for (uint32_t i = 0; i < 4; ++i) {
                         prod[((g & 4) + i) * TN + tid] = next[i];
                         const uint32_t k = min(kb + 4 + i, kb1 - 1);
-                        next[i] = __ldg(sa + k) * __ldg(sb + k);
+                        next[i] = ld_input(sa + k) * ld_input(sb + k);
                     }
                 }
                 // the promoting warps alone; two groups are enough, since a warp that still reads the one
