@@ -401,11 +401,18 @@ def _expect(t, what: str, shape, dtype, like):
     return _ptr(t)
 
 
+def _sizes(*sizes):
+    """Sizes for the 32-bit fields of a tiling record, which would keep their low bits only."""
+    if max(sizes) > 0x7FFFFFFF:
+        raise HcError(HC_ERR_UNSUPPORTED, f"sizes over 2^31 - 1: {sizes}")
+    return sizes
+
+
 def _rows_cols(x):
     if x.dim() < 1:
         raise HcError(HC_ERR_INVALID, "expected at least one dimension")
     cols = x.shape[-1]
-    return (x.numel() // cols if cols else 0), cols
+    return _sizes(x.numel() // cols if cols else 0, cols)
 
 
 def _fp8_scale_shape(shape, block_rows: int):
@@ -467,7 +474,7 @@ def matmul_fp8_block(a, a_scale, b, b_scale, bias=None, dtype=None, stream=None)
     bsp = _expect(b_scale, "b_scale", _fp8_scale_shape((N, K), FP8_BLOCK), torch.float32, a)
     biasp = None if bias is None else _expect(bias, "bias", (N,), dtype, a)
     c = torch.empty((M, N), dtype=dtype, device=a.device)
-    t = MatmulFp8BlockTiling(M, K, N)
+    t = MatmulFp8BlockTiling(*_sizes(M, K, N))
     with _on(a):
         check(load().hc_matmul_fp8_block_launch(ap, asp, bp, bsp, biasp, _ptr(c), C.byref(t), dtype_code(c),
                                                 _stream(stream)))
