@@ -744,13 +744,19 @@ uint32_t read_error_word(const char** name) {
 
 thread_local int t_last_path = 0;
 
+// The launch's status; its path is noted if it succeeded.
+int launched(int path, const char* name) {
+    const int rc = check_launch(name);
+    if (rc == HC_OK) t_last_path = path;
+    return rc;
+}
+
 template <typename T>
 int launch_simt(const Params& p, cudaStream_t s) {
     const uint64_t mt = (static_cast<uint64_t>(p.M) + 63) / 64;
     const dim3 grid(static_cast<unsigned>((static_cast<uint64_t>(p.N) + 63) / 64), mt < 65535 ? static_cast<unsigned>(mt) : 65535);
     launch_overlapped(mm8_simt_kernel<T>, grid, 256, 0, 0, s, p);
-    t_last_path = 2;
-    return check_launch("mm8_simt_kernel");
+    return launched(2, "mm8_simt_kernel");
 }
 
 int operand_map(CUtensorMap* out, const uint8_t* base, uint32_t rows, uint32_t K, uint32_t box_rows) {
@@ -798,8 +804,7 @@ int launch_pair(Params p, int pairs, cudaStream_t s) {
     if (int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(k), kPairSmem, "mm8_pair_kernel")) return rc;
     const uint32_t clusters = static_cast<uint32_t>(pairs) < p.num_tiles ? static_cast<uint32_t>(pairs) : p.num_tiles;
     launch_overlapped(k, 2 * clusters, kPairThreads, kPairSmem, 0, s, tma, tmb, p);
-    t_last_path = 3;
-    return check_launch("mm8_pair_kernel");
+    return launched(3, "mm8_pair_kernel");
 }
 
 // Clusters of `c` CTAs of the few-token kernel that the current device holds at once (cached per device):
@@ -885,8 +890,7 @@ int launch_few(const Params& p, cudaStream_t s) {
     const uint32_t splits = few_plan<T, TN>(p).splits;
     launch_overlapped(k, dim3(splits, p.nb, (p.M + TN - 1) / TN), Few<TN>::kThreads, Few<TN>::kSmem, splits, s, tma, tmb, p,
                       splits);
-    t_last_path = 1;
-    return check_launch("mm8_few_kernel");
+    return launched(1, "mm8_few_kernel");
 }
 
 constexpr uint64_t kL2Weight = 64ull << 20;  // half of the L2

@@ -198,3 +198,23 @@ def test_plain_quantize_format():
     assert bool(R.values(q, s).isnan().all())
     q, s = R.quantize_rows(torch.tensor([[1.0, float("inf")]]))
     assert bool(R.values(q, s).isnan().all())
+
+
+@pytest.mark.parametrize("K", [33, 128])
+def test_failed_launch_leaves_the_path(lib, K):
+    """hc_matmul_fp8_block_last_path() tells of successful launches; a thread of its own starts with none.  Without a
+    GPU the launch fails; with one, an output type that the product does not have is refused before it."""
+    import threading
+
+    seen = []
+
+    def call():
+        t = hc.MatmulFp8BlockTiling(4, K, 16)
+        dtype = 9 if torch.cuda.is_available() else 2
+        seen.append(lib.hc_matmul_fp8_block_launch(FAKE, FAKE, FAKE, FAKE, None, FAKE, C.byref(t), dtype, None))
+        seen.append(lib.hc_matmul_fp8_block_last_path())
+
+    thread = threading.Thread(target=call)
+    thread.start()
+    thread.join()
+    assert seen[0] != hc.HC_OK and seen[1] == 0
