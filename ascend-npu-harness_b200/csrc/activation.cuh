@@ -36,11 +36,11 @@ struct ActOp {
 // With the constants folded into the base-2 exponent, both are x / (1 + 2^y), y = -x (a + b x^2):
 // GELU a = 2 sqrt(2/pi) log2 e, b = 0.044715 a; SiLU a = log2 e, b = 0.  Relative error ~1e-6, far
 // below the rounding of the bf16/fp16 result (2^-9 / 2^-12); the fp32 path (ActOp) keeps the
-// golden's operation order.  y is held to 127: there 1 + 2^y is finite and its reciprocal, below the
-// smallest normal number, is flushed to 0, so a finite x far below zero gives -0 however large it is,
-// as the golden does (a reciprocal of 2^-126 would leave -3.5 of -3e38).  From y = 126 to 127 the
-// flush takes less than |x| 2^-126 off the result; -inf * 0 is NaN, in the golden, too.  x^2 is held to
-// 256 (at |x| = 16 GELU's y is past 127; SiLU makes no use of it): an infinite one times SiLU's b = 0 is NaN.
+// golden's operation order.  Far below zero 2^y becomes infinite and its reciprocal 0 (from y = 126 on, where it
+// would be below the smallest normal number, it is flushed to 0, which takes less than |x| 2^-126 off
+// the result): a finite x gives -0 however large it is, as the golden does, and -inf * 0 is NaN, there, too.
+// x^2 is held to 256 (at |x| = 16 GELU's y is past 127; SiLU makes no use of it): an infinite one times SiLU's
+// b = 0 is NaN.
 __device__ __forceinline__ float ex2_ftz(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -66,8 +66,7 @@ struct FastActOp {
         x2 = make_float2(fminf(x2.x, 256.f), fminf(x2.y, 256.f));
         const float2 w = __ffma2_rn(make_float2(-b, -b), x2, make_float2(-a, -a));
         const float2 y = __fmul2_rn(x, w);
-        float2 d = make_float2(ex2_ftz(fminf(y.x, 127.f)), ex2_ftz(fminf(y.y, 127.f)));
-        d = __fadd2_rn(d, make_float2(1.f, 1.f));
+        const float2 d = __fadd2_rn(make_float2(ex2_ftz(y.x), ex2_ftz(y.y)), make_float2(1.f, 1.f));
         // MUFU rcp: measured faster here than three Newton steps on the FMA pipe
         return __fmul2_rn(x, make_float2(rcp_ftz(d.x), rcp_ftz(d.y)));
     }
