@@ -16,15 +16,17 @@
 //
 // Both directions are HBM streams: the forward moves 2 e bytes per element (e = element size) and 1 + 1/32 more
 // for the checkpoint, the backward 3 e, or 2 e + 1 + 1/32 from the checkpoint.  Measured on one B200, copy rate 6.56 TB/s:
-//   [16384, 4096] bf16   forward 51 us (5.3 TB/s, 80 %), gradients 72.5 us (5.6 TB/s, the join of the partial
+//   [16384, 4096] bf16   forward 50 us (5.4 TB/s, 82 %), gradients 72 us (5.6 TB/s, the join of the partial
 //                        sums included)
-//   [8192, 4096] fp32    forward 44 us (6.1 TB/s), gradients 65 us (6.2 TB/s)
-//   [8192, 8192] bf16    with the checkpoint: forward 72 us, gradients 76 us (4.5 TB/s)
-//   [8192, 4001] bf16    (rows that are not whole packs) forward 43 us, gradients 72 us (2.7 TB/s); with the
-//                        checkpoint 63 and 70 us
-// The [16384, 4096] gradients' own kernel takes 68 us (5.9 TB/s, 90 %).  The other 16-bit rows are bound by issue slots
-// and shared-memory traffic per element (issue 46-58 % active, 14-17 warp instructions per 32 elements), not
-// by DRAM: fp32 rows, with half the elements per byte, run at 94 %.
+//   [8192, 4096] fp32    forward 44 us (6.1 TB/s), gradients 65 us (6.2 TB/s); with the checkpoint 50 (6.1 TB/s) and 66
+//   [8192, 8192] bf16    with the checkpoint: forward 72 us, gradients 75 us (4.5 TB/s)
+//   [8192, 4001] bf16    (rows that are not whole packs) forward 40 us, gradients 65 us (3.0 TB/s); with the
+//                        checkpoint 63 and 68 us
+//   [4096, 12288] bf16   (over 8192 columns) forward 117 us, gradients 301 us; with the checkpoint 143 and 313 us
+// The [16384, 4096] gradients' own kernel takes 68 us (5.9 TB/s, 90 %).  The other 16-bit rows wait within a row: for
+// shuffles and shared memory, and at the barrier that joins its warps (forward: short scoreboard 2.0, barrier 0.9
+// stalled warps per issue; 64 % of the issue slots used, with 16 warps per row 51 %).  fp32 rows, with half the elements
+// per byte, run at 94 %.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -447,9 +449,9 @@ __device__ __forceinline__ float2 row_sum2(float2 v, float2* sh, uint32_t group,
 }
 
 // Rows loaded one element at a time: whether the next row is held in registers, which leaves room for
-// one CTA per SM without spills; otherwise two, which wait for each row.  x form, bf16: [16384, 2001] 76 us with, 109
-// without; [32768, 1001] 74 and 89; [8192, 4001] 100 and 72; [4096, 7777] 97 and 90.  Checkpoint: 77 and 120 at
-// [16384, 2001], 97 and 70 at [8192, 4001].
+// one CTA per SM without spills; otherwise two, which wait for each row.  x form, bf16: [16384, 2001] 74 us with, 104
+// without; [32768, 1001] 73 and 84; [8192, 4001] 97 and 65; [4096, 7777] 96 and 84.  Checkpoint: 77 and 120 at
+// [16384, 2001], 94 and 68 at [8192, 4001].
 constexpr bool bwd_ahead(int W) { return W <= 4; }
 constexpr int bwd_ctas(int W, bool vec) { return W > 8 || (!vec && bwd_ahead(W)) ? 1 : 2; }
 template <typename T, int W, bool Ckpt>
@@ -465,9 +467,10 @@ __device__ __forceinline__ float lanes_sum(float v) {
 
 // CTAs per SM that the registers are divided for.  Rows loaded one element at a time hold the next row in
 // 16 registers instead of 8 and spilled with three ([8192, 4001] bf16: 55 us with three, 43 with two).  Packs of fp32 and
-// the checkpoint spill up to 156 bytes with three, and two are better up to four warps ([8192, 2048] bf16 with the
-// checkpoint 18.9 us, with three 19.4; fp32 27.2 and 33.2, without it 24.6 and 25.7), not with eight ([8192, 3584] 42.5
-// fp32 with two, 38.9 with three) or one ([16384, 512] bf16 10.6 and 10.5).
+// the checkpoint spill up to 156 bytes with three, and for two and four warps two are better ([8192, 2048] bf16 with
+// the checkpoint 18.9 us, with three 19.4; fp32 27.2 and 33.2, without it 24.6 and 25.7), not for eight ([8192, 3584]
+// fp32 42.5 with two, 38.9 with three).  What is left with three spills 4-12 bytes, and fp32 rows of one warp 36, with
+// the checkpoint 164.
 constexpr int fwd_ctas(int W, bool vec, bool ckpt, size_t bytes) {
     return W > 8 ? 1 : !vec || ((ckpt || bytes == 4) && (W == 2 || W == 4)) ? 2 : 3;
 }

@@ -15,7 +15,7 @@
 //   * otherwise the weight as the 128-row operand and up to 128 tokens as the columns, K split over
 //     a thread-block cluster whose CTAs join their sums through distributed shared memory.
 // SIMT path for the rest: 64x64 output tiles, 16x16 threads, 4x4 outputs per thread; codes are scaled
-// to fp32 as they are staged (one more fp32 rounding per operand).
+// to fp32 as they are staged (one more fp32 rounding per operand).  300 x 260 x 1001: 122 us.
 // Waits are bounded as in the other tensor-core kernels.
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -410,10 +410,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 // ======================================================================================
 // Few tokens: the transposed product.  A CTA takes 128 rows of the weight as the M operand, TN tokens
 // as the N operand and every S-th run of K blocks; the S CTAs of a cluster then add their sums in
-// rank order through distributed shared memory.  Reading the weight is the work (N K bytes), so S is
-// chosen to give every SM a part of it, and the ring holds all that fits beside a second CTA.
+// rank order through distributed shared memory.  Reading the weight is the work (N K bytes); few_plan()
+// chooses S.  Up to 64 tokens the ring holds all that fits beside a second CTA, with more it takes an SM's memory.
 // 1 x 4096 x 4096: 6.2 us with the weight in hand after 3.6 (6.8 TB/s once loads run; 1.2 us to the first
-// block, 2 us for the join); 1 x 8192 x 8192: 17 us (67 MB, 4.0 TB/s); 77 x 10001 x 2064: 13 us.
+// block, 2 us for the join); 1 x 8192 x 8192: 16.3 us (67 MB, 4.1 TB/s; S = 2 gives 128 CTAs, one on each of
+// 128 SMs); 77 x 10001 x 2064: 12.5 us.
 //   warp 0      TMA producer: 16 KB of weight and TN x 128 bytes of tokens per K block
 //   warp 1      issues M=128, N=TN, K=32 MMAs into one of kAcc accumulators of TN columns
 //   warps 2 on  promotion, kEpi = 4 or 8 warps: thread = weight row (TMEM lane), kCols of the tokens:
@@ -849,7 +850,8 @@ uint32_t few_clusters(uint32_t c) {
 
 // Splits of K: the least time in K blocks (about 0.4 us each) of the busiest SM, with what a wave of
 // clusters costs besides: some three blocks to start, and to join the sums two more, five with over
-// 64 tokens.
+// 64 tokens.  A block counts the same whether one or two CTAs share the SM, so of equal counts the fewer
+// splits are taken.
 struct FewPlan {
     uint32_t splits;
     uint64_t cost;

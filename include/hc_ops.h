@@ -351,7 +351,9 @@ int hc_activation_gelu_silu_ckpt_bwd_launch(const void* dy, const void* q, const
 
 /* The layer norm of x [rows, lastDim] with the statistics its backward needs: y, mean [rows] (may
  * be NULL) and rstd [rows] = 1 / sqrt(var + eps), fp32.  With q and q_scale (both or neither) the
- * normalised rows (x - mean) * rstd are also kept in 8-bit blocks (blockRows 1). */
+ * normalised rows (x - mean) * rstd are also kept in 8-bit blocks (blockRows 1).  y and the kept rows are
+ * formed from the mean before it is rounded to fp32.  A finite row whose squares pass the largest
+ * fp32 has rstd 0 and y = beta. */
 int hc_layer_norm_fwd_train_launch(const void* x, const float* gamma, const float* beta, void* y, float* mean,
                                    float* rstd, void* q, float* q_scale, const struct layer_norm_tiling_data* t,
                                    int dtype, void* stream);
@@ -359,6 +361,8 @@ int hc_layer_norm_fwd_train_launch(const void* x, const float* gamma, const floa
 /* Gradients of the layer norm: dx [rows, lastDim] (of x's type), dgamma and dbeta [lastDim] fp32.
  * With xh = (x - mean) * rstd and g = dy * gamma:
  *     dx = rstd * (g - mean(g) - xh * mean(g * xh)), dgamma = sum_rows dy * xh, dbeta = sum_rows dy.
+ * `mean` is given in fp32, so this xh is off by up to |mean| * rstd * 2^-24; the checkpointed form below
+ * has no such term.
  * No rows: dgamma and dbeta are zero.  `workspace` (16-byte aligned, at least
  * hc_layer_norm_bwd_workspace_size() bytes, contents irrelevant) holds partial sums between the
  * launches of one call: calls that may overlap in time need one each.  The sums are added in a
