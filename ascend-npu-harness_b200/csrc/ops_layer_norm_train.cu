@@ -477,7 +477,8 @@ constexpr int fwd_ctas(int W, bool vec, bool ckpt, size_t bytes) {
 
 // Statistics: each warp takes the mean m_w of the first half of its n_w columns (over deviations from its first one), and
 // the sums r_w and M2_w of all its columns' deviations from that and of their squares, with shuffles alone.  Half of the
-// columns will do, since r_w makes up for the difference.  The row's follow from the W triples behind one barrier, relative to the first warp's m_0:
+// columns will do, since r_w makes up for the difference.  The row's follow from the W triples behind one barrier,
+// relative to the first warp's m_0:
 //   d_w = m_w - m_0, delta = sum_w (n_w d_w + r_w) / H, mean = m_0 + delta, x - mean = (x - m_w) + (d_w - delta),
 //   M2 = sum_w (M2_w + d_w (n_w d_w + 2 r_w)) - H delta^2,
 // two sums that need not wait for one another.  What cancels in M2 is at most H / 256 of it (m_0 is the mean of 256

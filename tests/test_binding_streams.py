@@ -80,3 +80,6 @@ def test_backward_on_a_busy_stream(cuda, ckpt):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         assert all(bool((o == 7.0).all()) for o in others)
+    got = call(0)  # the default stream by its handle
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
